@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/sonar_marlin.h.
+"""ctypes binding of the C ABIs in include/sonar_marlin.h and include/sonar_layer.h.
 
 Loading fails loudly when the HIP library has not been built: there is no
 fallback path."""
@@ -9,6 +9,7 @@ import os
 from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_marlin.so")
+_LAYER_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_layer.so")
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -118,7 +119,21 @@ PROTOTYPES = {
     "sonar_moe_sum": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p]),
 }
 
+# the same for include/sonar_layer.h
+LAYER_PROTOTYPES = {
+    "sonar_layer_last_error": (c_char_p, []),
+    "sonar_rms_norm_per_token_quant": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                               c_int, c_void_p, c_int, c_int64, c_int64, c_double, c_void_p]),
+    "sonar_scaled_mm_int8_scratch_bytes": (c_size_t, [c_int64] * 3),
+    "sonar_scaled_mm_int8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                     c_void_p, c_void_p, c_size_t, c_int, c_int64, c_int64, c_int64, c_void_p]),
+    "sonar_topk_routing": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                   c_int, c_int64, c_int64, c_double, c_void_p]),
+}
+SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
+
 _lib = None
+_layer = None
 
 
 class SonarMarlinError(RuntimeError):
@@ -131,26 +146,45 @@ def lib_path() -> str:
     return _LIB_PATH
 
 
-def load() -> ctypes.CDLL:
-    global _lib
-    if _lib is not None:
-        return _lib
-    if not os.path.exists(_LIB_PATH):
+def _open(path: str, prototypes) -> ctypes.CDLL:
+    if not os.path.exists(path):
         raise ImportError(
-            f"{_LIB_PATH} is missing: build it with `python -m sonar_amd.build` "
+            f"{path} is missing: build it with `python -m sonar_amd.build` "
             "(hipcc --offload-arch=gfx950); there is no fallback implementation")
-    lib = ctypes.CDLL(_LIB_PATH)
-    for name, (restype, argtypes) in PROTOTYPES.items():
+    lib = ctypes.CDLL(path)
+    for name, (restype, argtypes) in prototypes.items():
         fn = getattr(lib, name)  # AttributeError if the library does not export it
         fn.restype = restype
         fn.argtypes = argtypes
-    _lib = lib
     return lib
+
+
+def load() -> ctypes.CDLL:
+    global _lib
+    if _lib is None:
+        _lib = _open(_LIB_PATH, PROTOTYPES)
+    return _lib
+
+
+def load_layer() -> ctypes.CDLL:
+    global _layer
+    if _layer is None:
+        _layer = _open(_LAYER_PATH, LAYER_PROTOTYPES)
+    return _layer
+
+
+def _raise(rc: int, msg: bytes) -> None:
+    text = msg.decode("utf-8", "replace")
+    if rc == E_UNSUPPORTED:
+        raise NotImplementedError(text)
+    raise SonarMarlinError(rc, text)
 
 
 def check(rc: int) -> None:
     if rc != OK:
-        msg = load().sonar_marlin_last_error().decode("utf-8", "replace")
-        if rc == E_UNSUPPORTED:
-            raise NotImplementedError(msg)
-        raise SonarMarlinError(rc, msg)
+        _raise(rc, load().sonar_marlin_last_error())
+
+
+def check_layer(rc: int) -> None:
+    if rc != OK:
+        _raise(rc, load_layer().sonar_layer_last_error())

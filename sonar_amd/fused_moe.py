@@ -34,6 +34,72 @@ def moe_block_size(num_tokens: int, top_k: int, num_experts: int) -> int:
     return block_size_m
 
 
+def _topk_routing_torch(logits, topk, scoring_func, renormalize, bias, groups, kept_groups, factor):
+    """ops.topk_routing as torch expressions (any device), in 64 bits."""
+    tokens, experts = logits.shape
+    x = logits.to(torch.float64)
+    x = torch.where(x.isnan(), -math.inf, x)
+    if scoring_func == "sigmoid":
+        scores = torch.sigmoid(x)
+    else:
+        top = x.amax(dim=-1, keepdim=True)
+        e = torch.where(x == top, torch.ones_like(x), torch.exp(x - top))
+        e = torch.where(x == -math.inf, torch.zeros_like(x), e)
+        total = e.sum(dim=-1, keepdim=True)
+        scores = e / torch.where(total > 0, total, torch.ones_like(total))
+    choice = x if bias is None else scores + bias.to(torch.float64)
+    choice = torch.where(choice.isnan(), -math.inf, choice)
+    order = torch.sort(choice, dim=-1, descending=True, stable=True).indices
+    if groups > 1:   # experts outside the kept groups go behind all others
+        size = experts // groups
+        best = torch.topk(choice.view(tokens, groups, size), 1 if bias is None else min(2, size), dim=-1).values.sum(dim=-1)
+        best = torch.where(best.isnan(), -math.inf, best)
+        kept = torch.sort(best, dim=-1, descending=True, stable=True).indices[:, :kept_groups]
+        outside = torch.ones((tokens, groups), dtype=torch.int8, device=x.device).scatter_(1, kept, 0)
+        order = order.gather(1, torch.sort(outside.gather(1, order // size), dim=-1, stable=True).indices)
+    ids = order[:, :topk]
+    w = scores.gather(1, ids)
+    if renormalize:
+        total = w.sum(dim=-1, keepdim=True)
+        w = w / torch.where(total > 0, total, torch.ones_like(total))
+    return (w * factor).to(torch.float32), ids.to(torch.int32)
+
+
+def _route(hidden_states, logits, topk, scoring_func, renormalize, bias, groups, kept_groups, factor):
+    assert hidden_states.size(0) == logits.size(0), "Number of tokens mismatch"
+    if scoring_func not in ("softmax", "sigmoid"):
+        raise ValueError(f"Unsupported scoring function: {scoring_func}")
+    experts = logits.shape[1]
+    if groups < 1 or experts % groups or not 1 <= kept_groups <= groups:
+        raise ValueError(f"{groups} groups, {kept_groups} of them kept, do not fit {experts} experts")
+    if not 1 <= topk <= kept_groups * (experts // groups):
+        raise ValueError(f"topk = {topk} of {kept_groups * (experts // groups)} experts")
+    if bias is not None:
+        bias = bias.to(torch.float32)
+    if logits.is_cuda:
+        return ops.topk_routing(logits, topk, scoring_func, renormalize, bias, groups, kept_groups, factor)
+    return _topk_routing_torch(logits, topk, scoring_func, renormalize, bias, groups, kept_groups, factor)
+
+
+def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor, topk: int, renormalize: bool,
+               scoring_func: str = "softmax", e_score_correction_bias: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The router in front of `fused_marlin_moe`: (topk_weights float32, topk_ids int32), both (tokens, topk), from the
+    logits (tokens, experts).  The reference's fused_topk and, with e_score_correction_bias, fused_topk_bias, without the
+    table of slots that its kernel leaves beside them.  ops.topk_routing says what is computed."""
+    return _route(hidden_states, gating_output, topk, scoring_func, renormalize, e_score_correction_bias, 1, 1, 1.0)
+
+
+def grouped_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor, topk: int, renormalize: bool,
+                 num_expert_group: int = 1, topk_group: int = 1, scoring_func: str = "softmax",
+                 routed_scaling_factor: float = 1.0, e_score_correction_bias: torch.Tensor | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The router of models whose experts come in groups (the reference's grouped_topk): only experts of the topk_group
+    best of num_expert_group groups may be chosen.  ops.topk_routing says what is computed."""
+    return _route(hidden_states, gating_output, topk, scoring_func, renormalize, e_score_correction_bias, num_expert_group,
+                  topk_group, routed_scaling_factor)
+
+
 def moe_align_block_size(topk_ids: torch.Tensor, block_size: int, num_experts: int,
                          expert_map: torch.Tensor | None = None, pad_sorted_ids: bool = False,
                          ignore_invalid_experts: bool = False

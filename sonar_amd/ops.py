@@ -12,15 +12,20 @@ from . import _lib
 from .scalar_type import ScalarType
 
 _OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_marlin_torch.so")
+_LAYER_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_layer_torch.so")
 
 
 def _load_ops() -> None:
-    if hasattr(torch.ops._C, "marlin_gemm") and hasattr(torch.ops._C, "marlin_to_gfx950"):
-        return
-    _lib.load()  # raises with build instructions when the HIP library is missing
-    if not os.path.exists(_OPS_PATH):
-        raise ImportError(f"{_OPS_PATH} is missing: build it with `python -m sonar_amd.build`")
-    torch.ops.load_library(_OPS_PATH)
+    def load(library, path):
+        library()  # raises with build instructions when the HIP library is missing
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `python -m sonar_amd.build`")
+        torch.ops.load_library(path)
+
+    if not (hasattr(torch.ops._C, "marlin_gemm") and hasattr(torch.ops._C, "marlin_to_gfx950")):
+        load(_lib.load, _OPS_PATH)
+    if not hasattr(torch.ops.sonar_amd, "scaled_mm_int8"):
+        load(_lib.load_layer, _LAYER_OPS_PATH)
 
 
 _load_ops()
@@ -60,6 +65,24 @@ def _register_fakes() -> None:
 
     reg("sonar_amd::per_token_quant_int8")(quant_fake(torch.int8))
     reg("sonar_amd::per_token_quant_fp8")(quant_fake(torch.float8_e4m3fn))
+
+    @reg("sonar_amd::rms_norm_per_token_quant")
+    def _(x, weight, residual, epsilon, quant_dtype, with_norm):
+        q, scales = quant_fake(quant_dtype)(x)
+
+        def like_x(wanted):   # the op answers contiguous tensors
+            return torch.empty(x.shape if wanted else (0,), dtype=x.dtype, device=x.device)
+        return q, scales, like_x(residual is not None), like_x(with_norm)
+
+    @reg("sonar_amd::scaled_mm_int8")
+    def _(a, b, a_scales, b_scales, out_dtype, bias):
+        return torch.empty(a.shape[:-1] + (b.shape[1],), dtype=out_dtype, device=a.device)
+
+    @reg("sonar_amd::topk_routing")
+    def _(logits, topk, scoring_func, renormalize, bias, num_expert_group, topk_group, routed_scaling_factor):
+        shape = (logits.shape[0], topk)
+        return (torch.empty(shape, dtype=torch.float32, device=logits.device),
+                torch.empty(shape, dtype=torch.int32, device=logits.device))
 
     @reg("sonar_amd::gptq_marlin_moe_repack")
     def _(b_q_weight, perm, size_k, size_n):
@@ -191,6 +214,51 @@ def per_token_quant_fp8(x: torch.Tensor):
     """Dynamic per-token float8_e4m3fn quantisation (QuantFP8(False, GroupShape.PER_TOKEN),
     layers/quantization/input_quant_fp8.py:188-204): scale = max(absmax / 448, 1 / (448 * 512))."""
     return torch.ops.sonar_amd.per_token_quant_fp8(x)
+
+
+def rms_norm_per_token_quant(x: torch.Tensor, weight: torch.Tensor, epsilon: float,
+                             quant_dtype: torch.dtype = torch.int8, residual: torch.Tensor | None = None,
+                             with_norm: bool = False):
+    """Root-mean-square norm of the rows of x (float16, bfloat16, float32), with the residual's addition before it and
+    8-bit codes with one scale a row behind it, in one launch (the reference's rms_norm_dynamic_per_token_quant):
+
+      z = x + residual, rounded to x's type;  y = z / sqrt(mean(z^2) + epsilon) * weight in float32
+
+    Returns (codes, scales, z, norm): the codes (quant_dtype: int8 or float8_e4m3fn, of x's shape) and float32 scales
+    (..., 1) of y as per_token_quant_int8 / _fp8 make them, what `marlin_gemm` and `scaled_mm_int8` take as `a` and
+    `a_scales`; z where a residual was given, the next residual, else None; y rounded to x's type where `with_norm`
+    (for a router, which reads 16 bits), else None.  The codes are those of y itself, not of the rounded norm.
+    A row with an infinity or a NaN in z has the scale NaN."""
+    q, scales, z, norm = torch.ops.sonar_amd.rms_norm_per_token_quant(x, weight, residual, epsilon, quant_dtype, with_norm)
+    return q, scales, z if residual is not None else None, norm if with_norm else None
+
+
+def scaled_mm_int8(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: torch.Tensor,
+                   out_dtype: torch.dtype, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """Product of 8-bit integers with a scale for each token and channel (W8A8; the reference's cutlass_scaled_mm with
+    int8 operands):  out = out_dtype((a @ b) * (a_scales * b_scales) + bias), the sum in 32-bit integers.
+
+    a: int8 (..., K).  b: int8 (K, N), column by column: `weight.t()` of a checkpoint's (N, K) weight, read as it lies.
+    a_scales: float32, one a token or one in all; b_scales: one a channel or one in all.  out_dtype: float16 or
+    bfloat16; bias: (N,) of out_dtype.  K below 131072, where the sum could leave 32 bits."""
+    return torch.ops.sonar_amd.scaled_mm_int8(a, b, a_scales, b_scales, out_dtype, bias)
+
+
+def topk_routing(gating_output: torch.Tensor, topk: int, scoring_func: str = "softmax", renormalize: bool = False,
+                 bias: torch.Tensor | None = None, num_expert_group: int = 1, topk_group: int = 1,
+                 routed_scaling_factor: float = 1.0):
+    """The experts of each token and their weights: (topk_weights float32, topk_ids int32), both (tokens, topk), as
+    `fused_marlin_moe` takes them.  gating_output: the router's logits (tokens, experts), float16, bfloat16 or float32.
+
+    Scores are softmax(logits) or sigmoid(logits) (`scoring_func`); experts are chosen by score + bias (float32,
+    (experts,); the bias balances loads and is no part of a weight), in falling order, equal ones by the lower number.
+    With num_expert_group > 1 neighbouring experts form groups, and only those of the topk_group best groups may be
+    chosen; a group counts by its best expert or, with a bias, by the sum of its two best.  The weights are the scores of
+    the chosen, divided by their sum if `renormalize`, times routed_scaling_factor.  A NaN logit counts as -inf; a token
+    whose logits are all -inf gets the lowest experts that may be chosen, with softmax weights 0.  At most 1024 experts,
+    64 groups, 64 choices."""
+    return torch.ops.sonar_amd.topk_routing(gating_output, topk, scoring_func, renormalize, bias, num_expert_group,
+                                            topk_group, routed_scaling_factor)
 
 
 def marlin_gemm(a: torch.Tensor, c: torch.Tensor | None, b_q_weight: torch.Tensor,
