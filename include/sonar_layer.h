@@ -51,10 +51,12 @@ int sonar_rms_norm_per_token_quant(const void* x, int64_t x_row_stride, const vo
  *   c         dtype[size_m][size_n] (SONAR_DTYPE_F16 / _BF16)
  *   a_scales  float[a_scales_len], a_scales_len 1 or size_m; b_scales likewise, 1 or size_n
  *   bias      dtype[size_n] or NULL
- *   scratch   device memory, 16-byte aligned, of sonar_scaled_mm_int8_scratch_bytes(...) bytes (may be 0) for partial
- *             sums; a smaller or no scratch is allowed and splits K less or not at all.  Calls that overlap in time
- *             need scratches of their own. */
-size_t sonar_scaled_mm_int8_scratch_bytes(int64_t size_m, int64_t size_n, int64_t size_k);
+ *   scratch   device memory, 16-byte aligned, of sonar_scaled_mm_int8_scratch_bytes(...) bytes (may be 0): partial sums
+ *             where K is split, aligned copies of rows that are not.  A smaller one or none is allowed and slower, with the
+ *             same results.  Calls that overlap in time need scratches of their own.
+ *   aligned   whether a, b and both row strides are multiples of 16 bytes, the strides below 2^23
+ * size_m and size_n below 2^25. */
+size_t sonar_scaled_mm_int8_scratch_bytes(int64_t size_m, int64_t size_n, int64_t size_k, int aligned);
 int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const int8_t* b, int64_t b_row_stride, void* c,
                          const float* a_scales, int64_t a_scales_len, const float* b_scales,
                          int64_t b_scales_len, const void* bias, void* scratch, size_t scratch_bytes, int dtype,
@@ -78,6 +80,13 @@ int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const int8_t* b,
 int sonar_topk_routing(const void* logits, int dtype, int64_t row_stride, const float* bias, float* weights,
                        int32_t* ids, int64_t tokens, int64_t experts, int64_t topk, int scoring,
                        int renormalize, int64_t groups, int64_t kept_groups, double factor, void* stream);
+
+/* Diagnostics for tests.  sonar_debug_int8_choice: the number of the kernel form that sonar_scaled_mm_int8 takes for a call
+ * (0 general, 1 to 3 streams of up to 16, 16 and 32 rows, 4 to 8 tiles of 64 x 64, 64 x 128, 128 x 128, 256 x 128, 256 x 256) and
+ * in how many parts it splits K; runs on the host.  sonar_debug_int8_form: the calling thread's calls take that form (-1: the
+ * rule's again); a call that a stream form has too many rows for is refused. */
+int sonar_debug_int8_choice(int64_t size_m, int64_t size_n, int64_t size_k, int aligned, int* splits);
+int sonar_debug_int8_form(int form, int splits);
 
 #ifdef __cplusplus
 }

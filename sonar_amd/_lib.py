@@ -124,7 +124,9 @@ LAYER_PROTOTYPES = {
     "sonar_layer_last_error": (c_char_p, []),
     "sonar_rms_norm_per_token_quant": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                                c_int, c_void_p, c_int, c_int64, c_int64, c_double, c_void_p]),
-    "sonar_scaled_mm_int8_scratch_bytes": (c_size_t, [c_int64] * 3),
+    "sonar_scaled_mm_int8_scratch_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
+    "sonar_debug_int8_choice": (c_int, [c_int64] * 3 + [c_int, c_void_p]),
+    "sonar_debug_int8_form": (c_int, [c_int, c_int]),
     "sonar_scaled_mm_int8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
                                      c_void_p, c_void_p, c_size_t, c_int, c_int64, c_int64, c_int64, c_void_p]),
     "sonar_topk_routing": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int,

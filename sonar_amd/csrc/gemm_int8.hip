@@ -1,4 +1,15 @@
-// Product of 8-bit integers with a scale for each token and channel (W8A8), on the int8 matrix instructions.
+// Product of 8-bit integers with a scale for each token and channel (W8A8), on the int8 matrix instructions:
+//   c[m][n] = T(float(sum over k of a[m][k] b[n][k]) * (a_scales[m] * b_scales[n]) + bias[n])
+// Both operands lie along K, as a checkpoint and a quantiser leave them, and both are read as they lie: nothing is laid
+// out anew.  The sums are integers, so every kernel, split and order gives the same bits.
+//
+//   int8_stream_kernel   up to 16 (32) rows: bound by the bytes of the weight
+//   int8_tile_kernel     more rows, five tile sizes: bound by the matrix pipes from a few hundred rows on
+//   int8_join_kernel     sums of a K that was split over workgroups
+//   int8_pad_kernel      rows that no 16-byte vector is aligned to, laid down aligned for the tiles
+//   int8_general_kernel  anything, without any scratch
+#include <type_traits>
+
 #include "common.hpp"
 #include "sonar_layer.h"
 
@@ -20,7 +31,13 @@ struct Int8Params {
   int a_many, b_many;   // a scale for each row of a / of b (else one)
 };
 
-// 16 bytes of a row from k0 on, zeros behind its end.  Any alignment.
+// What a sum becomes, the same in every kernel: two roundings of float32 (the sum's own where it passes 2^24), and the type's.
+template <typename T>
+__device__ __forceinline__ T int8_result(int sum, float scale_a, float scale_b, float bias) {
+  return (T)__builtin_fmaf((float)sum, scale_a * scale_b, bias);
+}
+
+// 16 bytes of a row from k0 on, zeros behind its end.  Any alignment: the hardware loads a vector from any byte.
 __device__ __forceinline__ intx4_t load_16(const int8_t* row, int k0, int k) {
   intx4_t v = {0, 0, 0, 0};
   if (k0 + 16 <= k) {
@@ -32,14 +49,15 @@ __device__ __forceinline__ intx4_t load_16(const int8_t* row, int k0, int k) {
   return v;
 }
 
+// ---- anything
 // Any strides, alignments and sizes: 64 x 64 results a workgroup, 32 x 32 a wavefront, 128 bytes of K a step through
-// registers into LDS.
-constexpr int kStep = 128, kPitch = kStep + 16;
+// registers into LDS.  Runs where the caller of the C ABI gave no scratch for aligned copies.
 template <typename T>
-__global__ __launch_bounds__(256) void int8_general_kernel(const Int8Params p) {
+__global__ __launch_bounds__(256) void int8_general_kernel(const Int8Params p, int cols) {
+  constexpr int kStep = 128, kPitch = kStep + 16;
   __shared__ __attribute__((aligned(16))) int8_t lds[2][128][kPitch];   // rows of a, then rows of b
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long m0 = (long)blockIdx.y * 64, n0 = (long)blockIdx.x * 64;
+  const long m0 = (long)(blockIdx.x / cols) * 64, n0 = (long)(blockIdx.x % cols) * 64;
   const int row = tid >> 3, chunk = tid & 7;   // a thread's rows row + 32 i, their 16 bytes at 16 chunk
   intx4_t held[4];
   auto fetch = [&](int k0) {
@@ -50,15 +68,12 @@ __global__ __launch_bounds__(256) void int8_general_kernel(const Int8Params p) {
       held[2 + i] = load_16(p.b + n * p.ldb, k0 + 16 * chunk, p.k);
     }
   };
-  auto put = [&](int at) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<intx4_t*>(&lds[at][row + 32 * i][16 * chunk]) = held[i];
-  };
   intx16_t acc = {};
   const int mw = (wave & 1) * 32, nw = 64 + (wave >> 1) * 32;
   fetch(0);
   for (int k0 = 0, at = 0; k0 < p.k; k0 += kStep, at ^= 1) {
-    put(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<intx4_t*>(&lds[at][row + 32 * i][16 * chunk]) = held[i];
     __syncthreads();
     if (k0 + kStep < p.k) fetch(k0 + kStep);
 #pragma unroll
@@ -76,12 +91,571 @@ __global__ __launch_bounds__(256) void int8_general_kernel(const Int8Params p) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const long n = n0 + (nw - 64) + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-    if (n < p.n) {
-      float v = (float)acc[r] * (sa * p.b_scales[p.b_many ? n : 0]);
-      if (p.bias != nullptr) v += (float)((const T*)p.bias)[n];
-      out[n] = (T)v;
+    if (n < p.n)
+      out[n] = int8_result<T>(acc[r], sa, p.b_scales[p.b_many ? n : 0], p.bias ? (float)((const T*)p.bias)[n] : 0.0f);
+  }
+}
+
+// ---- few rows
+// Up to 16 MB tokens: the weight is read once, past LDS, straight into the operand registers of 16 x 16 x 64 matrix
+// instructions (its 16 channels the first operand), 64 bytes of a row an instruction; any alignment.  A workgroup owns 16 NB
+// channels; its wavefronts take steps of 128 bytes of K in turn, so that together they read a run of each row, and join their
+// sums through LDS.  A wavefront has DEEP steps of loads in flight, 4 KB at DEEP = 2: with 16 wavefronts on each compute unit
+// that covers the latency of memory.
+template <typename T, int kWaves, int MB, int NB, int DEEP>
+__global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8Params p, bool vectors) {
+  constexpr int kStepK = 128;
+  __shared__ intx4_t sums[kWaves][NB * MB][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, at = 16 * (lane >> 4);   // an operand's row, and its 16 bytes of 64
+  const long n0 = (long)blockIdx.x * (16 * NB);
+  const int8_t* a_rows[MB];
+  const int8_t* b_rows[NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) a_rows[i] = p.a + min((long)(16 * i + r), (long)p.m - 1) * p.lda;   // (tokens past the end: the last one's)
+#pragma unroll
+  for (int j = 0; j < NB; ++j) b_rows[j] = p.b + min(n0 + 16 * j + r, (long)p.n - 1) * p.ldb;
+  intx4_t acc[NB][MB] = {};
+  struct Step {
+    intx4_t a[MB][2], b[NB][2];
+  } held[DEEP];
+  auto fetch = [&](Step& s, int k) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) __builtin_memcpy(&s.b[j][x], b_rows[j] + at + k + 64 * x, 16);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) __builtin_memcpy(&s.a[i][x], a_rows[i] + at + k + 64 * x, 16);
+    }
+  };
+  auto multiply = [&](const Step& s) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.b[j][x], s.a[i][x], acc[j][i], 0, 0, 0);
+  };
+  const int whole = p.k / kStepK, mine = (whole - wave + kWaves - 1) / kWaves;   // this wavefront's steps
+  const int first = wave * kStepK, next = kWaves * kStepK;
+  int done = 0;
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d)
+    if (d < mine) fetch(held[d], first + d * next);
+  for (; done + 2 * DEEP <= mine; done += DEEP)
+#pragma unroll
+    for (int d = 0; d < DEEP; ++d) {
+      multiply(held[d]);
+      fetch(held[d], first + (done + d + DEEP) * next);
+    }
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d) {
+    if (done + d < mine) multiply(held[d]);
+    if (done + d + DEEP < mine) fetch(held[d], first + (done + d + DEEP) * next);
+  }
+#pragma unroll
+  for (int d = 0; d < DEEP; ++d)
+    if (done + d + DEEP < mine) multiply(held[d]);
+  if (p.k % kStepK != 0 && wave == whole % kWaves) {   // the rest of K
+    Step s;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int k = whole * kStepK + 64 * x + at;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) s.b[j][x] = load_16(b_rows[j], k, p.k);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) s.a[i][x] = load_16(a_rows[i], k, p.k);
+    }
+    multiply(s);
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int i = 0; i < MB; ++i) sums[wave][j * MB + i][lane] = acc[j][i];
+  __syncthreads();
+  for (int x = wave; x < NB * MB; x += kWaves) {
+    intx4_t v = sums[0][x][lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += sums[w][x][lane];
+    // a lane has token 16 i + lane % 16 and channels 4 (lane / 16) + 0 .. 3 of the sixteen
+    const long m = 16 * (x % MB) + r, n = n0 + 16 * (x / MB) + 4 * (lane >> 4);
+    if (m >= p.m) continue;
+    const float sa = p.a_scales[p.a_many ? m : 0];
+    T* out = (T*)p.c + m * p.n + n;
+    typedef T four_t __attribute__((ext_vector_type(4)));
+    four_t result;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long at_n = min(n + e, (long)p.n - 1);
+      result[e] = int8_result<T>(v[e], sa, p.b_scales[p.b_many ? at_n : 0], p.bias ? (float)((const T*)p.bias)[at_n] : 0.0f);
+    }
+    if (vectors && n + 4 <= p.n) {
+      *reinterpret_cast<four_t*>(out) = result;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.n) out[e] = result[e];
     }
   }
+}
+
+// ---- tiles
+struct TilePlan {
+  int tiles_m, tiles_n, splits, per_xcd;
+};
+
+// Tile number -> row and column of tiles: panels of up to eight rows of tiles, down the rows first, so that the 32
+// workgroups of a die at work together share operands.
+__device__ __forceinline__ void tile_at(int tile, const TilePlan& t, int& tm, int& tn) {
+  const int panel = tile / (8 * t.tiles_n), rows = min(8, t.tiles_m - 8 * panel), in = tile - panel * 8 * t.tiles_n;
+  tn = __builtin_amdgcn_readfirstlane(in / rows);   // (the division leaves its quotient in a vector register)
+  tm = __builtin_amdgcn_readfirstlane(8 * panel + in - tn * rows);
+}
+
+// The 32 x 32 results of a wavefront at (m0, n0).  The halves of the wavefront trade quadruples, so that a lane has 16
+// neighbouring channels of its token, 32 bytes of a row.  `scale_a`: of the lane's token; `scales_b` and `bias`: of the 16 channels.
+template <typename T>
+__device__ __forceinline__ void store_block(const intx16_t& acc, const Int8Params& p, long m0, long n0, int lane, bool vectors,
+                                            float scale_a, const floatx4_t* scales_b, const floatx4_t* bias) {
+  const long m = m0 + (lane & 31), n = n0 + 16 * (lane >> 5);
+  T* out = (T*)p.c + m * p.n + n;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    typedef T eight_t __attribute__((ext_vector_type(8)));
+    eight_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // channels 8 q + e of the first half and 16 + 8 q + e; + 4 .. 7 are the other half's
+      const auto both = __builtin_amdgcn_permlane32_swap((unsigned)acc[4 * q + e], (unsigned)acc[8 + 4 * q + e], false, false);
+      v[e] = int8_result<T>((int)both[0], scale_a, scales_b[2 * q][e], bias[2 * q][e]);
+      v[4 + e] = int8_result<T>((int)both[1], scale_a, scales_b[2 * q + 1][e], bias[2 * q + 1][e]);
+    }
+    if (m < p.m) {
+      if (vectors && n + 8 * q + 8 <= p.n) {
+        *reinterpret_cast<eight_t*>(out + 8 * q) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + 8 * q + e < p.n) out[8 * q + e] = v[e];
+      }
+    }
+  }
+}
+
+// A wavefront owns 32 MT rows x 32 NT columns in 32 x 32 x 32 instructions, WM x 2 wavefronts a tile.  The weight is the first
+// operand: a lane then has one token and four neighbouring channels a register quadruple.
+// K goes in stages of kStageK bytes, which LDS-DMA brings into a ring of kRing stages.  16-byte piece c of row i of a stage
+// stands at c ^ (i / 2 & 7) (rows of 64: c ^ (i / 4 & 3)), so that lanes that read together find different banks: 548 bytes/ns
+// a compute unit, where c ^ (i & 7) reaches half and no turn a quarter of that.  Stages of 128 bytes because a copy of whole
+// 128-byte lines runs at 55 bytes a cycle and compute unit, one of half lines at 41 (2048 x 14336 x 4096: 133 -> 104 us); the
+// 256 x 256 tile has no room for three of them and takes four of 64 (859 us for 8192 x 4096 x 28672, 888 with two of 128).
+// Operands are read one step (32 of K) ahead of their matrix instructions.
+// Eight wavefronts for the tiles of 128 rows and up: while one waits at a barrier or issues its copies, the other of its
+// SIMD multiplies (four wavefronts with 128 x 128 each: 944 us instead of 859).
+// KG: that many sets of wavefronts take stages in turn and join their sums through LDS, for tiles too small to keep a compute
+// unit busy otherwise (100 x 4096 x 4096: 9.7 -> 9.2 us).
+// What K is over whole rounds of stages is one more stage, whose pieces behind the end of a row are copied from its last
+// one and cleared (those of a) once they have landed.
+template <typename T, int WM, int MT, int NT, int KG, int kStageK, int kRing>
+__global__ __launch_bounds__(128 * WM * KG, (32 * MT * WM + 64 * NT) * kStageK * kRing * KG <= 81920 ? WM * KG : WM * KG / 2)
+void int8_tile_kernel(const Int8Params p, const TilePlan t, int* __restrict__ partial, bool vectors) {
+  constexpr int BM = 32 * MT * WM, BN = 64 * NT, kWaves = 2 * WM, kThreads = 64 * kWaves, kStage = (BM + BN) * kStageK;
+  constexpr int kPieces = kStageK / 16, kSteps = kStageK / 32;                                    // of a row
+  constexpr int kRows = 64 / kPieces, kLoadsA = BM / kRows / kWaves, kLoads = (BM + BN) / kRows / kWaves;   // of a copy; copies of a wavefront
+  static_assert(BM <= kThreads && BN <= kThreads && (kRing - 2) * kLoads < 64, "");
+  extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = all_waves % kWaves, group = all_waves / kWaves;
+  const int unit = (blockIdx.x & 7) * t.per_xcd + (blockIdx.x >> 3);   // workgroups go to the eight dies in turn
+  const int tiles = t.tiles_m * t.tiles_n;
+  if (unit >= tiles * t.splits) return;
+  const int split = unit / tiles, tile = unit - split * tiles;
+  int tm, tn;
+  tile_at(tile, t, tm, tn);
+  const long m0 = (long)tm * BM, n0 = (long)tn * BN;
+  // rounds of KG stages, dealt evenly; the last split has the rest of K too
+  const int all = p.k / (kStageK * KG), first = split * all / t.splits, whole = (split + 1) * all / t.splits - first;
+  const bool rest = split == t.splits - 1 && p.k % (kStageK * KG) != 0;
+  const int count = whole + (rest ? 1 : 0);
+
+  // the scales and the bias of the tile, a row and a column a thread, until its results are scaled
+  float my_scale_a = 0, my_scale_b = 0, my_bias = 0;
+  if (partial == nullptr) {
+    const long m = min(m0 + tid % kThreads, (long)p.m - 1), n = min(n0 + tid % kThreads, (long)p.n - 1);
+    my_scale_a = p.a_scales[p.a_many ? m : 0];
+    my_scale_b = p.b_scales[p.b_many ? n : 0];
+    if (p.bias != nullptr) my_bias = (float)((const T*)p.bias)[n];
+  }
+
+  // copies: of kRows rows each; lane i brings piece i % kPieces of row i / kPieces
+  int8_t* ring = lds + group * (kRing * kStage);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)ring;
+  const char* a_base = (const char*)p.a + m0 * p.lda;
+  const char* b_base = (const char*)p.b + n0 * p.ldb;
+  auto turned = [](int row) { return kStageK == 64 ? row >> 2 & 3 : row >> 1 & 7; };
+  uint32_t off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const bool b = i >= kLoadsA;
+    const int row = (b ? wave * (kLoads - kLoadsA) + i - kLoadsA : wave * kLoadsA + i) * kRows + lane / kPieces;
+    const long end = b ? p.n - 1 - n0 : p.m - 1 - m0;   // rows past the end repeat the last one and are not stored
+    off[i] = (uint32_t)(min((long)row, end) * (b ? p.ldb : p.lda)) + (lane % kPieces ^ turned(row)) * 16;
+  }
+  auto to = [&](int i, int stage) {
+    const bool b = i >= kLoadsA;
+    return lds0 + (stage % kRing) * kStage +
+           (b ? BM * kStageK + (wave * (kLoads - kLoadsA) + i - kLoadsA) * 1024 : (wave * kLoadsA + i) * 1024);
+  };
+  auto copy = [&](int i, int stage) {   // of this split; a whole one
+    copy_to_lds<16>(to(i, stage), off[i], (i >= kLoadsA ? b_base : a_base) + ((long)(first + stage) * KG + group) * kStageK);
+  };
+  auto copy_rest = [&]() {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool b = i >= kLoadsA;
+      const int row = (b ? wave * (kLoads - kLoadsA) + i - kLoadsA : wave * kLoadsA + i) * kRows + lane / kPieces;
+      const uint32_t piece = (lane % kPieces ^ turned(row)) * 16, k = (all * KG + group) * kStageK + piece;
+      copy_to_lds<16>(to(i, whole), off[i] - piece + min(k, (uint32_t)p.k - 16), b ? b_base : a_base);
+    }
+  };
+  auto clear_rest = [&]() {   // the pieces of a behind the end of K
+    for (int i = tid % kThreads; i < BM * kPieces; i += kThreads) {
+      const int row = i / kPieces, c = i % kPieces;
+      if ((all * KG + group) * kStageK + 16 * c >= p.k)
+        *reinterpret_cast<intx4_t*>(ring + (whole % kRing) * kStage + row * kStageK + (c ^ turned(row)) * 16) = intx4_t{0, 0, 0, 0};
+    }
+    __syncthreads();
+  };
+
+  // operands: row lane % 32 of a block, piece 2 s + lane / 32 of step s
+  const int wm = wave % WM, wn = wave / WM, r = lane & 31, h = lane >> 5;
+  const int at0 = r * kStageK + (h ^ turned(r)) * 16;
+  const int a_at = wm * MT * 32 * kStageK + at0, b_at = (BM + wn * NT * 32) * kStageK + at0;
+  intx4_t fa[2][MT], fb[2][NT];
+  auto read_a = [&](int s, int i, int stage) {
+    fa[s & 1][i] = *reinterpret_cast<const intx4_t*>(ring + (stage % kRing) * kStage + (a_at ^ (32 * s)) + i * 32 * kStageK);
+  };
+  auto read_b = [&](int s, int i, int stage) {
+    fb[s & 1][i] = *reinterpret_cast<const intx4_t*>(ring + (stage % kRing) * kStage + (b_at ^ (32 * s)) + i * 32 * kStageK);
+  };
+  intx16_t acc[MT][NT] = {};
+
+  // Step s of a stage: its matrix instructions, between them the reads of the next step and a share of the copies.
+  auto step = [&](int s, int stage, bool copies) {
+    constexpr int kAll = MT * NT, kSpread = kSteps > 2 ? kSteps - 1 : 1;   // the copies are over before the last step
+#pragma unroll
+    for (int x = 0; x < kAll; ++x) {
+      // the next step's operands, spread over the first three quarters: a's first, then b's, then a's others
+#pragma unroll
+      for (int y = 0; y < MT + NT; ++y)
+        if (y * (kAll * 3 / 4) / (MT + NT) == x) {
+          const int next = s == kSteps - 1 ? stage + 1 : stage, at = (s + 1) % kSteps;
+          if (y == 0) read_a(at, 0, next);
+          else if (y <= NT) read_b(at, y - 1, next);
+          else read_a(at, y - NT, next);
+        }
+      if (copies) {
+#pragma unroll
+        for (int y = 0; y < kLoads; ++y)
+          if (y * kSpread * kAll / kLoads == s * kAll + x) copy(y, stage + kRing - 1);
+      }
+      acc[x / NT][x % NT] =
+          __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[s & 1][x % NT], fa[s & 1][x / NT], acc[x / NT][x % NT], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  const int ahead = min(whole, kRing - 1);
+  for (int i = 0; i < ahead; ++i)
+#pragma unroll
+    for (int y = 0; y < kLoads; ++y) copy(y, i);
+  const bool rest_early = rest && whole < kRing - 1;
+  if (rest_early) copy_rest();
+  // stage 0: its copies have landed once those of the stages behind it are all that is out
+  if (whole >= kRing - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kRing - 2) * kLoads) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  if (rest && whole == 0) clear_rest();
+#pragma unroll
+  for (int i = 0; i < MT; ++i) read_a(0, i, 0);
+#pragma unroll
+  for (int i = 0; i < NT; ++i) read_b(0, i, 0);
+  // The next stage has landed in every wavefront's copies, and every wavefront has read this one: behind the barrier the
+  // next one may be read and this one's room filled.
+  auto next_stage = [&](auto waits) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(decltype(waits)::value) : "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int stage = 0;
+  for (; stage + kRing - 1 < whole; ++stage) {
+#pragma unroll
+    for (int s = 0; s < kSteps - 1; ++s) step(s, stage, true);
+    next_stage(std::integral_constant<int, (kRing - 2) * kLoads>());
+    step(kSteps - 1, stage, false);
+  }
+  if (rest && !rest_early) copy_rest();
+  for (; stage < count; ++stage) {   // (the last one reads operands that nothing uses)
+#pragma unroll
+    for (int s = 0; s < kSteps - 1; ++s) step(s, stage, false);
+    next_stage(std::integral_constant<int, 0>());
+    if (rest && stage + 1 == whole) clear_rest();
+    step(kSteps - 1, stage, false);
+  }
+
+  // Groups: every sum to LDS, and each group's wavefront takes the blocks x with x % KG == group.
+  if constexpr (KG > 1) {
+    __syncthreads();
+    intx4_t* sums = reinterpret_cast<intx4_t*>(lds);   // [group][wave][block][quadruple][lane]
+#pragma unroll
+    for (int x = 0; x < MT * NT; ++x)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const intx16_t& v = acc[x / NT][x % NT];
+        sums[(((group * kWaves + wave) * MT * NT + x) * 4 + q) * 64 + lane] =
+            intx4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < MT * NT; ++x) {
+      if (x % KG != group) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        intx4_t v = {0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < KG; ++g) v += sums[(((g * kWaves + wave) * MT * NT + x) * 4 + q) * 64 + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[x / NT][x % NT][4 * q + e] = v[e];
+      }
+    }
+  }
+  const long wm0 = m0 + wm * MT * 32, wn0 = n0 + wn * NT * 32;
+  if (partial != nullptr) {   // sums in the order of the registers, block after block
+    int* out = partial + ((long)(split * tiles + tile) * kWaves + wave) * (MT * NT * 1024);
+#pragma unroll
+    for (int x = 0; x < MT * NT; ++x) {
+      if (KG > 1 && x % KG != group) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<intx4_t*>(out + x * 1024 + q * 256 + lane * 4) =
+            intx4_t{acc[x / NT][x % NT][4 * q], acc[x / NT][x % NT][4 * q + 1], acc[x / NT][x % NT][4 * q + 2],
+                    acc[x / NT][x % NT][4 * q + 3]};
+    }
+    return;
+  }
+  float* scales = reinterpret_cast<float*>(lds);   // of a's rows, of b's rows, and the bias
+  __syncthreads();
+  if (tid < BM) scales[tid] = my_scale_a;
+  if (tid < BN) scales[BM + tid] = my_scale_b, scales[BM + BN + tid] = my_bias;
+  __syncthreads();
+  if constexpr (KG > 1) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const float scale_a = scales[(wm * MT + i) * 32 + r];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if ((i * NT + j) % KG != group) continue;
+        const float* of_b = scales + BM + (wn * NT + j) * 32 + 16 * h;
+        floatx4_t sb[4], add[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sb[e] = *reinterpret_cast<const floatx4_t*>(of_b + 4 * e);
+          add[e] = *reinterpret_cast<const floatx4_t*>(of_b + BN + 4 * e);
+        }
+        store_block<T>(acc[i][j], p, wm0 + i * 32, wn0 + j * 32, lane, vectors, scale_a, sb, add);
+      }
+    }
+  } else {
+    // 32 rows at a time turn in LDS, so that they leave as whole lines, 64 NT bytes a row (in pieces of 32 bytes from where
+    // they are: 8192 x 4096 x 28672 926 us instead of 901)
+    constexpr int kPitch = 64 * NT + 16, kLanes = 4 * NT, kRowsOut = 64 / kLanes;
+    typedef T eight_t __attribute__((ext_vector_type(8)));
+    typedef T four_t __attribute__((ext_vector_type(4)));
+    int8_t* turn_lds = lds + (BM + 2 * BN) * 4 + wave * 32 * kPitch;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const float scale_a = scales[(wm * MT + i) * 32 + r];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = j * 32 + 8 * q + 4 * h;   // of the wavefront's columns
+          const floatx4_t sb = *reinterpret_cast<const floatx4_t*>(scales + BM + wn * NT * 32 + n);
+          const floatx4_t add = *reinterpret_cast<const floatx4_t*>(scales + BM + BN + wn * NT * 32 + n);
+          four_t v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = int8_result<T>(acc[i][j][4 * q + e], scale_a, sb[e], add[e]);
+          *reinterpret_cast<four_t*>(turn_lds + r * kPitch + n * 2) = v;
+        }
+      __builtin_amdgcn_sched_barrier(0);   // (one strip's registers at a time)
+#pragma unroll
+      for (int x = 0; x < 32 / kRowsOut; ++x) {
+        const int row = x * kRowsOut + lane / kLanes, col = lane % kLanes * 8;
+        const eight_t v = *reinterpret_cast<const eight_t*>(turn_lds + row * kPitch + col * 2);
+        const long m = wm0 + i * 32 + row, n = wn0 + col;
+        T* out = (T*)p.c + m * p.n + n;
+        if (m < p.m) {
+          if (vectors && n + 8 <= p.n) {
+            *reinterpret_cast<eight_t*>(out) = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < p.n) out[e] = v[e];
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// The sum of the splits' partial tiles, a wavefront a block of 32 x 32.
+template <typename T, int WM, int MT, int NT>
+__global__ __launch_bounds__(256) void int8_join_kernel(const Int8Params p, const TilePlan t, const int* __restrict__ partial, bool vectors) {
+  const int lane = threadIdx.x & 63;
+  const long block = (long)blockIdx.x * 4 + (threadIdx.x >> 6);   // ((tile * 2 WM + wave) * MT + i) * NT + j
+  const int tiles = t.tiles_m * t.tiles_n;
+  if (block >= (long)tiles * 2 * WM * MT * NT) return;
+  const int j = block % NT, i = block / NT % MT, wave = block / (MT * NT) % (2 * WM), tile = block / (MT * NT * 2 * WM);
+  intx16_t acc = {};
+  for (int s = 0; s < t.splits; ++s) {
+    const int* from = partial + ((long)s * tiles * 2 * WM * MT * NT + block) * 1024;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const intx4_t v = *reinterpret_cast<const intx4_t*>(from + q * 256 + lane * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
+    }
+  }
+  int tm, tn;
+  tile_at(tile, t, tm, tn);   // (a workgroup's four blocks are of one tile)
+  const long m0 = (long)tm * 32 * MT * WM + (wave % WM * MT + i) * 32, n0 = (long)tn * 64 * NT + (wave / WM * NT + j) * 32;
+  if (m0 >= p.m || n0 >= p.n) return;
+  const long m = min(m0 + (lane & 31), (long)p.m - 1);
+  floatx4_t sb[4], add[4];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const long n = min(n0 + 16 * (lane >> 5) + e, (long)p.n - 1);
+    sb[e / 4][e % 4] = p.b_scales[p.b_many ? n : 0];
+    add[e / 4][e % 4] = p.bias ? (float)((const T*)p.bias)[n] : 0.0f;
+  }
+  store_block<T>(acc, p, m0, n0, lane, vectors, p.a_scales[p.a_many ? m : 0], sb, add);
+}
+
+// Rows of a and of b -> rows `pitch` bytes apart, zeros behind K; 16 bytes a thread.
+__global__ __launch_bounds__(256) void int8_pad_kernel(const Int8Params p, int8_t* __restrict__ a, int8_t* __restrict__ b, int pitch) {
+  const int pieces = pitch / 16;
+  const long all = ((long)p.m + p.n) * pieces;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
+    const long row = i / pieces;
+    const int k = (int)(i - row * pieces) * 16;
+    const bool of_a = row < p.m;
+    const long at = of_a ? row : row - p.m;
+    *reinterpret_cast<intx4_t*>((of_a ? a : b) + at * pitch + k) = load_16(of_a ? p.a + at * p.lda : p.b + at * p.ldb, k, p.k);
+  }
+}
+
+// ---- host
+enum Form { kGeneral, kStream32, kStream16, kStreamTwo, kTile64, kTile128Wide, kTile128, kTile256Tall, kTile256, kForms };
+// Rows and columns of a form's tile, and what it takes (us): a round of 256 workgroups, and 1024 of K in it.  Fitted to 140
+// shapes of 24 to 4096 rows, 256 to 28672 channels, K of 2048 to 14336; the choice they make is 0.2 % slower than the best one
+// (geometric mean; at most 5 %).
+struct FormCost {
+  int rows, cols;
+  float round, per_k;
+};
+constexpr FormCost kCosts[kForms] = {{64, 64, 0, 0},       {16, 32, 0, 0},        {16, 16, 0, 0},        {32, 16, 0, 0}, {64, 64, 4.4f, 1.3f},
+                                     {64, 128, 5.0f, 2.0f}, {128, 128, 5.0f, 3.1f}, {256, 128, 6.5f, 4.6f}, {256, 256, 8.1f, 8.3f}};
+constexpr float kJoinUs = 4.5f, kJoinBytesPerUs = 4.5e6f;   // a launch more; partial sums written and read
+
+struct Int8Choice {
+  int form, splits;
+};
+thread_local Int8Choice g_forced = {-1, 1};
+
+int64_t tiles_of(int form, int64_t m, int64_t n) {
+  return ((m + kCosts[form].rows - 1) / kCosts[form].rows) * ((n + kCosts[form].cols - 1) / kCosts[form].cols);
+}
+
+// Whether tiles can split K so: every split has 512 of it at least, so that the join costs less than it saves.
+bool may_split(int splits, int64_t k) { return splits == 1 || k / splits >= 512; }
+
+Int8Choice choose_form(int64_t m, int64_t n, int64_t k, bool aligned) {
+  if (g_forced.form >= 0) return g_forced;
+  // Up to 256 workgroups of 16 channels sixteen wavefronts each, else eight with 32 channels, two workgroups on a compute unit
+  // (1 x 4096 x 4096 5.8 us, 7.2 with 32 channels; 16 x 4096 x 28672 29.0, 35.7 with 16).
+  if (m <= 16) return {n <= 4096 ? kStream16 : kStream32, 1};
+  // 17 to 32 rows: less than the tiles' 64 where the weight is small (24 x 2048 x 2048 6.1 us, tiles 6.8; 24 x 14336 x 1024 at
+  // 18, split tiles 13.0).  Unaligned rows would first be laid down for the tiles.
+  if (m <= 32 && ((n <= 4096 && k <= 6144) || !aligned)) return {kStreamTwo, 1};
+  if (k < 16) return {kGeneral, 1};
+  Int8Choice best = {kTile64, 1};
+  float least = 3.4e38f;
+  for (int form = kTile64; form <= kTile256; ++form)
+    for (int splits = 1; splits <= 8 && may_split(splits, k); splits *= 2) {
+      const int64_t tiles = tiles_of(form, m, n);
+      if (splits > 1 && tiles * splits > 1024) break;
+      const float rounds = (float)((tiles * splits + 255) / 256);
+      float us = rounds * (kCosts[form].round + kCosts[form].per_k * (float)k / splits / 1024);
+      if (splits > 1) us += kJoinUs + (float)tiles * splits * kCosts[form].rows * kCosts[form].cols * 8 / kJoinBytesPerUs;
+      if (us < least) least = us, best = {form, splits};
+    }
+  return best;
+}
+
+bool is_tile(int form) { return form >= kTile64; }
+
+size_t partial_bytes(const Int8Choice& s, int64_t m, int64_t n) {
+  if (!is_tile(s.form) || s.splits <= 1) return 0;
+  return (size_t)tiles_of(s.form, m, n) * s.splits * kCosts[s.form].rows * kCosts[s.form].cols * 4;
+}
+int64_t padded_k(int64_t k) { return (k + 255) / 256 * 256; }   // whole rounds of every form
+size_t padded_bytes(const Int8Choice& s, int64_t m, int64_t n, int64_t k, bool aligned) {
+  return is_tile(s.form) && !aligned ? (size_t)(m + n) * padded_k(k) : 0;
+}
+
+template <typename T, int WM, int MT, int NT, int KG, int kStageK, int kRing>
+int launch_tiles(const Int8Params& p, int splits, int* partial, bool vectors, hipStream_t st) {
+  constexpr int BM = 32 * MT * WM, BN = 64 * NT;
+  constexpr int kStages = (BM + BN) * kStageK * kRing * KG;
+  constexpr int kSums = KG > 1 ? KG * BM * BN * 4 : 4 * (BM + 2 * BN) + 2 * WM * 32 * (64 * NT + 16);
+  constexpr int kLds = kStages > kSums ? kStages : kSums;
+  static_assert(kLds <= 163840, "");
+  TilePlan t;
+  t.tiles_m = (int)(((int64_t)p.m + BM - 1) / BM), t.tiles_n = (int)(((int64_t)p.n + BN - 1) / BN);
+  t.splits = splits;
+  const int64_t units = (int64_t)t.tiles_m * t.tiles_n * splits;
+  SONAR_REQUIRE(units < (1 << 22), "size_m = %d, size_n = %d: more tiles than a launch takes", p.m, p.n);
+  t.per_xcd = (int)((units + 7) / 8);
+  if (kLds > 65536)
+    SONAR_HIP(hipFuncSetAttribute((const void*)int8_tile_kernel<T, WM, MT, NT, KG, kStageK, kRing>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+  int8_tile_kernel<T, WM, MT, NT, KG, kStageK, kRing><<<8 * t.per_xcd, 128 * WM * KG, kLds, st>>>(p, t, partial, vectors);
+  if (partial != nullptr) {
+    static_assert(MT * NT * 2 * WM % 4 == 0, "");
+    int8_join_kernel<T, WM, MT, NT><<<t.tiles_m * t.tiles_n * (MT * NT * WM / 2), 256, 0, st>>>(p, t, partial, vectors);
+  }
+  return launch_status("int8_tile_kernel");
+}
+
+template <typename T>
+int run_form(const Int8Params& p, const Int8Choice& s, int* partial, bool vectors, hipStream_t st) {
+  switch (s.form) {
+    case kTile64: return launch_tiles<T, 2, 1, 1, 2, 128, 4>(p, s.splits, partial, vectors, st);
+    case kTile128Wide: return launch_tiles<T, 2, 1, 2, 2, 128, 3>(p, s.splits, partial, vectors, st);
+    case kTile128: return launch_tiles<T, 4, 1, 2, 1, 128, 3>(p, s.splits, partial, vectors, st);
+    case kTile256Tall: return launch_tiles<T, 4, 2, 2, 1, 128, 3>(p, s.splits, partial, vectors, st);
+    case kTile256: return launch_tiles<T, 4, 2, 4, 1, 64, 4>(p, s.splits, partial, vectors, st);
+    case kStream32: int8_stream_kernel<T, 8, 1, 2, 3><<<(p.n + 31) / 32, 512, 0, st>>>(p, vectors); break;
+    case kStream16: int8_stream_kernel<T, 16, 1, 1, 2><<<(p.n + 15) / 16, 1024, 0, st>>>(p, vectors); break;
+    case kStreamTwo: int8_stream_kernel<T, 16, 2, 1, 2><<<(p.n + 15) / 16, 1024, 0, st>>>(p, vectors); break;
+    default: {
+      const int64_t rows = ((int64_t)p.m + 63) / 64, cols = ((int64_t)p.n + 63) / 64;
+      SONAR_REQUIRE(rows * cols < (1 << 23), "size_m = %d, size_n = %d: more tiles than a launch takes", p.m, p.n);
+      int8_general_kernel<T><<<(int)(rows * cols), 256, 0, st>>>(p, (int)cols);
+    }
+  }
+  return launch_status("int8 product");
 }
 
 }  // namespace
@@ -89,18 +663,31 @@ __global__ __launch_bounds__(256) void int8_general_kernel(const Int8Params p) {
 
 using namespace sonar;
 
-extern "C" size_t sonar_scaled_mm_int8_scratch_bytes(int64_t size_m, int64_t size_n, int64_t size_k) {
-  (void)size_m, (void)size_n, (void)size_k;
-  return 0;
+extern "C" int sonar_debug_int8_form(int form, int splits) {
+  SONAR_REQUIRE(form >= -1 && form < kForms && splits >= 1 && splits <= 8, "form = %d, splits = %d", form, splits);
+  g_forced = {form, splits};
+  return SONAR_OK;
+}
+
+extern "C" int sonar_debug_int8_choice(int64_t size_m, int64_t size_n, int64_t size_k, int aligned, int* splits) {
+  const Int8Choice s = choose_form(size_m, size_n, size_k, aligned && size_k % 16 == 0);
+  if (splits != nullptr) *splits = s.splits;
+  return s.form;
+}
+
+extern "C" size_t sonar_scaled_mm_int8_scratch_bytes(int64_t size_m, int64_t size_n, int64_t size_k, int aligned) {
+  if (size_m <= 0 || size_n <= 0 || size_k <= 0) return 0;
+  const bool vectors_of_k = aligned && size_k % 16 == 0;
+  const Int8Choice s = choose_form(size_m, size_n, size_k, vectors_of_k);
+  return padded_bytes(s, size_m, size_n, size_k, vectors_of_k) + partial_bytes(s, size_m, size_n);
 }
 
 extern "C" int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const int8_t* b, int64_t b_row_stride, void* c,
                                     const float* a_scales, int64_t a_scales_len, const float* b_scales, int64_t b_scales_len,
                                     const void* bias, void* scratch, size_t scratch_bytes, int dtype, int64_t size_m,
                                     int64_t size_n, int64_t size_k, void* stream) {
-  (void)scratch, (void)scratch_bytes;
   SONAR_REQUIRE(dtype == SONAR_DTYPE_F16 || dtype == SONAR_DTYPE_BF16, "unknown dtype = %d: float16 or bfloat16 results", dtype);
-  SONAR_REQUIRE(size_m >= 0 && size_m < (1LL << 31) - 256 && size_n >= 0 && size_n < (1LL << 31) - 256, "size_m = %ld, size_n = %ld",
+  SONAR_REQUIRE(size_m >= 0 && size_m < (1LL << 25) && size_n >= 0 && size_n < (1LL << 25), "size_m = %ld, size_n = %ld",
                 (long)size_m, (long)size_n);
   SONAR_REQUIRE(size_k >= 0 && size_k < 131072, "size_k = %ld: the 32-bit sums hold fewer than 131072 products", (long)size_k);
   if (size_m == 0 || size_n == 0) return SONAR_OK;
@@ -110,13 +697,28 @@ extern "C" int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const
   SONAR_REQUIRE((a_scales_len == 1 || a_scales_len == size_m) && (b_scales_len == 1 || b_scales_len == size_n),
                 "a_scales holds %ld numbers (1 or size_m = %ld are needed), b_scales %ld (1 or size_n = %ld)", (long)a_scales_len,
                 (long)size_m, (long)b_scales_len, (long)size_n);
-  const Int8Params p{a,        b,        c, a_scales, b_scales, bias, a_row_stride, b_row_stride, (int)size_m, (int)size_n,
-                     (int)size_k, a_scales_len > 1, b_scales_len > 1};
+  SONAR_REQUIRE(scratch == nullptr || (uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
+  Int8Params p{a,        b,        c, a_scales, b_scales, bias, a_row_stride, b_row_stride, (int)size_m, (int)size_n,
+               (int)size_k, a_scales_len > 1, b_scales_len > 1};
   hipStream_t st = (hipStream_t)stream;
-  const int64_t rows = (size_m + 63) / 64, cols = (size_n + 63) / 64;
-  SONAR_REQUIRE(rows < 65536 && cols < (1 << 24), "size_m = %ld, size_n = %ld", (long)size_m, (long)size_n);
-  const dim3 grid((unsigned)cols, (unsigned)rows);
-  if (dtype == SONAR_DTYPE_F16) int8_general_kernel<_Float16><<<grid, 256, 0, st>>>(p);
-  else int8_general_kernel<__bf16><<<grid, 256, 0, st>>>(p);
-  return launch_status("int8_general_kernel");
+  // (a tile's rows are found with 32-bit offsets: rows further than 8 MB apart are laid down nearer first)
+  const bool aligned = ((uintptr_t)a | (uintptr_t)b | (uintptr_t)a_row_stride | (uintptr_t)b_row_stride | (uintptr_t)size_k) % 16 == 0 &&
+                       a_row_stride < (1 << 23) && b_row_stride < (1 << 23);
+  const bool vectors = size_n % 8 == 0 && ((uintptr_t)c | (uintptr_t)bias) % 16 == 0;
+  if (scratch == nullptr) scratch_bytes = 0;
+  Int8Choice s = choose_form(size_m, size_n, size_k, aligned);
+  if (is_tile(s.form) && size_k < 16) s = {kGeneral, 1};
+  SONAR_REQUIRE(is_tile(s.form) || s.form == kGeneral || size_m <= kCosts[s.form].rows, "form %d takes %d rows", s.form, kCosts[s.form].rows);
+  const size_t padded = padded_bytes(s, size_m, size_n, size_k, aligned);
+  if (padded > scratch_bytes) s = {kGeneral, 1};
+  if (is_tile(s.form) && padded > 0) {
+    const int pitch = (int)padded_k(size_k);
+    int8_t* copies = (int8_t*)scratch;
+    const int64_t pieces = (size_m + size_n) * (pitch / 16);
+    int8_pad_kernel<<<(int)(pieces < 256 * 4096 ? (pieces + 255) / 256 : 4096), 256, 0, st>>>(p, copies, copies + size_m * pitch, pitch);
+    p.a = copies, p.b = copies + size_m * pitch, p.lda = p.ldb = p.k = pitch;
+  }
+  if (!is_tile(s.form) || !may_split(s.splits, size_k) || padded + partial_bytes(s, size_m, size_n) > scratch_bytes) s.splits = 1;
+  int* partial = s.splits > 1 ? (int*)((char*)scratch + padded) : nullptr;
+  return dtype == SONAR_DTYPE_F16 ? run_form<_Float16>(p, s, partial, vectors, st) : run_form<__bf16>(p, s, partial, vectors, st);
 }

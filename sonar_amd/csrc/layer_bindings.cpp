@@ -102,12 +102,16 @@ Tensor scaled_mm_int8(const Tensor& a, const Tensor& b, const Tensor& a_scales, 
   int64_t lda = k;
   const Tensor rows = k > 0 ? rows_of(a, k, lda) : a;
   const Tensor sa = a_scales.contiguous(), sb = b_scales.contiguous(), bc = bias.has_value() ? bias->contiguous() : Tensor();
-  const size_t scratch_bytes = sonar_scaled_mm_int8_scratch_bytes(m, n, k);
+  const int64_t ldb = n > 1 && k > 0 ? b.stride(1) : k;
+  const auto bits = reinterpret_cast<uintptr_t>(rows.const_data_ptr()) | reinterpret_cast<uintptr_t>(b.const_data_ptr()) |
+                    (uintptr_t)lda | (uintptr_t)ldb;
+  const size_t scratch_bytes =
+      sonar_scaled_mm_int8_scratch_bytes(m, n, k, bits % 16 == 0 && lda < (1 << 23) && ldb < (1 << 23) ? 1 : 0);
   Tensor scratch;
   if (scratch_bytes > 0) scratch = at::empty({(int64_t)scratch_bytes}, a.options().dtype(at::kByte));
   raise_if_failed(sonar_scaled_mm_int8(
       static_cast<const int8_t*>(rows.const_data_ptr()), lda, static_cast<const int8_t*>(b.const_data_ptr()),
-      n > 1 && k > 0 ? b.stride(1) : k, c.mutable_data_ptr(), static_cast<const float*>(sa.const_data_ptr()), sa.numel(),
+      ldb, c.mutable_data_ptr(), static_cast<const float*>(sa.const_data_ptr()), sa.numel(),
       static_cast<const float*>(sb.const_data_ptr()), sb.numel(), bias.has_value() ? bc.const_data_ptr() : nullptr,
       scratch_bytes > 0 ? scratch.mutable_data_ptr() : nullptr, scratch_bytes,
       out_dtype == at::kHalf ? SONAR_DTYPE_F16 : SONAR_DTYPE_BF16, m, n, k, current_stream(a)));

@@ -71,6 +71,47 @@ def test_larger(m, k, n):
     run(m, k, n, bias=True)
 
 
+FORMS = {0: 1 << 20, 1: 16, 2: 16, 3: 32, 4: 1 << 20, 5: 1 << 20, 6: 1 << 20, 7: 1 << 20, 8: 1 << 20}   # and the rows each takes
+
+
+@pytest.fixture
+def force():
+    from sonar_amd import _lib
+    lib = _lib.load_layer()
+    yield lambda form, splits=1: _lib.check_layer(lib.sonar_debug_int8_form(form, splits))
+    lib.sonar_debug_int8_form(-1, 1)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_every_form(form, dtype, force):
+    """Each kernel form at sizes around its tile, K shorter than its ring, K that ends inside a round, and at each of
+    them with and without aligned rows."""
+    force(form)
+    for m in (1, 16, 32, 63, 65, 129, 257, 300):
+        if m > FORMS[form]:
+            continue
+        for k in (16, 64, 112, 128, 256, 272, 400, 1024, 1040, 2944, 203):
+            for n in (40, 264):
+                run(m, k, n, dtype, bias=(m + k) % 2 == 0, seed=form)
+
+
+@pytest.mark.parametrize("form", [4, 5, 6, 7, 8])
+@pytest.mark.parametrize("splits", [2, 3, 5, 8])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_split_sums(form, splits, dtype, force):
+    """K in parts that its rounds do not divide into evenly."""
+    force(form, splits)
+    for m, k, n in ((70, 512 * splits, 136), (33, 512 * splits + 16, 300), (130, 4400, 72), (40, 600 * splits + 3, 130)):
+        run(m, k, n, dtype, bias=True)
+
+
+def test_a_form_with_too_few_rows_is_refused(force):
+    force(2)
+    with pytest.raises(RuntimeError, match="rows"):
+        run(17, 64, 64)
+
+
 def test_extremes_of_the_sum():
     """Every product 128 * 128, over the deepest K: 2^31 - 2^14 is the largest sum that 32 bits hold; and its opposite."""
     from sonar_amd import ops
@@ -171,10 +212,10 @@ def test_smaller_scratch_gives_the_same_bits():
     from sonar_amd import _lib
     from tests import gpu_util as gu
     lib = _lib.load_layer()
-    for m, k, n in ((1, 4096, 512), (40, 14336, 256), (200, 4096, 1024), (520, 8192, 512)):
+    for m, k, n in ((1, 4096, 512), (40, 14336, 256), (200, 4096, 1024), (520, 8192, 512), (40, 1003, 300), (100, 14335, 200)):
         a, b, sa, sb, _ = make(m, m, k, n, "bf16", False)
         da, db, dsa, dsb = dev(a), dev(b), dev(sa), dev(sb)
-        full = lib.sonar_scaled_mm_int8_scratch_bytes(m, n, k)
+        full = lib.sonar_scaled_mm_int8_scratch_bytes(m, n, k, int(k % 16 == 0))
         results = []
         for size in {0, full // 2 // 16 * 16, full}:
             scratch = torch.full((size + 64,), 99, dtype=torch.uint8, device=DEV)

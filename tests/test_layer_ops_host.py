@@ -90,6 +90,33 @@ def test_router_refuses(change, message):
     assert route_call(lib, **change) == _lib.E_INVALID and message in lib.sonar_layer_last_error().decode()
 
 
+def test_the_rule_of_the_int8_product():
+    """Which form takes a call, at the borders of the rule, and that its scratch is what the form needs."""
+    import ctypes
+    _lib, lib = layer()
+    def choice(m, n, k, aligned=1):
+        splits = ctypes.c_int(0)
+        return lib.sonar_debug_int8_choice(m, n, k, aligned, ctypes.byref(splits)), splits.value
+    assert choice(1, 4096, 4096) == (2, 1) and choice(16, 4097, 4096) == (1, 1)
+    assert choice(17, 4096, 6144) == (3, 1) and choice(32, 4112, 4096)[0] >= 4 and choice(32, 4112, 4096, 0) == (3, 1)
+    assert choice(17, 28672, 100) == (3, 1)           # K is no multiple of 16: unaligned whatever the strides are
+    assert choice(33, 100, 15) == (0, 1)
+    assert choice(8192, 28672, 4096) == (8, 1) and choice(2048, 4096, 14336) == (7, 1)
+    form, splits = choice(64, 256, 14336)
+    assert form == 4 and splits > 1
+    rows, cols = (64, 64, 128, 256, 256), (64, 128, 128, 128, 256)
+    for m, n, k in ((1, 512, 4096), (64, 256, 14336), (200, 1024, 14336), (500, 4096, 4096), (70, 700, 1001), (3000, 3000, 8191)):
+        for aligned in (0, 1):
+            form, splits = choice(m, n, k, aligned)
+            want = 0
+            if form >= 4:
+                tiles = -(-m // rows[form - 4]) * -(-n // cols[form - 4])
+                want = tiles * rows[form - 4] * cols[form - 4] * 4 * splits if splits > 1 else 0
+                want += 0 if aligned and k % 16 == 0 else (m + n) * (-(-k // 256) * 256)
+            assert lib.sonar_scaled_mm_int8_scratch_bytes(m, n, k, aligned) == want, (m, n, k, aligned)
+    assert lib.sonar_scaled_mm_int8_scratch_bytes(0, 8, 8, 1) == 0
+
+
 def test_calls_without_rows_launch_nothing():
     _lib, lib = layer()
     assert norm_call(lib, rows=0, x=None, q=None) == 0
@@ -201,7 +228,8 @@ def test_oracle_values():
     assert c.tolist() == [[-1.5, -382.0]]
 
 
-KERNEL_FORMS = {"rms_norm_quant_kernel": 6, "int8_general_kernel": 2, "topk_routing_kernel": 3}
+KERNEL_FORMS = {"rms_norm_quant_kernel": 6, "int8_general_kernel": 2, "topk_routing_kernel": 3, "int8_stream_kernel": 6,
+                "int8_tile_kernel": 10, "int8_join_kernel": 10, "int8_pad_kernel": 1}
 
 
 def test_library_holds_the_kernel_forms_the_gpu_tests_launch():
