@@ -10,6 +10,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "sonar_layer.h"
 
@@ -36,15 +37,16 @@ int dtype_code(const Tensor& t, const char* name) {
 // The rows of `t` (its last dimension, `cols` long) behind each other, `stride` apart: `t` itself where its strides say
 // so, else a copy.  Rows that share memory (an expanded tensor) are copied too.
 Tensor rows_of(const Tensor& t, int64_t cols, int64_t& stride) {
-  Tensor rows = t.reshape({-1, cols});
+  Tensor rows = t.dim() == 2 ? t : t.reshape({-1, cols});
   if (rows.numel() > 0 && ((cols > 1 && rows.stride(1) != 1) || (rows.size(0) > 1 && rows.stride(0) < cols))) rows = rows.contiguous();
   stride = rows.size(0) > 1 ? rows.stride(0) : cols;
   return rows;
 }
 
 // ---------------------------------------------------------------- norm
-std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm_per_token_quant(const Tensor& x, const Tensor& weight, const OptTensor& residual,
-                                                                    double epsilon, at::ScalarType quant_dtype, bool with_norm) {
+// {codes, scales}, then z where there is a residual, then the norm where it is asked for
+std::vector<Tensor> rms_norm_per_token_quant(const Tensor& x, const Tensor& weight, const OptTensor& residual, double epsilon,
+                                             at::ScalarType quant_dtype, bool with_norm) {
   TORCH_CHECK(x.is_cuda(), "x is not on GPU");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have a non-empty last dimension");
   const int dtype = dtype_code(x, "x");
@@ -65,14 +67,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rms_norm_per_token_quant(const Tensor
   auto scale_shape = x.sizes().vec();
   scale_shape.back() = 1;
   Tensor scales = at::empty(scale_shape, x.options().dtype(at::kFloat));
-  Tensor sum = residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-  Tensor norm = with_norm ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  Tensor sum = residual.has_value() ? at::empty(x.sizes(), x.options()) : Tensor();
+  Tensor norm = with_norm ? at::empty(x.sizes(), x.options()) : Tensor();
   raise_if_failed(sonar_rms_norm_per_token_quant(
       in.const_data_ptr(), x_stride, residual.has_value() ? old.const_data_ptr() : nullptr, residual_stride,
       scale_of_column.const_data_ptr(), residual.has_value() ? sum.mutable_data_ptr() : nullptr,
       with_norm ? norm.mutable_data_ptr() : nullptr, q.mutable_data_ptr(), fp8 ? SONAR_ADTYPE_FP8 : SONAR_ADTYPE_INT8,
       static_cast<float*>(scales.mutable_data_ptr()), dtype, in.size(0), cols, epsilon, current_stream(x)));
-  return {q, scales, sum, norm};
+  std::vector<Tensor> results{std::move(q), std::move(scales)};
+  if (residual.has_value()) results.push_back(std::move(sum));
+  if (with_norm) results.push_back(std::move(norm));
+  return results;
 }
 
 // ---------------------------------------------------------------- int8 product
@@ -148,7 +153,7 @@ std::tuple<Tensor, Tensor> topk_routing(const Tensor& logits, int64_t topk, c10:
 TORCH_LIBRARY_FRAGMENT(sonar_amd, m) {
   m.def(
       "rms_norm_per_token_quant(Tensor x, Tensor weight, Tensor? residual, float epsilon, ScalarType quant_dtype, bool with_norm) "
-      "-> (Tensor, Tensor, Tensor, Tensor)");
+      "-> Tensor[]");
   m.def(
       "scaled_mm_int8(Tensor a, Tensor b, Tensor a_scales, Tensor b_scales, ScalarType out_dtype, Tensor? bias) -> Tensor");
   m.def(

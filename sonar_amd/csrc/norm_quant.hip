@@ -1,5 +1,13 @@
-// Root-mean-square norm with the residual's addition before it and 8-bit codes with one scale a token behind it.
+// Root-mean-square norm with the residual's addition before it and 8-bit codes with one scale a token behind it:
+//   z = T(x + residual);  r = 1 / sqrt(mean(z^2) + epsilon);  y = (z * r) * weight;  codes of y against its largest magnitude
+// The sum of squares and r are held in 64 bits and r is rounded once, y and the codes' arithmetic are float32, so that the
+// result does not depend on the order of the sum (but for one r in 2^24): a code is a rounding of y, and one last bit of r
+// would turn some.
+//
+// One pass over memory: a row is read once, z stays in registers (16 bits a number where the type has 16), y is formed
+// twice, for the maximum and for the codes.  Bound by the bytes.
 #include "common.hpp"
+#include "lane_reduce.hpp"
 #include "sonar_layer.h"
 
 namespace sonar {
@@ -12,10 +20,23 @@ namespace {
 
 constexpr int kThreads = 256;
 
+struct NormParams {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* residual_out;
+  void* norm_out;
+  uint8_t* q;
+  float* scales;
+  long x_stride, residual_stride, rows;
+  int cols;
+  double epsilon;
+};
+
+// Joins over a workgroup; `part` may be used again behind another call's barrier.
 template <typename V, typename F>
-__device__ __forceinline__ V across_block(V v, V* part, F join) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = join(v, __shfl_xor(v, off, 64));
+__device__ __forceinline__ V over_block(V v, V none, V* part, F join) {
+  v = over_wave(v, none, join);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   v = part[0];
@@ -24,37 +45,20 @@ __device__ __forceinline__ V across_block(V v, V* part, F join) {
   return v;
 }
 
-// One workgroup a row, element by element; z is read again in each pass.
-template <typename T, bool FP8>
-__global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const T* x, long x_stride, const T* residual, long residual_stride,
-                                                                  const T* __restrict__ weight, T* residual_out, T* norm_out,
-                                                                  uint8_t* __restrict__ q, float* __restrict__ scales, int cols,
-                                                                  double epsilon) {
-#pragma clang fp contract(off)
-  __shared__ double sums[kThreads / 64];
-  __shared__ float mosts[kThreads / 64];
-  const long row = blockIdx.x;
-  const T* in = x + row * x_stride;
-  const T* z = in;
-  double sum = 0;
-  if (residual != nullptr) {
-    T* out = residual_out + row * cols;
-    for (int c = threadIdx.x; c < cols; c += kThreads) {
-      const T v = (T)((float)in[c] + (float)residual[row * residual_stride + c]);
-      out[c] = v;
-      sum += (double)(float)v * (double)(float)v;
-    }
-    z = out;
-  } else {
-    for (int c = threadIdx.x; c < cols; c += kThreads) sum += (double)(float)in[c] * (double)(float)in[c];
+// 1 / sqrt(x) for x >= 2^-126 (or infinite, NaN), rounded once: an estimate of 2^-24 or better, two of Newton's steps.
+__device__ __forceinline__ float inverse_root(double x) {
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const double e = __builtin_fma(-x * y, y, 1.0);
+    y = __builtin_fma(y * e, 0.5, y);
   }
-  sum = across_block(sum, sums, [](double a, double b) { return a + b; });
-  const float r = (float)(1.0 / sqrt(sum / cols + epsilon));
-  float most = 0.0f;
-  for (int c = threadIdx.x; c < cols; c += kThreads) most = fmaxf(most, fabsf((float)z[c] * r * (float)weight[c]));
-  most = across_block(most, mosts, [](float a, float b) { return fmaxf(a, b); });
-  const bool finite = sum <= 1.7976931348623157e308;   // false for infinities and NaN
-  float by, scale;
+  return x <= 1.7976931348623157e308 ? (float)y : (float)(x - x);   // (infinities and NaN: NaN)
+}
+
+// A row's scale, and what its numbers are multiplied by; `r` NaN marks a row whose sum is none.
+template <bool FP8>
+__device__ __forceinline__ void scale_of(float most, float r, float& scale, float& by) {
   if (FP8) {
     scale = fmaxf(most / 448.0f, 1.0f / (448.0f * 512.0f));
     by = 1.0f / scale;
@@ -63,29 +67,202 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const T* x, lo
     scale = most / 127.0f;
     by = 127.0f / most;
   }
-  if (threadIdx.x == 0) scales[row] = finite ? scale : __builtin_nanf("");
-  for (int c = threadIdx.x; c < cols; c += kThreads) {
-    const float y = (float)z[c] * r * (float)weight[c];
-    if (norm_out != nullptr) norm_out[row * cols + c] = (T)y;
-    const float t = y * by;
-    uint8_t code;
-    if (FP8) code = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(t, -448.0f), 448.0f), 0.0f, 0, false) & 0xff);
-    else code = (uint8_t)(int)(t + copysignf(0.5f, t));
-    q[row * cols + c] = finite ? code : 0;
+  if (r != r) scale = r;
+}
+
+// A code in the low byte: halves away from zero (int8), the nearest float8_e4m3fn.  A NaN's is 0 (int8).
+__device__ __forceinline__ int int8_code(float y, float by) {
+#pragma clang fp contract(off)
+  const float t = y * by;
+  return (int)(t + __builtin_copysignf(0.5f, t)) & 0xff;
+}
+__device__ __forceinline__ float fp8_number(float y, float by) {
+#pragma clang fp contract(off)
+  const float t = y * by;
+  return fminf(fmaxf(t, -448.0f), 448.0f);
+}
+
+// Eight neighbouring numbers.
+template <typename T>
+struct Eight {
+  typedef T vec __attribute__((ext_vector_type(8)));
+  vec v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const vec*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<vec*>(p) = v; }
+  __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
+};
+
+// THREADS (64 or 256) a row, eight neighbouring columns of a row's KEPT turns a thread.  THREADS = 64: four rows a workgroup,
+// sums and maxima by lane moves, no barrier.  THREADS = 256: rows too long for a wavefront's registers, which beyond KEPT
+// turns are read again (as z), or too few to fill the card with wavefronts.  Workgroups go on from row to row with the
+// weight in registers.  16384 x 4096 bf16 to int8 with a residual (470 MB): 220 us element by element with three passes.
+template <typename T, bool FP8, int THREADS, int KEPT>
+__global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormParams p) {
+#pragma clang fp contract(off)
+  constexpr int kRows = kThreads / THREADS, kStep = THREADS * 8;
+  __shared__ double sums[kThreads / 64];
+  __shared__ float mosts[kThreads / 64];
+  const int first = threadIdx.x % THREADS * 8, cols = p.cols;
+  Eight<T> weight[KEPT], z[KEPT];
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i)
+    if (first + i * kStep < cols) weight[i].load((const T*)p.weight + first + i * kStep);
+  for (long row = (long)blockIdx.x * kRows + threadIdx.x / THREADS; row < p.rows; row += (long)gridDim.x * kRows) {
+    const T* x = (const T*)p.x + row * p.x_stride;
+    const T* residual = (const T*)p.residual + row * p.residual_stride;
+    T* out = (T*)p.residual_out + row * cols;
+    double sum = 0;
+    auto add = [&](const Eight<T>& v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)v.at(e), (double)v.at(e), sum);
+    };
+    auto join = [&](Eight<T>& v, const Eight<T>& r, int c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.v[e] = (T)(v.at(e) + r.at(e));
+      v.store(out + c);
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (first + i * kStep < cols) z[i].load(x + first + i * kStep);
+    if (p.residual != nullptr) {
+      Eight<T> more[KEPT];
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (first + i * kStep < cols) more[i].load(residual + first + i * kStep);
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (first + i * kStep < cols) join(z[i], more[i], first + i * kStep);
+    }
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (first + i * kStep < cols) add(z[i]);
+    const T* again = p.residual != nullptr ? out : x;   // z of the turns that no register keeps
+    if (THREADS > 64)
+      for (int c = first + KEPT * kStep; c < cols; c += kStep) {
+        Eight<T> v;
+        v.load(x + c);
+        if (p.residual != nullptr) {
+          Eight<T> more;
+          more.load(residual + c);
+          join(v, more, c);
+        }
+        add(v);
+      }
+    sum = THREADS == 64 ? wave_sum(sum) : over_block(sum, 0.0, sums, [](double a, double b) { return a + b; });
+    const float r = inverse_root(sum / cols + p.epsilon);
+    float most = 0.0f;
+    auto larger = [&](const Eight<T>& v, const Eight<T>& w) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v.at(e) * r * w.at(e)));
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (first + i * kStep < cols) larger(z[i], weight[i]);
+    if (THREADS > 64)
+      for (int c = first + KEPT * kStep; c < cols; c += kStep) {
+        Eight<T> v, w;
+        v.load(again + c), w.load((const T*)p.weight + c);
+        larger(v, w);
+      }
+    auto max_of = [](float a, float b) { return fmaxf(a, b); };
+    most = THREADS == 64 ? over_wave(most, 0.0f, max_of) : over_block(most, 0.0f, mosts, max_of);
+    float scale, by;
+    scale_of<FP8>(most, r, scale, by);
+    if (first == 0) p.scales[row] = scale;
+    auto code = [&](const Eight<T>& v, const Eight<T>& w, int c) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = v.at(e) * r * w.at(e);
+      if (p.norm_out != nullptr) {
+        Eight<T> n;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n.v[e] = (T)y[e];
+        n.store((T*)p.norm_out + row * cols + c);
+      }
+      uint32_t word[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (FP8) {
+          const int low = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_number(y[4 * h], by), fp8_number(y[4 * h + 1], by), 0, false);
+          word[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(fp8_number(y[4 * h + 2], by), fp8_number(y[4 * h + 3], by), low, true);
+        } else {
+          word[h] = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) word[h] |= (uint32_t)int8_code(y[4 * h + e], by) << (8 * e);
+        }
+      }
+      *reinterpret_cast<uint2*>(p.q + row * cols + c) = make_uint2(word[0], word[1]);
+    };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (first + i * kStep < cols) code(z[i], weight[i], first + i * kStep);
+    if (THREADS > 64)
+      for (int c = first + KEPT * kStep; c < cols; c += kStep) {
+        Eight<T> v, w;
+        v.load(again + c), w.load((const T*)p.weight + c);
+        code(v, w, c);
+      }
   }
 }
 
-template <bool FP8>
-int launch(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, void* residual_out,
-           void* norm_out, void* q, float* scales, int dtype, int64_t rows, int64_t cols, double epsilon, hipStream_t st) {
-#define SONAR_NORM(T)                                                                                                       \
-  rms_norm_quant_kernel<T, FP8><<<(int)rows, kThreads, 0, st>>>((const T*)x, x_stride, (const T*)residual, residual_stride, \
-                                                                (const T*)weight, (T*)residual_out, (T*)norm_out,           \
-                                                                (uint8_t*)q, scales, (int)cols, epsilon)
-  if (dtype == SONAR_DTYPE_F16) SONAR_NORM(_Float16);
-  else if (dtype == SONAR_DTYPE_BF16) SONAR_NORM(__bf16);
-  else SONAR_NORM(float);
-#undef SONAR_NORM
+// Any column count, stride and alignment: a workgroup a row, element by element; z is read again in each pass.
+template <typename T, bool FP8>
+__global__ __launch_bounds__(kThreads) void rms_norm_quant_any_kernel(const NormParams p) {
+#pragma clang fp contract(off)
+  __shared__ double sums[kThreads / 64];
+  __shared__ float mosts[kThreads / 64];
+  const int cols = p.cols;
+  const T* weight = (const T*)p.weight;
+  for (long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T* z = (const T*)p.x + row * p.x_stride;
+    double sum = 0;
+    if (p.residual != nullptr) {
+      const T* residual = (const T*)p.residual + row * p.residual_stride;
+      T* out = (T*)p.residual_out + row * cols;
+      for (int c = threadIdx.x; c < cols; c += kThreads) {
+        const T v = (T)((float)z[c] + (float)residual[c]);
+        out[c] = v;
+        sum = __builtin_fma((double)(float)v, (double)(float)v, sum);
+      }
+      z = out;
+    } else {
+      for (int c = threadIdx.x; c < cols; c += kThreads) sum = __builtin_fma((double)(float)z[c], (double)(float)z[c], sum);
+    }
+    sum = over_block(sum, 0.0, sums, [](double a, double b) { return a + b; });
+    const float r = inverse_root(sum / cols + p.epsilon);
+    float most = 0.0f;
+    for (int c = threadIdx.x; c < cols; c += kThreads) most = fmaxf(most, fabsf((float)z[c] * r * (float)weight[c]));
+    most = over_block(most, 0.0f, mosts, [](float a, float b) { return fmaxf(a, b); });
+    float scale, by;
+    scale_of<FP8>(most, r, scale, by);
+    if (threadIdx.x == 0) p.scales[row] = scale;
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+      const float y = (float)z[c] * r * (float)weight[c];
+      if (p.norm_out != nullptr) ((T*)p.norm_out)[row * cols + c] = (T)y;
+      p.q[row * cols + c] = FP8 ? (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(fp8_number(y, by), 0.0f, 0, false) & 0xff)
+                                : (uint8_t)int8_code(y, by);
+    }
+  }
+}
+
+template <typename T, bool FP8>
+int launch(const NormParams& p, hipStream_t st) {
+  auto at_16 = [](const void* q) { return (uintptr_t)q % 16 == 0; };
+  const long pitch = (long)(16 / sizeof(T));
+  const bool vectors = p.cols % 8 == 0 && at_16(p.x) && at_16(p.residual) && at_16(p.weight) && at_16(p.residual_out) &&
+                       at_16(p.norm_out) && (uintptr_t)p.q % 8 == 0 && p.x_stride % pitch == 0 && p.residual_stride % pitch == 0;
+  const long most = 256 * 8;   // workgroups: a compute unit holds eight at most
+  if (!vectors) {
+    rms_norm_quant_any_kernel<T, FP8><<<(int)(p.rows < most ? p.rows : most), kThreads, 0, st>>>(p);
+    return launch_status("rms_norm_quant_any_kernel");
+  }
+  const bool waves = p.cols <= 512 || (p.cols <= 4096 && p.rows >= 2048);
+  const long groups = waves ? (p.rows + 3) / 4 : p.rows;
+  const int grid = (int)(groups < most ? groups : most);
+  if (waves && p.cols <= 1024) rms_norm_quant_kernel<T, FP8, 64, 2><<<grid, kThreads, 0, st>>>(p);
+  else if (waves) rms_norm_quant_kernel<T, FP8, 64, 8><<<grid, kThreads, 0, st>>>(p);
+  else if (p.cols <= 4096) rms_norm_quant_kernel<T, FP8, 256, 2><<<grid, kThreads, 0, st>>>(p);
+  else rms_norm_quant_kernel<T, FP8, 256, 8><<<grid, kThreads, 0, st>>>(p);
   return launch_status("rms_norm_quant_kernel");
 }
 
@@ -112,10 +289,11 @@ extern "C" int sonar_rms_norm_per_token_quant(const void* x, int64_t x_row_strid
   if (rows == 0) return SONAR_OK;
   SONAR_REQUIRE(x && weight && q && scales, "x, weight, q and scales must not be NULL");
   SONAR_REQUIRE((residual == nullptr) == (residual_out == nullptr), "residual and residual_out go together");
+  const NormParams p{x, residual, weight, residual_out, norm_out, (uint8_t*)q, scales, x_row_stride, residual ? residual_row_stride : 0,
+                     rows, (int)cols, epsilon};
   hipStream_t st = (hipStream_t)stream;
-  return q_dtype == SONAR_ADTYPE_FP8
-             ? launch<true>(x, x_row_stride, residual, residual_row_stride, weight, residual_out, norm_out, q, scales, dtype, rows,
-                            cols, epsilon, st)
-             : launch<false>(x, x_row_stride, residual, residual_row_stride, weight, residual_out, norm_out, q, scales, dtype, rows,
-                             cols, epsilon, st);
+  const bool fp8 = q_dtype == SONAR_ADTYPE_FP8;
+  if (dtype == SONAR_DTYPE_F16) return fp8 ? launch<_Float16, true>(p, st) : launch<_Float16, false>(p, st);
+  if (dtype == SONAR_DTYPE_BF16) return fp8 ? launch<__bf16, true>(p, st) : launch<__bf16, false>(p, st);
+  return fp8 ? launch<float, true>(p, st) : launch<float, false>(p, st);
 }

@@ -68,11 +68,8 @@ def _register_fakes() -> None:
 
     @reg("sonar_amd::rms_norm_per_token_quant")
     def _(x, weight, residual, epsilon, quant_dtype, with_norm):
-        q, scales = quant_fake(quant_dtype)(x)
-
-        def like_x(wanted):   # the op answers contiguous tensors
-            return torch.empty(x.shape if wanted else (0,), dtype=x.dtype, device=x.device)
-        return q, scales, like_x(residual is not None), like_x(with_norm)
+        more = (residual is not None) + bool(with_norm)
+        return [*quant_fake(quant_dtype)(x), *(torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(more))]
 
     @reg("sonar_amd::scaled_mm_int8")
     def _(a, b, a_scales, b_scales, out_dtype, bias):
@@ -216,6 +213,12 @@ def per_token_quant_fp8(x: torch.Tensor):
     return torch.ops.sonar_amd.per_token_quant_fp8(x)
 
 
+# (the ops themselves, not the names that look for an overload at every call)
+_rms_norm_per_token_quant = torch.ops.sonar_amd.rms_norm_per_token_quant.default
+_scaled_mm_int8 = torch.ops.sonar_amd.scaled_mm_int8.default
+_topk_routing = torch.ops.sonar_amd.topk_routing.default
+
+
 def rms_norm_per_token_quant(x: torch.Tensor, weight: torch.Tensor, epsilon: float,
                              quant_dtype: torch.dtype = torch.int8, residual: torch.Tensor | None = None,
                              with_norm: bool = False):
@@ -229,8 +232,8 @@ def rms_norm_per_token_quant(x: torch.Tensor, weight: torch.Tensor, epsilon: flo
     `a_scales`; z where a residual was given, the next residual, else None; y rounded to x's type where `with_norm`
     (for a router, which reads 16 bits), else None.  The codes are those of y itself, not of the rounded norm.
     A row with an infinity or a NaN in z has the scale NaN."""
-    q, scales, z, norm = torch.ops.sonar_amd.rms_norm_per_token_quant(x, weight, residual, epsilon, quant_dtype, with_norm)
-    return q, scales, z if residual is not None else None, norm if with_norm else None
+    got = _rms_norm_per_token_quant(x, weight, residual, epsilon, quant_dtype, with_norm)
+    return got[0], got[1], got[2] if residual is not None else None, got[-1] if with_norm else None
 
 
 def scaled_mm_int8(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_scales: torch.Tensor,
@@ -241,7 +244,7 @@ def scaled_mm_int8(a: torch.Tensor, b: torch.Tensor, a_scales: torch.Tensor, b_s
     a: int8 (..., K).  b: int8 (K, N), column by column: `weight.t()` of a checkpoint's (N, K) weight, read as it lies.
     a_scales: float32, one a token or one in all; b_scales: one a channel or one in all.  out_dtype: float16 or
     bfloat16; bias: (N,) of out_dtype.  K below 131072, where the sum could leave 32 bits."""
-    return torch.ops.sonar_amd.scaled_mm_int8(a, b, a_scales, b_scales, out_dtype, bias)
+    return _scaled_mm_int8(a, b, a_scales, b_scales, out_dtype, bias)
 
 
 def topk_routing(gating_output: torch.Tensor, topk: int, scoring_func: str = "softmax", renormalize: bool = False,
@@ -257,8 +260,8 @@ def topk_routing(gating_output: torch.Tensor, topk: int, scoring_func: str = "so
     the chosen, divided by their sum if `renormalize`, times routed_scaling_factor.  A NaN logit counts as -inf; a token
     whose logits are all -inf gets the lowest experts that may be chosen, with softmax weights 0.  At most 1024 experts,
     64 groups, 64 choices."""
-    return torch.ops.sonar_amd.topk_routing(gating_output, topk, scoring_func, renormalize, bias, num_expert_group,
-                                            topk_group, routed_scaling_factor)
+    return _topk_routing(gating_output, topk, scoring_func, renormalize, bias, num_expert_group, topk_group,
+                         routed_scaling_factor)
 
 
 def marlin_gemm(a: torch.Tensor, c: torch.Tensor | None, b_q_weight: torch.Tensor,

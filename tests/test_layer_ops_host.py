@@ -129,7 +129,7 @@ def test_schemas():
     import sonar_amd.ops  # noqa: F401
     for name, want in (
             ("rms_norm_per_token_quant", "(Tensor x, Tensor weight, Tensor? residual, float epsilon, ScalarType quant_dtype, "
-             "bool with_norm) -> (Tensor, Tensor, Tensor, Tensor)"),
+             "bool with_norm) -> Tensor[]"),
             ("scaled_mm_int8", "(Tensor a, Tensor b, Tensor a_scales, Tensor b_scales, ScalarType out_dtype, Tensor? bias) -> Tensor"),
             ("topk_routing", "(Tensor logits, int topk, str scoring_func, bool renormalize, Tensor? bias, int num_expert_group, "
              "int topk_group, float routed_scaling_factor) -> (Tensor, Tensor)")):
@@ -228,7 +228,7 @@ def test_oracle_values():
     assert c.tolist() == [[-1.5, -382.0]]
 
 
-KERNEL_FORMS = {"rms_norm_quant_kernel": 6, "int8_general_kernel": 2, "topk_routing_kernel": 3, "int8_stream_kernel": 6,
+KERNEL_FORMS = {"rms_norm_quant_kernel": 24, "rms_norm_quant_any_kernel": 6, "int8_general_kernel": 2, "topk_routing_kernel": 3, "int8_stream_kernel": 6,
                 "int8_tile_kernel": 10, "int8_join_kernel": 10, "int8_pad_kernel": 1}
 
 
