@@ -1,6 +1,7 @@
 // Torch op registration of the operators of sonar_layer.h, in the library's own namespace `sonar_amd`.  No kernels live
 // here: argument checks, the tensors of the results, and the call of the C ABI on the current stream of the inputs' device.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <hip/hip_runtime_api.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -34,6 +35,12 @@ int dtype_code(const Tensor& t, const char* name) {
   return SONAR_DTYPE_F32;
 }
 
+// A new contiguous tensor on t's device, straight from the allocator: at::empty finds the same function through the
+// dispatcher, which a call of a few microseconds would feel.
+Tensor new_tensor(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, at::kStrided, t.device(), std::nullopt, std::nullopt);
+}
+
 // The rows of `t` (its last dimension, `cols` long) behind each other, `stride` apart: `t` itself where its strides say
 // so, else a copy.  Rows that share memory (an expanded tensor) are copied too.
 Tensor rows_of(const Tensor& t, int64_t cols, int64_t& stride) {
@@ -63,12 +70,12 @@ std::vector<Tensor> rms_norm_per_token_quant(const Tensor& x, const Tensor& weig
   const Tensor in = rows_of(x, cols, x_stride), scale_of_column = weight.contiguous();
   const Tensor old = residual.has_value() ? rows_of(*residual, cols, residual_stride) : Tensor();
   const bool fp8 = quant_dtype == at::kFloat8_e4m3fn;
-  Tensor q = at::empty(x.sizes(), x.options().dtype(quant_dtype));
+  Tensor q = new_tensor(x, x.sizes(), quant_dtype);
   auto scale_shape = x.sizes().vec();
   scale_shape.back() = 1;
-  Tensor scales = at::empty(scale_shape, x.options().dtype(at::kFloat));
-  Tensor sum = residual.has_value() ? at::empty(x.sizes(), x.options()) : Tensor();
-  Tensor norm = with_norm ? at::empty(x.sizes(), x.options()) : Tensor();
+  Tensor scales = new_tensor(x, scale_shape, at::kFloat);
+  Tensor sum = residual.has_value() ? new_tensor(x, x.sizes(), x.scalar_type()) : Tensor();
+  Tensor norm = with_norm ? new_tensor(x, x.sizes(), x.scalar_type()) : Tensor();
   raise_if_failed(sonar_rms_norm_per_token_quant(
       in.const_data_ptr(), x_stride, residual.has_value() ? old.const_data_ptr() : nullptr, residual_stride,
       scale_of_column.const_data_ptr(), residual.has_value() ? sum.mutable_data_ptr() : nullptr,
@@ -103,7 +110,7 @@ Tensor scaled_mm_int8(const Tensor& a, const Tensor& b, const Tensor& a_scales, 
     TORCH_CHECK(bias->device() == a.device() && bias->scalar_type() == out_dtype && bias->numel() == n, "bias must hold ", n,
                 " numbers of out_dtype on a's device");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(a.device());
-  Tensor c = at::empty(shape, a.options().dtype(out_dtype));
+  Tensor c = new_tensor(a, shape, out_dtype);
   int64_t lda = k;
   const Tensor rows = k > 0 ? rows_of(a, k, lda) : a;
   const Tensor sa = a_scales.contiguous(), sb = b_scales.contiguous(), bc = bias.has_value() ? bias->contiguous() : Tensor();
@@ -113,7 +120,7 @@ Tensor scaled_mm_int8(const Tensor& a, const Tensor& b, const Tensor& a_scales, 
   const size_t scratch_bytes =
       sonar_scaled_mm_int8_scratch_bytes(m, n, k, bits % 16 == 0 && lda < (1 << 23) && ldb < (1 << 23) ? 1 : 0);
   Tensor scratch;
-  if (scratch_bytes > 0) scratch = at::empty({(int64_t)scratch_bytes}, a.options().dtype(at::kByte));
+  if (scratch_bytes > 0) scratch = new_tensor(a, {(int64_t)scratch_bytes}, at::kByte);
   raise_if_failed(sonar_scaled_mm_int8(
       static_cast<const int8_t*>(rows.const_data_ptr()), lda, static_cast<const int8_t*>(b.const_data_ptr()),
       ldb, c.mutable_data_ptr(), static_cast<const float*>(sa.const_data_ptr()), sa.numel(),
@@ -138,8 +145,8 @@ std::tuple<Tensor, Tensor> topk_routing(const Tensor& logits, int64_t topk, c10:
   int64_t stride = experts;
   const Tensor rows = experts > 0 ? rows_of(logits, experts, stride) : logits;
   const Tensor bc = bias.has_value() ? bias->contiguous() : Tensor();
-  Tensor weights = at::empty({logits.size(0), std::max<int64_t>(topk, 0)}, logits.options().dtype(at::kFloat));
-  Tensor ids = at::empty({logits.size(0), std::max<int64_t>(topk, 0)}, logits.options().dtype(at::kInt));
+  Tensor weights = new_tensor(logits, {logits.size(0), std::max<int64_t>(topk, 0)}, at::kFloat);
+  Tensor ids = new_tensor(logits, {logits.size(0), std::max<int64_t>(topk, 0)}, at::kInt);
   raise_if_failed(sonar_topk_routing(
       rows.const_data_ptr(), dtype, stride, bias.has_value() ? static_cast<const float*>(bc.const_data_ptr()) : nullptr,
       static_cast<float*>(weights.mutable_data_ptr()), static_cast<int32_t*>(ids.mutable_data_ptr()), logits.size(0), experts, topk,

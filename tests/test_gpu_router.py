@@ -1,7 +1,7 @@
 """GPU: the router against the 64-bit oracle.  The experts are equal number by number.  Weights, with u = 2^-24: a softmax
-term e^d (d the distance to the largest logit) is off by at most (|d| + 3) u where it is taken in float32, so the sum of the
-terms by the mean of |d| + 3 over them (at most ln 1024 + 3 < 10) u and 22 u of its additions; a quotient, a factor and the
-result's rounding add 4 u: 40 u with the chosen term itself taken in 64 bits."""
+term e^d (d the distance to the largest logit, off by |d| u) is off by at most (2 |d| + 3) u where it is taken in float32, so
+the sum of the terms by the mean of that over them (|d| is ln 1024 at most in the mean: 17 u) and 21 u of its additions; the
+result's rounding adds one: 40 u with the chosen term itself, the quotients and the factor taken in 64 bits."""
 import numpy as np
 import pytest
 import torch
