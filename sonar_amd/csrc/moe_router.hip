@@ -5,10 +5,13 @@
 // float32 sums are equal are told apart, as a 64-bit program would.
 //
 // A choice is kept as two words whose unsigned order is that of the numbers: its float32 rounding and what that leaves (no
-// second word without a bias).  Every round finds the largest first word over a token's lanes by lane moves, asks which
-// lanes have it, looks at the second words only if there are several, and takes the lowest.  Word 0 is below every number's:
-// an expert that is taken, left out or not there.
-// Bound by the vector instructions of the rounds and, with a bias, of the 64-bit exponentials.
+// second word without a bias).  A lane holds R neighbouring experts of a token and knows the largest of them.  Every round finds
+// the largest first word over the token's lanes by lane moves, asks which lanes have it (and looks at the second words
+// only if several have), takes the lowest lane's lowest expert, and that lane looks for its next.  Word 0 is below every
+// number's: an expert that is taken, left out or not there.
+// Bound by the vector instructions of the rounds, and by the latency of their chains where tokens are few.  16384 x 256, sigmoid,
+// bias, 4 of 8 groups: 132 us with choices and 64-bit maxima in LDS, 28.5 so.  (Choices in float32 first, and in 64 bits only
+// for the tokens where two come near each other: 31.6.)
 #include "common.hpp"
 #include "lane_reduce.hpp"
 #include "sonar_layer.h"
@@ -17,6 +20,7 @@ namespace sonar {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxGroups = 64, kMaxTopk = 64, kWaves = 4;
+
 
 struct RouterParams {
   const void* logits;
@@ -38,7 +42,31 @@ __device__ __forceinline__ float number_of(uint32_t w) {
   return __builtin_bit_cast(float, w ^ (w & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
 
-// A number no NaN: a NaN counts as -infinity
+// The logits of experts e0 .. e0 + R - 1 of a row; -infinity for a NaN and behind the end.  `vectors`: 16 bytes at a time lie
+// aligned and whole in the row.
+template <typename T, int R>
+__device__ __forceinline__ void load_logits(const T* row, int e0, int E, bool vectors, float (&x)[R]) {
+  constexpr int kVec = 16 / sizeof(T);
+  typedef T vec_t __attribute__((ext_vector_type(kVec)));
+  const float inf = __builtin_inff();
+  if (R >= kVec && vectors) {
+#pragma unroll
+    for (int i = 0; i < R / kVec; ++i) {
+      const int e = e0 + i * kVec;
+      const vec_t v = *reinterpret_cast<const vec_t*>(row + (e < E ? e : 0));
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) x[i * kVec + j] = e < E ? (float)v[j] : -inf;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = (float)row[min(e0 + r, E - 1)];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = e0 + r < E ? x[r] : -inf;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) x[r] = x[r] == x[r] ? x[r] : -inf;
+}
+
 __device__ __forceinline__ float logit_at(const RouterParams& p, long at) {
   float f;
   if (p.dtype == SONAR_DTYPE_F32) f = ((const float*)p.logits)[at];
@@ -47,80 +75,118 @@ __device__ __forceinline__ float logit_at(const RouterParams& p, long at) {
   return f == f ? f : -__builtin_inff();
 }
 
+// e^-d for d >= 0 (also infinite): 2^n e^r with |r| <= ln(2) / 2, and the series of e^r to r^13, whose rest is below 2^-57.
+// The relative error grows with d, by 2^-53 for each of its units; that of a score by less, since e^-d falls faster.
+__device__ __forceinline__ double exp_minus(double d) {
+  const double t = -fmin(d, 800.0);
+  const double n = __builtin_rint(t * 1.4426950408889634);
+  const double r = __builtin_fma(-n, 1.9082149292705877e-10, __builtin_fma(-n, 0.6931471803691238, t));   // ln 2 in two parts
+  double e = 1.0 / 6227020800.0;
+  e = __builtin_fma(e, r, 1.0 / 479001600.0);
+  e = __builtin_fma(e, r, 1.0 / 39916800.0);
+  e = __builtin_fma(e, r, 1.0 / 3628800.0);
+  e = __builtin_fma(e, r, 1.0 / 362880.0);
+  e = __builtin_fma(e, r, 1.0 / 40320.0);
+  e = __builtin_fma(e, r, 1.0 / 5040.0);
+  e = __builtin_fma(e, r, 1.0 / 720.0);
+  e = __builtin_fma(e, r, 1.0 / 120.0);
+  e = __builtin_fma(e, r, 1.0 / 24.0);
+  e = __builtin_fma(e, r, 1.0 / 6.0);
+  e = __builtin_fma(e, r, 0.5);
+  e = __builtin_fma(e, r, 1.0);
+  e = __builtin_fma(e, r, 1.0);
+  return __builtin_ldexp(e, (int)n);
+}
+// 1 / x for x between 1 and 2^20: an estimate and two of Newton's steps
+__device__ __forceinline__ double inverse(double x) {
+  double y = __builtin_amdgcn_rcp(x);
+  y = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+  return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+}
 // e^(x - top), 0 for x = -infinity, 1 at the top (where both may be infinite)
 __device__ __forceinline__ double term(float x, float top) {
-  return x == -__builtin_inff() ? 0.0 : x == top ? 1.0 : exp((double)x - (double)top);
+  const double e = exp_minus((double)top - (double)x);
+  return x == -__builtin_inff() ? 0.0 : x == top ? 1.0 : e;
 }
-__device__ __forceinline__ double sigmoid(float x) { return 1.0 / (1.0 + exp(-(double)x)); }
+__device__ __forceinline__ double sigmoid(float x) {
+  const double e = exp_minus(fabs((double)x)), y = inverse(1.0 + e);
+  return x >= 0 ? y : e * y;
+}
 
-// LANES of a wavefront a token, R experts a lane: experts lane, lane + LANES, ..  R = 1 below 64 lanes.
+// LANES of a wavefront a token, R experts a lane.
 template <int LANES, int R, bool BIASED>
-__global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterParams p) {
-  static_assert(R == 1 || LANES == 64, "");
+__global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterParams p, bool vectors) {
   constexpr int kTokens = 64 / LANES;
-  struct Chosen {
-    double value;   // the logit, or with a bias the score
-    int expert;
-  };
-  __shared__ Chosen chosen[kWaves][64];
-  extern __shared__ double all_choices[];   // [kWaves][experts], of calls with groups
+  __shared__ int chosen[kWaves][kTokens * kMaxTopk];
+  extern __shared__ double all_choices[];   // [kWaves][kTokens][experts], of calls with groups
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l = lane % LANES, seg = lane / LANES, E = p.experts;
+  const int l = lane % LANES, seg = lane / LANES, E = p.experts, e0 = l * R;
   const float inf = __builtin_inff();
   auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
   auto add = [](double a, double b) { return a + b; };
   for (long first = ((long)blockIdx.x * kWaves + wave) * kTokens; first < p.tokens; first += (long)gridDim.x * kWaves * kTokens) {
     const long token = first + seg;
     const bool there = token < p.tokens;
+    const long at = (there ? token : p.tokens - 1) * p.row_stride;
     float x[R];
     uint32_t key[R], low[R];   // of the choices
-    double score[R];
-    uint32_t top_key = 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int e = r * LANES + l;
-      x[r] = there && e < E ? logit_at(p, token * p.row_stride + e) : -inf;
-      top_key = larger(top_key, ordered(x[r]));
-    }
+    if (p.dtype == SONAR_DTYPE_F32) load_logits((const float*)p.logits + at, e0, E, vectors, x);
+    else if (p.dtype == SONAR_DTYPE_BF16) load_logits((const __bf16*)p.logits + at, e0, E, vectors, x);
+    else load_logits((const _Float16*)p.logits + at, e0, E, vectors, x);
     const bool softmax = p.scoring == SONAR_SCORING_SOFTMAX;
     float top = 0;
-    if (softmax) top = number_of(over_lanes<LANES>(top_key, larger));
+    if (softmax) {
+      uint32_t top_key = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) top_key = larger(top_key, ordered(x[r]));
+      top = number_of(over_lanes<LANES>(top_key, larger));
+    }
     double sum = 0;   // of a token's terms
     if (BIASED) {
+      double score[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) sum += score[r] = softmax ? term(x[r], top) : sigmoid(x[r]);
       if (softmax) sum = over_lanes<LANES>(sum, add);
-    } else if (softmax && !p.renormalize) {   // (renormalised weights need no sum over all)
-      float terms = 0;
+      if (softmax && sum > 0) {
+        const double scale = inverse(sum);
 #pragma unroll
-      for (int r = 0; r < R; ++r) terms += x[r] == -inf ? 0.0f : x[r] == top ? 1.0f : __expf(x[r] - top);
-      sum = over_lanes<LANES>((double)terms, add);
-    }
+        for (int r = 0; r < R; ++r) score[r] *= scale;
+      }
+      float bias[R];
+      load_logits(p.bias, e0, E, vectors, bias);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int e = r * LANES + l;
-      key[r] = low[r] = 0;
-      double choice = (double)x[r];
-      if (BIASED) {
-        if (softmax && sum > 0) score[r] /= sum;
-        choice = e < E ? score[r] + (double)p.bias[e] : 0.0;
+      for (int r = 0; r < R; ++r) {
+        double choice = score[r] + (double)bias[r];
         if (choice != choice) choice = -(double)inf;
         const float near = (float)choice, rest = (float)(choice - (double)near);
-        if (there && e < E) key[r] = ordered(near), low[r] = rest == rest ? ordered(rest) : ordered(0.0f);
-      } else if (there && e < E) {
-        key[r] = ordered(x[r]);
+        key[r] = ordered(near), low[r] = ordered(rest == rest ? rest : 0.0f);
+        if (p.groups > 1 && e0 + r < E) all_choices[(wave * kTokens + seg) * E + e0 + r] = choice;
       }
-      if (LANES == 64 && p.groups > 1 && e < E) all_choices[wave * E + e] = choice;
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        key[r] = ordered(x[r]);
+        if (p.groups > 1 && e0 + r < E) all_choices[(wave * kTokens + seg) * E + e0 + r] = (double)x[r];
+      }
+      if (softmax && !p.renormalize) {   // (renormalised weights need no sum over all)
+        float terms = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) terms += x[r] == -inf ? 0.0f : x[r] == top ? 1.0f : __expf(x[r] - top);
+        sum = over_lanes<LANES>((double)terms, add);
+      }
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = e0 + r < E ? key[r] : 0;
 
-    if (LANES == 64 && p.groups > 1) {
+    if (p.groups > 1) {
       // 2^n lanes a group, as many as there are: the two largest choices of each, a lane's share first
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const int size = E / p.groups, shift = 31 - __builtin_clz(64 / p.groups), g = lane >> shift, share = 1 << shift;
+      const int size = E / p.groups, shift = 31 - __builtin_clz(LANES / p.groups), g = l >> shift, share = 1 << shift;
+      const double* choices = all_choices + (wave * kTokens + seg) * E;
       double best = -(double)inf, second = best;
       if (g < p.groups)
-        for (int j = lane & (share - 1); j < size; j += share) {
-          const double c = all_choices[wave * E + g * size + j];
+        for (int j = l & (share - 1); j < size; j += share) {
+          const double c = choices[g * size + j];
           second = fmax(second, fmin(best, c));
           best = fmax(best, c);
         }
@@ -133,87 +199,114 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
       if (best != best) best = -(double)inf;
       int rank = 0;   // groups before this one
       for (int other = 0; other < p.groups; ++other) {
-        const double b = of_lane(best, other << shift);
+        const double b = __shfl(best, seg * LANES + (other << shift), 64);
         rank += b > best || (b == best && other < g) ? 1 : 0;
       }
-      const unsigned long long open = __ballot(g < p.groups && rank < p.kept_groups);
+      const unsigned long long open = __ballot(g < p.groups && rank < p.kept_groups) >> (seg * LANES);
       const float per_group = 1.0f / (float)size;   // (e + 1 / 2) / size is 2^-11 from a whole number at least
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int of = (int)(((float)(r * LANES + l) + 0.5f) * per_group);
+        const int of = (int)(((float)(e0 + r) + 0.5f) * per_group);
         if (!(open >> ((of << shift) & 63) & 1)) key[r] = 0;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 
-    for (int k = 0; k < p.topk; ++k) {
-      uint32_t best = key[0];
+    uint32_t best;   // of this lane's experts, by the first word
+    auto look = [&]() {
+      best = key[0];
 #pragma unroll
       for (int r = 1; r < R; ++r) best = larger(best, key[r]);
-      best = over_lanes<LANES>(best, larger);
-      unsigned long long have[R];
+    };
+    auto low_of_best = [&]() {
+      uint32_t most = 0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) have[r] = __ballot(key[r] == best);
-      if (BIASED) {
-        int count = 0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) count += __popcll(have[r]);
-        if (count != kTokens) {   // several with the same float32 number
-          uint32_t rest = 0;
-#pragma unroll
-          for (int r = 0; r < R; ++r) rest = larger(rest, key[r] == best ? low[r] : 0);
-          rest = over_lanes<LANES>(rest, larger);
-#pragma unroll
-          for (int r = 0; r < R; ++r) have[r] = __ballot(key[r] == best && low[r] == rest);
-        }
+      for (int r = 0; r < R; ++r) most = larger(most, key[r] == best ? low[r] : 0);
+      return most;
+    };
+    look();
+    for (int k = 0; k < p.topk; ++k) {
+      const uint32_t most = over_lanes<LANES>(best, larger);
+      bool has = best == most;
+      unsigned long long have = __ballot(has);
+      if (BIASED && __popcll(have) != kTokens) {   // several lanes with the same first word
+        const uint32_t mine_low = has ? low_of_best() : 0, rest = over_lanes<LANES>(mine_low, larger);
+        has = has && mine_low == rest;
+        have = __ballot(has);
       }
-      auto take = [&](int r) {
-        key[r] = 0;
-        chosen[wave][seg * LANES + k] = Chosen{BIASED ? score[r] : (double)x[r], r * LANES + l};
-      };
-      if (LANES < 64) {
-        const uint32_t mine = (uint32_t)(have[0] >> (seg * LANES));   // (a lane of the token has it, so the lowest one is of the token)
-        if (l == __builtin_ctz(mine | 0x80000000u)) take(0);
-      } else {
-        bool found = false;
+      bool mine;
+      if (LANES == 64) mine = lane == __builtin_ctzll(have);
+      else mine = l == __builtin_ctz((uint32_t)(have >> (seg * LANES)) | 0x80000000u);   // (a lane of the token has it: the lowest is the token's)
+      if (mine) {
+        int at_r = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (!found && have[r] != 0) {
-            found = true;
-            if (lane == __builtin_ctzll(have[r])) take(r);
+        for (int r = R - 1; r > 0; --r) at_r = key[r] == best ? r : at_r;
+        at_r = key[0] == best ? 0 : at_r;
+        if (BIASED && R > 1) {
+          int same = 0;
+#pragma unroll
+          for (int r = 0; r < R; ++r) same += key[r] == best ? 1 : 0;
+          if (same > 1) {   // several here with the same first word: by the second
+            const uint32_t rest = low_of_best();
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r) at_r = key[r] == best && low[r] == rest ? r : at_r;
           }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) key[r] = r == at_r ? 0 : key[r];
+        chosen[wave][seg * kMaxTopk + k] = e0 + at_r;
+        look();
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    double w = 0;
-    int expert = 0;
-    if (l < p.topk) {
-      const Chosen c = chosen[wave][seg * LANES + l];
-      expert = c.expert;
-      w = c.value;
-      if (!BIASED) {
-        w = softmax ? term((float)c.value, top) : sigmoid((float)c.value);
+    double total = 0;
+    for (int pass = p.renormalize ? 0 : 1; pass < 2; ++pass)   // the sum of the chosen scores, then the weights
+      for (int k = l; k < (p.topk + LANES - 1) / LANES * LANES; k += LANES) {
+        const int expert = chosen[wave][seg * kMaxTopk + min(k, p.topk - 1)];
+        const float logit = logit_at(p, at + expert);
+        double w = softmax ? term(logit, top) : sigmoid(logit);
         if (softmax && sum > 0) w /= sum;
+        if (pass == 0) {
+          total += over_lanes<LANES>(k < p.topk ? w : 0.0, add);
+        } else if (there && k < p.topk) {
+          if (total > 0) w /= total;
+          p.weights[token * p.topk + k] = (float)(w * p.factor);
+          p.ids[token * p.topk + k] = expert;
+        }
       }
-    }
-    if (p.renormalize) {
-      const double total = over_lanes<LANES>(w, add);
-      if (total > 0) w /= total;
-    }
-    if (there && l < p.topk) {
-      p.weights[token * p.topk + l] = (float)(w * p.factor);
-      p.ids[token * p.topk + l] = expert;
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
-template <int LANES, int R>
+template <int LANES, int R, bool BIASED>
 void launch(const RouterParams& p, hipStream_t st) {
+  const long size = p.dtype == SONAR_DTYPE_F32 ? 4 : 2;
+  const bool vectors = (uintptr_t)p.logits % 16 == 0 && p.row_stride * size % 16 == 0 && p.experts * size % 16 == 0 &&
+                       (uintptr_t)p.bias % 16 == 0;   // (experts: a multiple of four, whole vectors of the bias too)
   const long waves = (p.tokens + 64 / LANES - 1) / (64 / LANES), groups = (waves + kWaves - 1) / kWaves;
   const int grid = (int)(groups < (1 << 20) ? groups : 1 << 20);
-  const size_t lds = p.groups > 1 ? (size_t)kWaves * p.experts * sizeof(double) : 0;
-  if (p.bias != nullptr) topk_routing_kernel<LANES, R, true><<<grid, 64 * kWaves, lds, st>>>(p);
-  else topk_routing_kernel<LANES, R, false><<<grid, 64 * kWaves, lds, st>>>(p);
+  const size_t lds = p.groups > 1 ? (size_t)kWaves * (64 / LANES) * p.experts * sizeof(double) : 0;
+  topk_routing_kernel<LANES, R, BIASED><<<grid, 64 * kWaves, lds, st>>>(p, vectors);
+}
+
+// Few tokens: a wavefront each, for its latency.  From 4096 on, where every SIMD has some, several share one (16384 x 128, top 8:
+// 8.0 us, 17.6 with a wavefront each; x 256 13.5 and 17.8).  With a bias and more than 128 experts two instead of four: the
+// 64-bit sums take the registers (16384 x 256, 4 of 8 groups: 28.5 us, 31.7 with four).
+template <bool BIASED>
+void launch_form(const RouterParams& p, hipStream_t st) {
+  const bool many = p.tokens >= 4096;
+  if (p.experts <= 8 && p.groups <= 8) return launch<8, 1, BIASED>(p, st);
+  if (many && p.experts <= 32 && p.groups <= 8) return launch<8, 4, BIASED>(p, st);
+  if (many && p.experts <= 64 && p.groups <= 16) return launch<16, 4, BIASED>(p, st);
+  if (many && p.experts <= 128 && p.groups <= 16) return launch<16, 8, BIASED>(p, st);
+  if constexpr (BIASED) {
+    if (many && p.experts <= 256 && p.groups <= 32) return launch<32, 8, true>(p, st);
+  } else {
+    if (many && p.experts <= 256 && p.groups <= 16) return launch<16, 16, false>(p, st);
+  }
+  if (p.experts <= 64) return launch<64, 1, BIASED>(p, st);
+  if (p.experts <= 256) return launch<64, 4, BIASED>(p, st);
+  launch<64, 16, BIASED>(p, st);
 }
 
 }  // namespace
@@ -240,13 +333,7 @@ extern "C" int sonar_topk_routing(const void* logits, int dtype, int64_t row_str
   const RouterParams p{logits, row_stride,   bias,         weights,     ids,         tokens,          dtype, (int)experts,
                        (int)topk, scoring,   renormalize,  (int)groups, (int)kept_groups, factor};
   hipStream_t st = (hipStream_t)stream;
-  if (groups == 1 && experts <= 8) launch<8, 1>(p, st);
-  else if (groups == 1 && experts <= 16) launch<16, 1>(p, st);
-  else if (groups == 1 && experts <= 32) launch<32, 1>(p, st);
-  else if (experts <= 64) launch<64, 1>(p, st);
-  else if (experts <= 128) launch<64, 2>(p, st);
-  else if (experts <= 256) launch<64, 4>(p, st);
-  else if (experts <= 512) launch<64, 8>(p, st);
-  else launch<64, 16>(p, st);
+  if (bias != nullptr) launch_form<true>(p, st);
+  else launch_form<false>(p, st);
   return launch_status("topk_routing_kernel");
 }

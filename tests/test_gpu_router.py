@@ -111,6 +111,37 @@ def test_masks_and_numbers_that_are_none(experts, groups, kept, topk, scoring, b
         check(x, topk, scoring, renormalize, bias, groups, kept)
 
 
+@pytest.mark.parametrize("experts,groups,kept,topk", [(6, 1, 1, 2), (8, 4, 2, 3), (9, 1, 1, 9), (32, 1, 1, 4), (32, 8, 3, 5), (30, 3, 2, 20), (33, 1, 1, 6),
+                                                      (64, 16, 5, 20), (64, 1, 1, 64), (100, 1, 1, 33), (128, 8, 4, 8), (128, 1, 1, 40),
+                                                      (160, 8, 3, 6), (250, 1, 1, 8), (256, 8, 4, 8), (256, 1, 1, 64), (256, 32, 3, 8)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_many_tokens(experts, groups, kept, topk, scoring, biased, dtype):
+    """From 4096 tokens several share a wavefront.  Rows with ties, masks, NaN and infinities among them; the last ones
+    share theirs with nobody.  Some rows of each kind are compared."""
+    from sonar_amd import ops
+    tokens = 4099
+    x, bias = make(experts + topk, tokens, experts, dtype, biased)
+    low = torch.finfo(DTYPES[dtype]).min
+    x[1::10] = torch.round(x[1::10].float()).to(x.dtype)
+    x[2::10, ::2] = -float("inf")
+    x[3::10] = -float("inf")
+    x[4::10, 1::3] = low
+    x[5::10, experts // 2] = float("nan")
+    x[6::10, 0] = x[6::10, experts - 1] = float("inf")
+    x[7::10] = x[7::10] * 0.01 - 200
+    if biased:
+        bias[experts // 2] = bias[0]   # (equal choices at equal logits)
+    for renormalize in (True, False):
+        w, ids = ops.topk_routing(x.to(DEV), topk, scoring, renormalize, None if bias is None else bias.to(DEV), groups, kept, 1.5)
+        rows = sorted({*range(0, tokens, 97), *range(tokens - 12, tokens)})
+        want_w, want_ids = lo.topk_routing(x[rows].double().numpy(), topk, scoring, renormalize,
+                                           None if bias is None else bias.double().numpy(), groups, kept, 1.5)
+        assert np.array_equal(ids.cpu().numpy()[rows], want_ids)
+        np.testing.assert_allclose(w.cpu().double().numpy()[rows], want_w, rtol=RTOL, atol=1e-40)
+
+
 def test_a_bias_that_masks():
     """Experts that the bias switches off, and choices that differ in the last bits of the sum."""
     x, _ = make(8, 12, 64)
