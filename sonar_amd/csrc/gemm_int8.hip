@@ -7,7 +7,7 @@
 //   int8_tile_kernel     more rows, five tile sizes: bound by the matrix pipes from a few hundred rows on
 //   int8_join_kernel     sums of a K that was split over workgroups
 //   int8_pad_kernel      rows that no 16-byte vector is aligned to, laid down aligned for the tiles
-//   int8_general_kernel  anything, without any scratch
+//   int8_general_kernel  such rows as they lie, of short K, and anything without scratch
 #include <type_traits>
 
 #include "common.hpp"
@@ -37,72 +37,190 @@ __device__ __forceinline__ T int8_result(int sum, float scale_a, float scale_b, 
   return (T)__builtin_fmaf((float)sum, scale_a * scale_b, bias);
 }
 
-// 16 bytes of a row from k0 on, zeros behind its end.  Any alignment: the hardware loads a vector from any byte.
+// 16 bytes of a row of k from k0 on, zeros behind its end; any alignment.  At the end of a row its last 16 bytes are loaded and
+// shifted.
 __device__ __forceinline__ intx4_t load_16(const int8_t* row, int k0, int k) {
-  intx4_t v = {0, 0, 0, 0};
-  if (k0 + 16 <= k) {
-    __builtin_memcpy(&v, row + k0, 16);
-  } else if (k0 < k) {
-    for (int i = 0; i < 16; ++i)
-      if (k0 + i < k) v[i >> 2] |= (int)((uint32_t)(uint8_t)row[k0 + i] << (8 * (i & 3)));
+  if (k >= 16) {
+    const int at = min(k0, k - 16), past = min(k0 - at, 16);
+    unsigned __int128 v;
+    __builtin_memcpy(&v, row + at, 16);
+    return __builtin_bit_cast(intx4_t, past < 16 ? v >> (8 * past) : (unsigned __int128)0);
   }
+  intx4_t v = {0, 0, 0, 0};   // rows shorter than a vector
+  for (int i = 0; i < 16; ++i)
+    if (k0 + i < k) v[i >> 2] |= (int)((uint32_t)(uint8_t)row[k0 + i] << (8 * (i & 3)));
   return v;
 }
 
-// ---- anything
-// Any strides, alignments and sizes: 64 x 64 results a workgroup, 32 x 32 a wavefront, 128 bytes of K a step through
-// registers into LDS.  Runs where the caller of the C ABI gave no scratch for aligned copies.
-template <typename T>
-__global__ __launch_bounds__(256) void int8_general_kernel(const Int8Params p, int cols) {
-  constexpr int kStep = 128, kPitch = kStep + 16;
-  __shared__ __attribute__((aligned(16))) int8_t lds[2][128][kPitch];   // rows of a, then rows of b
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long m0 = (long)(blockIdx.x / cols) * 64, n0 = (long)(blockIdx.x % cols) * 64;
-  const int row = tid >> 3, chunk = tid & 7;   // a thread's rows row + 32 i, their 16 bytes at 16 chunk
-  intx4_t held[4];
-  auto fetch = [&](int k0) {
+// A row that starts at any byte (ODD) is read by whole words: 16 bytes and the word behind them, and shifted by what is over.
+// Vectors at odd bytes take the hardware three times as long: 1 x 4095 x 28672 63 us, 25.8 with 4096.  No word is read that
+// holds none of the bytes asked for.
+template <bool ODD>
+struct Row {
+  const int8_t* words;
+  int over, behind;   // bytes before the row's first in its word; where the word behind a piece is (its own last one if none is needed)
+  __device__ __forceinline__ Row() {}
+  __device__ __forceinline__ explicit Row(const int8_t* row) {
+    over = ODD ? (int)((uintptr_t)row & 3) : 0;
+    words = row - over;
+    behind = over ? 16 : 12;
+  }
+};
+template <bool ODD>
+struct Piece {
+  intx4_t v;
+  int more;
+  __device__ __forceinline__ void load(const Row<ODD>& row, int k) {   // k: a multiple of 4, and k + 16 bytes in the row
+    typedef int words_t __attribute__((ext_vector_type(4), aligned(4)));
+    v = *reinterpret_cast<const words_t*>(row.words + k);
+    if (ODD) more = *reinterpret_cast<const int*>(row.words + k + row.behind);
+  }
+  __device__ __forceinline__ intx4_t bytes(const Row<ODD>& row) const {
+    if (!ODD) return v;
+    intx4_t out;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const long m = min(m0 + row + 32 * i, (long)p.m - 1), n = min(n0 + row + 32 * i, (long)p.n - 1);
-      held[i] = load_16(p.a + m * p.lda, k0 + 16 * chunk, p.k);
-      held[2 + i] = load_16(p.b + n * p.ldb, k0 + 16 * chunk, p.k);
+    for (int i = 0; i < 4; ++i) out[i] = (int)__builtin_amdgcn_alignbyte((uint32_t)(i < 3 ? v[i + 1] : more), (uint32_t)v[i], (uint32_t)row.over);
+    return out;
+  }
+};
+
+// The 32 x 32 results of a wavefront at (m0, n0).  The halves of the wavefront trade quadruples, so that a lane has 16
+// neighbouring channels of its token, 32 bytes of a row.  `scale_a`: of the lane's token; `scales_b` and `bias`: of the 16 channels.
+template <typename T>
+__device__ __forceinline__ void store_block(const intx16_t& acc, const Int8Params& p, long m0, long n0, int lane, bool vectors,
+                                            float scale_a, const floatx4_t* scales_b, const floatx4_t* bias) {
+  const long m = m0 + (lane & 31), n = n0 + 16 * (lane >> 5);
+  T* out = (T*)p.c + m * p.n + n;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    typedef T eight_t __attribute__((ext_vector_type(8)));
+    eight_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // channels 8 q + e of the first half and 16 + 8 q + e; + 4 .. 7 are the other half's
+      const auto both = __builtin_amdgcn_permlane32_swap((unsigned)acc[4 * q + e], (unsigned)acc[8 + 4 * q + e], false, false);
+      v[e] = int8_result<T>((int)both[0], scale_a, scales_b[2 * q][e], bias[2 * q][e]);
+      v[4 + e] = int8_result<T>((int)both[1], scale_a, scales_b[2 * q + 1][e], bias[2 * q + 1][e]);
+    }
+    if (m < p.m) {
+      if (vectors && n + 8 * q + 8 <= p.n) {
+        *reinterpret_cast<eight_t*>(out + 8 * q) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + 8 * q + e < p.n) out[8 * q + e] = v[e];
+      }
+    }
+  }
+}
+
+// The same with the scales and the bias from memory.
+template <typename T>
+__device__ __forceinline__ void scale_and_store(const intx16_t& acc, const Int8Params& p, long m0, long n0, int lane, bool vectors) {
+  if (m0 >= p.m || n0 >= p.n) return;
+  const long m = min(m0 + (lane & 31), (long)p.m - 1);
+  floatx4_t sb[4], add[4];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const long n = min(n0 + 16 * (lane >> 5) + e, (long)p.n - 1);
+    sb[e / 4][e % 4] = p.b_scales[p.b_many ? n : 0];
+    add[e / 4][e % 4] = p.bias ? (float)((const T*)p.bias)[n] : 0.0f;
+  }
+  store_block<T>(acc, p, m0, n0, lane, vectors, p.a_scales[p.a_many ? m : 0], sb, add);
+}
+
+// ---- rows of any alignment
+// 64 x 64 results a workgroup of two sets of 2 x 2 wavefronts, which take 128 bytes of K in turn and join their sums in LDS.
+// Rows go through registers into the tiles' LDS order; two rounds of loads are out while a third is multiplied.  Any strides
+// and sizes, and no scratch.
+template <typename T>
+__global__ __launch_bounds__(512) void int8_general_kernel(const Int8Params p, int cols, bool vectors) {
+  constexpr int KG = 2, kStep = 128, kSlot = 128 * kStep, kRound = KG * kStep;
+  extern __shared__ __attribute__((aligned(1024))) int8_t lds[];   // [group][2][row of a, then of b][piece]
+  const int tid = threadIdx.x, lane = tid & 63, all_waves = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = all_waves & 3, group = all_waves >> 2;
+  const long m0 = (long)(blockIdx.x / cols) * 64, n0 = (long)(blockIdx.x % cols) * 64;
+  int8_t* slots = lds + group * 2 * kSlot;
+  const int row = tid >> 3 & 31, piece = tid & 7;   // a thread's rows row + 32 i of a, then of b
+  const int8_t* rows[4];
+  Row<true> words[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    rows[i] = i < 2 ? p.a + min(m0 + row + 32 * i, (long)p.m - 1) * p.lda : p.b + min(n0 + row + 32 * (i - 2), (long)p.n - 1) * p.ldb;
+    words[i] = Row<true>(rows[i]);
+  }
+  const int put_at = row * kStep + (piece ^ (row >> 1 & 7)) * 16;
+  Piece<true> held[2][4];
+  auto fetch = [&](int set, int round) {
+    const int k = (round * KG + group) * kStep + 16 * piece;
+    if ((round + 1) * kRound <= p.k) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) held[set][i].load(words[i], k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) held[set][i].v = load_16(rows[i], k, p.k);
     }
   };
+  const int wm = (wave & 1) * 32, wn = 64 + (wave >> 1) * 32, r = lane & 31, h = lane >> 5;
+  const int at0 = r * kStep + (h ^ (r >> 1 & 7)) * 16;
   intx16_t acc = {};
-  const int mw = (wave & 1) * 32, nw = 64 + (wave >> 1) * 32;
-  fetch(0);
-  for (int k0 = 0, at = 0; k0 < p.k; k0 += kStep, at ^= 1) {
+  auto put = [&](int set, int round) {
+    const bool whole = (round + 1) * kRound <= p.k;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<intx4_t*>(&lds[at][row + 32 * i][16 * chunk]) = held[i];
-    __syncthreads();
-    if (k0 + kStep < p.k) fetch(k0 + kStep);
+    for (int i = 0; i < 4; ++i) {
+      intx4_t v = held[set][i].v;
+      if (whole) v = held[set][i].bytes(words[i]);
+      *reinterpret_cast<intx4_t*>(slots + set * kSlot + put_at + 32 * i * kStep) = v;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (no wait for the loads that are out)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto multiply = [&](int set) {
+    intx4_t av[4], bv[4];
 #pragma unroll
-    for (int s = 0; s < kStep / 32; ++s) {
-      const intx4_t av = *reinterpret_cast<const intx4_t*>(&lds[at][mw + (lane & 31)][32 * s + 16 * (lane >> 5)]);
-      const intx4_t bv = *reinterpret_cast<const intx4_t*>(&lds[at][nw + (lane & 31)][32 * s + 16 * (lane >> 5)]);
-      acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv, av, acc, 0, 0, 0);
+    for (int s = 0; s < 4; ++s) {
+      av[s] = *reinterpret_cast<const intx4_t*>(slots + set * kSlot + wm * kStep + (at0 ^ (32 * s)));
+      bv[s] = *reinterpret_cast<const intx4_t*>(slots + set * kSlot + wn * kStep + (at0 ^ (32 * s)));
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[s], av[s], acc, 0, 0, 0);
+  };
+  const int rounds = (p.k + 2 * kRound - 1) / (2 * kRound) * 2;   // an even number: zeros behind the end of K
+  if (rounds > 0) fetch(0, 0), fetch(1, 1);
+  for (int round = 0; round < rounds; round += 2) {
+#pragma unroll
+    for (int set = 0; set < 2; ++set) {
+      put(set, round + set);   // (the other slot's readers are through: each passed this barrier after its reads)
+      if (round + 2 < rounds) fetch(set, round + 2 + set);
+      multiply(set);
     }
   }
-  // a lane has row lane % 32 of a and columns 8 (r / 4) + 4 (lane / 32) + r % 4
-  const long m = m0 + mw + (lane & 31);
-  if (m >= p.m) return;
-  const float sa = p.a_scales[p.a_many ? m : 0];
-  T* out = (T*)p.c + m * p.n;
+  __syncthreads();
+  intx4_t* sums = reinterpret_cast<intx4_t*>(lds);   // [group][wave][quadruple][lane]
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const long n = n0 + (nw - 64) + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-    if (n < p.n)
-      out[n] = int8_result<T>(acc[r], sa, p.b_scales[p.b_many ? n : 0], p.bias ? (float)((const T*)p.bias)[n] : 0.0f);
+  for (int q = 0; q < 4; ++q)
+    sums[((group * 4 + wave) * 4 + q) * 64 + lane] = intx4_t{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  if (group != 0) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    intx4_t v = {0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < KG; ++g) v += sums[((g * 4 + wave) * 4 + q) * 64 + lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[4 * q + e] = v[e];
   }
+  scale_and_store<T>(acc, p, m0 + wm, n0 + wn - 64, lane, vectors);
 }
 
 // ---- few rows
 // Up to 16 MB tokens: the weight is read once, past LDS, straight into the operand registers of 16 x 16 x 64 matrix
-// instructions (its 16 channels the first operand), 64 bytes of a row an instruction; any alignment.  A workgroup owns 16 NB
+// instructions (its 16 channels the first operand), 64 bytes of a row an instruction; rows of any alignment (ODD: not of words).  A workgroup owns 16 NB
 // channels; its wavefronts take steps of 128 bytes of K in turn, so that together they read a run of each row, and join their
 // sums through LDS.  A wavefront has DEEP steps of loads in flight, 4 KB at DEEP = 2: with 16 wavefronts on each compute unit
 // that covers the latency of memory.
-template <typename T, int kWaves, int MB, int NB, int DEEP>
+template <typename T, bool ODD, int kWaves, int MB, int NB, int DEEP>
 __global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8Params p, bool vectors) {
   constexpr int kStepK = 128;
   __shared__ intx4_t sums[kWaves][NB * MB][64];
@@ -116,16 +234,21 @@ __global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8P
 #pragma unroll
   for (int j = 0; j < NB; ++j) b_rows[j] = p.b + min(n0 + 16 * j + r, (long)p.n - 1) * p.ldb;
   intx4_t acc[NB][MB] = {};
+  Row<ODD> a_words[MB], b_words[NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i) a_words[i] = Row<ODD>(a_rows[i]);
+#pragma unroll
+  for (int j = 0; j < NB; ++j) b_words[j] = Row<ODD>(b_rows[j]);
   struct Step {
-    intx4_t a[MB][2], b[NB][2];
+    Piece<ODD> a[MB][2], b[NB][2];
   } held[DEEP];
   auto fetch = [&](Step& s, int k) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j) __builtin_memcpy(&s.b[j][x], b_rows[j] + at + k + 64 * x, 16);
+      for (int j = 0; j < NB; ++j) s.b[j][x].load(b_words[j], at + k + 64 * x);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) __builtin_memcpy(&s.a[i][x], a_rows[i] + at + k + 64 * x, 16);
+      for (int i = 0; i < MB; ++i) s.a[i][x].load(a_words[i], at + k + 64 * x);
     }
   };
   auto multiply = [&](const Step& s) {
@@ -134,7 +257,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8P
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.b[j][x], s.a[i][x], acc[j][i], 0, 0, 0);
+        for (int i = 0; i < MB; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.b[j][x].bytes(b_words[j]), s.a[i][x].bytes(a_words[i]), acc[j][i], 0, 0, 0);
   };
   const int whole = p.k / kStepK, mine = (whole - wave + kWaves - 1) / kWaves;   // this wavefront's steps
   const int first = wave * kStepK, next = kWaves * kStepK;
@@ -157,16 +281,19 @@ __global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8P
   for (int d = 0; d < DEEP; ++d)
     if (done + d + DEEP < mine) multiply(held[d]);
   if (p.k % kStepK != 0 && wave == whole % kWaves) {   // the rest of K
-    Step s;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int k = whole * kStepK + 64 * x + at;
+      intx4_t of_a[MB];
 #pragma unroll
-      for (int j = 0; j < NB; ++j) s.b[j][x] = load_16(b_rows[j], k, p.k);
+      for (int i = 0; i < MB; ++i) of_a[i] = load_16(a_rows[i], k, p.k);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) s.a[i][x] = load_16(a_rows[i], k, p.k);
+      for (int j = 0; j < NB; ++j) {
+        const intx4_t of_b = load_16(b_rows[j], k, p.k);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(of_b, of_a[i], acc[j][i], 0, 0, 0);
+      }
     }
-    multiply(s);
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j)
@@ -210,36 +337,6 @@ __device__ __forceinline__ void tile_at(int tile, const TilePlan& t, int& tm, in
   const int panel = tile / (8 * t.tiles_n), rows = min(8, t.tiles_m - 8 * panel), in = tile - panel * 8 * t.tiles_n;
   tn = __builtin_amdgcn_readfirstlane(in / rows);   // (the division leaves its quotient in a vector register)
   tm = __builtin_amdgcn_readfirstlane(8 * panel + in - tn * rows);
-}
-
-// The 32 x 32 results of a wavefront at (m0, n0).  The halves of the wavefront trade quadruples, so that a lane has 16
-// neighbouring channels of its token, 32 bytes of a row.  `scale_a`: of the lane's token; `scales_b` and `bias`: of the 16 channels.
-template <typename T>
-__device__ __forceinline__ void store_block(const intx16_t& acc, const Int8Params& p, long m0, long n0, int lane, bool vectors,
-                                            float scale_a, const floatx4_t* scales_b, const floatx4_t* bias) {
-  const long m = m0 + (lane & 31), n = n0 + 16 * (lane >> 5);
-  T* out = (T*)p.c + m * p.n + n;
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    typedef T eight_t __attribute__((ext_vector_type(8)));
-    eight_t v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      // channels 8 q + e of the first half and 16 + 8 q + e; + 4 .. 7 are the other half's
-      const auto both = __builtin_amdgcn_permlane32_swap((unsigned)acc[4 * q + e], (unsigned)acc[8 + 4 * q + e], false, false);
-      v[e] = int8_result<T>((int)both[0], scale_a, scales_b[2 * q][e], bias[2 * q][e]);
-      v[4 + e] = int8_result<T>((int)both[1], scale_a, scales_b[2 * q + 1][e], bias[2 * q + 1][e]);
-    }
-    if (m < p.m) {
-      if (vectors && n + 8 * q + 8 <= p.n) {
-        *reinterpret_cast<eight_t*>(out + 8 * q) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + 8 * q + e < p.n) out[8 * q + e] = v[e];
-      }
-    }
-  }
 }
 
 // A wavefront owns 32 MT rows x 32 NT columns in 32 x 32 x 32 instructions, WM x 2 wavefronts a tile.  The weight is the first
@@ -530,28 +627,30 @@ __global__ __launch_bounds__(256) void int8_join_kernel(const Int8Params p, cons
   int tm, tn;
   tile_at(tile, t, tm, tn);   // (a workgroup's four blocks are of one tile)
   const long m0 = (long)tm * 32 * MT * WM + (wave % WM * MT + i) * 32, n0 = (long)tn * 64 * NT + (wave / WM * NT + j) * 32;
-  if (m0 >= p.m || n0 >= p.n) return;
-  const long m = min(m0 + (lane & 31), (long)p.m - 1);
-  floatx4_t sb[4], add[4];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    const long n = min(n0 + 16 * (lane >> 5) + e, (long)p.n - 1);
-    sb[e / 4][e % 4] = p.b_scales[p.b_many ? n : 0];
-    add[e / 4][e % 4] = p.bias ? (float)((const T*)p.bias)[n] : 0.0f;
-  }
-  store_block<T>(acc, p, m0, n0, lane, vectors, p.a_scales[p.a_many ? m : 0], sb, add);
+  scale_and_store<T>(acc, p, m0, n0, lane, vectors);
 }
 
-// Rows of a and of b -> rows `pitch` bytes apart, zeros behind K; 16 bytes a thread.
+// Rows of a and of b -> rows `pitch` bytes apart, zeros behind K; a wavefront a row, 1 KB at a time, four of them asked for at once.
 __global__ __launch_bounds__(256) void int8_pad_kernel(const Int8Params p, int8_t* __restrict__ a, int8_t* __restrict__ b, int pitch) {
-  const int pieces = pitch / 16;
-  const long all = ((long)p.m + p.n) * pieces;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
-    const long row = i / pieces;
-    const int k = (int)(i - row * pieces) * 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long all = (long)p.m + p.n;
+  for (long row = (long)blockIdx.x * 4 + wave; row < all; row += (long)gridDim.x * 4) {
     const bool of_a = row < p.m;
-    const long at = of_a ? row : row - p.m;
-    *reinterpret_cast<intx4_t*>((of_a ? a : b) + at * pitch + k) = load_16(of_a ? p.a + at * p.lda : p.b + at * p.ldb, k, p.k);
+    const int8_t* from = of_a ? p.a + row * p.lda : p.b + (row - p.m) * p.ldb;
+    int8_t* to = of_a ? a + row * pitch : b + (row - p.m) * pitch;
+    const Row<true> words(from);
+    for (int k0 = lane * 16; k0 < pitch; k0 += 4096) {
+      Piece<true> pieces[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k0 + 1024 * i + 16 <= p.k) pieces[i].load(words, k0 + 1024 * i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 1024 * i;
+        if (k + 16 <= p.k) *reinterpret_cast<intx4_t*>(to + k) = pieces[i].bytes(words);
+        else if (k < pitch) *reinterpret_cast<intx4_t*>(to + k) = load_16(from, k, p.k);
+      }
+    }
   }
 }
 
@@ -564,9 +663,9 @@ struct FormCost {
   int rows, cols;
   float round, per_k;
 };
-constexpr FormCost kCosts[kForms] = {{64, 64, 0, 0},       {16, 32, 0, 0},        {16, 16, 0, 0},        {32, 16, 0, 0}, {64, 64, 4.4f, 1.3f},
+constexpr FormCost kCosts[kForms] = {{64, 64, 4.0f, 5.5f},      {16, 32, 0, 0},        {16, 16, 0, 0},        {32, 16, 0, 0}, {64, 64, 4.4f, 1.3f},
                                      {64, 128, 5.0f, 2.0f}, {128, 128, 5.0f, 3.1f}, {256, 128, 6.5f, 4.6f}, {256, 256, 8.1f, 8.3f}};
-constexpr float kJoinUs = 4.5f, kJoinBytesPerUs = 4.5e6f;   // a launch more; partial sums written and read
+constexpr float kLaunchUs = 4.5f, kBytesPerUs = 4.5e6f;   // a launch more, for partial sums or aligned copies; their bytes
 
 struct Int8Choice {
   int form, splits;
@@ -590,14 +689,20 @@ Int8Choice choose_form(int64_t m, int64_t n, int64_t k, bool aligned) {
   if (m <= 32 && ((n <= 4096 && k <= 6144) || !aligned)) return {kStreamTwo, 1};
   if (k < 16) return {kGeneral, 1};
   Int8Choice best = {kTile64, 1};
-  float least = 3.4e38f;
+  float least = 3.4e38f, copies = 0;
+  if (!aligned) {   // the tiles would have to wait for copies
+    best = {kGeneral, 1};
+    least = (float)((tiles_of(kGeneral, m, n) + 255) / 256) * (kCosts[kGeneral].round + kCosts[kGeneral].per_k * (float)k / 1024);
+    copies = kLaunchUs + 2.0f * (float)(m + n) * (float)k / kBytesPerUs;
+  }
   for (int form = kTile64; form <= kTile256; ++form)
     for (int splits = 1; splits <= 8 && may_split(splits, k); splits *= 2) {
       const int64_t tiles = tiles_of(form, m, n);
       if (splits > 1 && tiles * splits > 1024) break;
       const float rounds = (float)((tiles * splits + 255) / 256);
       float us = rounds * (kCosts[form].round + kCosts[form].per_k * (float)k / splits / 1024);
-      if (splits > 1) us += kJoinUs + (float)tiles * splits * kCosts[form].rows * kCosts[form].cols * 8 / kJoinBytesPerUs;
+      if (splits > 1) us += kLaunchUs + (float)tiles * splits * kCosts[form].rows * kCosts[form].cols * 8 / kBytesPerUs;
+      us += copies;
       if (us < least) least = us, best = {form, splits};
     }
   return best;
@@ -638,6 +743,15 @@ int launch_tiles(const Int8Params& p, int splits, int* partial, bool vectors, hi
   return launch_status("int8_tile_kernel");
 }
 
+template <typename T, int kWaves, int MB, int NB, int DEEP>
+void launch_stream(const Int8Params& p, bool vectors, hipStream_t st) {
+  const int grid = (p.n + 16 * NB - 1) / (16 * NB);
+  if (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.lda | (uintptr_t)p.ldb) % 4 != 0)
+    int8_stream_kernel<T, true, kWaves, MB, NB, DEEP < 2 ? DEEP : 2><<<grid, 64 * kWaves, 0, st>>>(p, vectors);
+  else
+    int8_stream_kernel<T, false, kWaves, MB, NB, DEEP><<<grid, 64 * kWaves, 0, st>>>(p, vectors);
+}
+
 template <typename T>
 int run_form(const Int8Params& p, const Int8Choice& s, int* partial, bool vectors, hipStream_t st) {
   switch (s.form) {
@@ -646,13 +760,14 @@ int run_form(const Int8Params& p, const Int8Choice& s, int* partial, bool vector
     case kTile128: return launch_tiles<T, 4, 1, 2, 1, 128, 3>(p, s.splits, partial, vectors, st);
     case kTile256Tall: return launch_tiles<T, 4, 2, 2, 1, 128, 3>(p, s.splits, partial, vectors, st);
     case kTile256: return launch_tiles<T, 4, 2, 4, 1, 64, 4>(p, s.splits, partial, vectors, st);
-    case kStream32: int8_stream_kernel<T, 8, 1, 2, 3><<<(p.n + 31) / 32, 512, 0, st>>>(p, vectors); break;
-    case kStream16: int8_stream_kernel<T, 16, 1, 1, 2><<<(p.n + 15) / 16, 1024, 0, st>>>(p, vectors); break;
-    case kStreamTwo: int8_stream_kernel<T, 16, 2, 1, 2><<<(p.n + 15) / 16, 1024, 0, st>>>(p, vectors); break;
+    case kStream32: launch_stream<T, 8, 1, 2, 3>(p, vectors, st); break;   // (two steps in flight where a word more goes with each)
+    case kStream16: launch_stream<T, 16, 1, 1, 2>(p, vectors, st); break;
+    case kStreamTwo: launch_stream<T, 16, 2, 1, 2>(p, vectors, st); break;
     default: {
       const int64_t rows = ((int64_t)p.m + 63) / 64, cols = ((int64_t)p.n + 63) / 64;
-      SONAR_REQUIRE(rows * cols < (1 << 23), "size_m = %d, size_n = %d: more tiles than a launch takes", p.m, p.n);
-      int8_general_kernel<T><<<(int)(rows * cols), 256, 0, st>>>(p, (int)cols);
+      SONAR_REQUIRE(rows * cols < (1 << 22), "size_m = %d, size_n = %d: more tiles than a launch takes", p.m, p.n);
+      constexpr int kLds = 65536;
+      int8_general_kernel<T><<<(int)(rows * cols), 512, kLds, st>>>(p, (int)cols, vectors);
     }
   }
   return launch_status("int8 product");
@@ -714,8 +829,8 @@ extern "C" int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const
   if (is_tile(s.form) && padded > 0) {
     const int pitch = (int)padded_k(size_k);
     int8_t* copies = (int8_t*)scratch;
-    const int64_t pieces = (size_m + size_n) * (pitch / 16);
-    int8_pad_kernel<<<(int)(pieces < 256 * 4096 ? (pieces + 255) / 256 : 4096), 256, 0, st>>>(p, copies, copies + size_m * pitch, pitch);
+    const int64_t groups = (size_m + size_n + 3) / 4;
+    int8_pad_kernel<<<(int)(groups < 16384 ? groups : 16384), 256, 0, st>>>(p, copies, copies + size_m * pitch, pitch);
     p.a = copies, p.b = copies + size_m * pitch, p.lda = p.ldb = p.k = pitch;
   }
   if (!is_tile(s.form) || !may_split(s.splits, size_k) || padded + partial_bytes(s, size_m, size_n) > scratch_bytes) s.splits = 1;
