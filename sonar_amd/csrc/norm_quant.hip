@@ -18,7 +18,7 @@ char* last_error_buffer() { return g_layer_error; }
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;   // of a workgroup, where a row has no more
 
 struct NormParams {
   const void* x;
@@ -30,18 +30,18 @@ struct NormParams {
   float* scales;
   long x_stride, residual_stride, rows;
   int cols;
-  double epsilon;
+  double inverse_cols, epsilon;
 };
 
 // Joins over a workgroup; `part` may be used again behind another call's barrier.
-template <typename V, typename F>
+template <int THREADS, typename V, typename F>
 __device__ __forceinline__ V over_block(V v, V none, V* part, F join) {
   v = over_wave(v, none, join);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   v = part[0];
 #pragma unroll
-  for (int w = 1; w < kThreads / 64; ++w) v = join(v, part[w]);
+  for (int w = 1; w < THREADS / 64; ++w) v = join(v, part[w]);
   return v;
 }
 
@@ -92,22 +92,44 @@ struct Eight {
   __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
 };
 
-// THREADS (64 or 256) a row, eight neighbouring columns of a row's KEPT turns a thread.  THREADS = 64: four rows a workgroup,
-// sums and maxima by lane moves, no barrier.  THREADS = 256: rows too long for a wavefront's registers, which beyond KEPT
-// turns are read again (as z), or too few to fill the card with wavefronts.  Workgroups go on from row to row with the
-// weight in registers.  16384 x 4096 bf16 to int8 with a residual (470 MB): 220 us element by element with three passes.
+// THREADS (64, 256 or 1024) a row, eight neighbouring columns of a row's KEPT turns a thread.  THREADS = 64: four rows a
+// workgroup, sums and maxima by lane moves, no barrier.  THREADS = 1024: rows of any length; turns beyond KEPT are read
+// again (as z).  A workgroup that goes on to a further row has its numbers loaded before it works on its own; the weight
+// stays in registers.
+// 16384 x 4096 bf16 to int8 with a residual (470 MB): 80 us, 5.8 TB/s; 92 with eight workgroups a compute unit that walk
+// the rows instead of a workgroup a row (fresh ones overlap their loads with the others' stores), 97 with a wavefront a row,
+// 220 element by element with three passes.  Registers decide: row bases in scalar registers with 32-bit offsets of the
+// columns, and no code of the repeated reads where no call needs them, took 107 registers to 68 and 16384 x 2880 without a
+// residual from 47 to 34 us.
 template <typename T, bool FP8, int THREADS, int KEPT>
-__global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormParams p) {
+__global__ __launch_bounds__(THREADS > kThreads ? THREADS : kThreads) void rms_norm_quant_kernel(const NormParams p) {
 #pragma clang fp contract(off)
-  constexpr int kRows = kThreads / THREADS, kStep = THREADS * 8;
-  __shared__ double sums[kThreads / 64];
-  __shared__ float mosts[kThreads / 64];
-  const int first = threadIdx.x % THREADS * 8, cols = p.cols;
+  constexpr int kRows = THREADS < kThreads ? kThreads / THREADS : 1, kStep = THREADS * 8;
+  __shared__ double sums[THREADS / 64];
+  __shared__ float mosts[THREADS / 64];
+  const uint32_t first = threadIdx.x % THREADS * 8, cols = p.cols;
   Eight<T> weight[KEPT], z[KEPT];
 #pragma unroll
   for (int i = 0; i < KEPT; ++i)
     if (first + i * kStep < cols) weight[i].load((const T*)p.weight + first + i * kStep);
-  for (long row = (long)blockIdx.x * kRows + threadIdx.x / THREADS; row < p.rows; row += (long)gridDim.x * kRows) {
+  const long step = (long)gridDim.x * kRows;
+  long row = (long)blockIdx.x * kRows + __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
+  Eight<T> more[KEPT];
+  auto fetch = [&](long at, Eight<T> (&to)[KEPT]) {
+    const T* x = (const T*)p.x + at * p.x_stride;
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (first + i * kStep < cols) to[i].load(x + first + i * kStep);
+    if (p.residual != nullptr) {
+      const T* residual = (const T*)p.residual + at * p.residual_stride;
+#pragma unroll
+      for (int i = 0; i < KEPT; ++i)
+        if (first + i * kStep < cols) more[i].load(residual + first + i * kStep);
+    }
+  };
+  Eight<T> next[KEPT];
+  if (row < p.rows) fetch(row, next);
+  for (; row < p.rows; row += step) {
     const T* x = (const T*)p.x + row * p.x_stride;
     const T* residual = (const T*)p.residual + row * p.residual_stride;
     T* out = (T*)p.residual_out + row * cols;
@@ -116,29 +138,25 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormPara
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = __builtin_fma((double)v.at(e), (double)v.at(e), sum);
     };
-    auto join = [&](Eight<T>& v, const Eight<T>& r, int c) {
+    auto join = [&](Eight<T>& v, const Eight<T>& r, uint32_t c) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v.v[e] = (T)(v.at(e) + r.at(e));
       v.store(out + c);
     };
 #pragma unroll
-    for (int i = 0; i < KEPT; ++i)
-      if (first + i * kStep < cols) z[i].load(x + first + i * kStep);
+    for (int i = 0; i < KEPT; ++i) z[i] = next[i];
     if (p.residual != nullptr) {
-      Eight<T> more[KEPT];
-#pragma unroll
-      for (int i = 0; i < KEPT; ++i)
-        if (first + i * kStep < cols) more[i].load(residual + first + i * kStep);
 #pragma unroll
       for (int i = 0; i < KEPT; ++i)
         if (first + i * kStep < cols) join(z[i], more[i], first + i * kStep);
     }
+    if (row + step < p.rows) fetch(row + step, next);
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
       if (first + i * kStep < cols) add(z[i]);
     const T* again = p.residual != nullptr ? out : x;   // z of the turns that no register keeps
-    if (THREADS > 64)
-      for (int c = first + KEPT * kStep; c < cols; c += kStep) {
+    if (THREADS > kThreads)
+      for (uint32_t c = first + KEPT * kStep; c < cols; c += kStep) {
         Eight<T> v;
         v.load(x + c);
         if (p.residual != nullptr) {
@@ -148,8 +166,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormPara
         }
         add(v);
       }
-    sum = THREADS == 64 ? wave_sum(sum) : over_block(sum, 0.0, sums, [](double a, double b) { return a + b; });
-    const float r = inverse_root(sum / cols + p.epsilon);
+    sum = THREADS == 64 ? wave_sum(sum) : over_block<THREADS>(sum, 0.0, sums, [](double a, double b) { return a + b; });
+    const float r = inverse_root(__builtin_fma(sum, p.inverse_cols, p.epsilon));
     float most = 0.0f;
     auto larger = [&](const Eight<T>& v, const Eight<T>& w) {
 #pragma unroll
@@ -158,18 +176,18 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormPara
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
       if (first + i * kStep < cols) larger(z[i], weight[i]);
-    if (THREADS > 64)
-      for (int c = first + KEPT * kStep; c < cols; c += kStep) {
+    if (THREADS > kThreads)
+      for (uint32_t c = first + KEPT * kStep; c < cols; c += kStep) {
         Eight<T> v, w;
         v.load(again + c), w.load((const T*)p.weight + c);
         larger(v, w);
       }
     auto max_of = [](float a, float b) { return fmaxf(a, b); };
-    most = THREADS == 64 ? over_wave(most, 0.0f, max_of) : over_block(most, 0.0f, mosts, max_of);
+    most = THREADS == 64 ? over_wave(most, 0.0f, max_of) : over_block<THREADS>(most, 0.0f, mosts, max_of);
     float scale, by;
     scale_of<FP8>(most, r, scale, by);
     if (first == 0) p.scales[row] = scale;
-    auto code = [&](const Eight<T>& v, const Eight<T>& w, int c) {
+    auto code = [&](const Eight<T>& v, const Eight<T>& w, uint32_t c) {
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = v.at(e) * r * w.at(e);
@@ -196,8 +214,8 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_kernel(const NormPara
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
       if (first + i * kStep < cols) code(z[i], weight[i], first + i * kStep);
-    if (THREADS > 64)
-      for (int c = first + KEPT * kStep; c < cols; c += kStep) {
+    if (THREADS > kThreads)
+      for (uint32_t c = first + KEPT * kStep; c < cols; c += kStep) {
         Eight<T> v, w;
         v.load(again + c), w.load((const T*)p.weight + c);
         code(v, w, c);
@@ -228,11 +246,11 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_any_kernel(const Norm
     } else {
       for (int c = threadIdx.x; c < cols; c += kThreads) sum = __builtin_fma((double)(float)z[c], (double)(float)z[c], sum);
     }
-    sum = over_block(sum, 0.0, sums, [](double a, double b) { return a + b; });
-    const float r = inverse_root(sum / cols + p.epsilon);
+    sum = over_block<kThreads>(sum, 0.0, sums, [](double a, double b) { return a + b; });
+    const float r = inverse_root(__builtin_fma(sum, p.inverse_cols, p.epsilon));
     float most = 0.0f;
     for (int c = threadIdx.x; c < cols; c += kThreads) most = fmaxf(most, fabsf((float)z[c] * r * (float)weight[c]));
-    most = over_block(most, 0.0f, mosts, [](float a, float b) { return fmaxf(a, b); });
+    most = over_block<kThreads>(most, 0.0f, mosts, [](float a, float b) { return fmaxf(a, b); });
     float scale, by;
     scale_of<FP8>(most, r, scale, by);
     if (threadIdx.x == 0) p.scales[row] = scale;
@@ -245,24 +263,31 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_any_kernel(const Norm
   }
 }
 
+// Workgroups: `each` a compute unit at most, which go on to further rows.
+int grid_of(long groups, int each) { return (int)(groups < 256L * each ? groups : 256L * each); }
+
 template <typename T, bool FP8>
 int launch(const NormParams& p, hipStream_t st) {
   auto at_16 = [](const void* q) { return (uintptr_t)q % 16 == 0; };
   const long pitch = (long)(16 / sizeof(T));
   const bool vectors = p.cols % 8 == 0 && at_16(p.x) && at_16(p.residual) && at_16(p.weight) && at_16(p.residual_out) &&
                        at_16(p.norm_out) && (uintptr_t)p.q % 8 == 0 && p.x_stride % pitch == 0 && p.residual_stride % pitch == 0;
-  const long most = 256 * 8;   // workgroups: a compute unit holds eight at most
   if (!vectors) {
-    rms_norm_quant_any_kernel<T, FP8><<<(int)(p.rows < most ? p.rows : most), kThreads, 0, st>>>(p);
+    rms_norm_quant_any_kernel<T, FP8><<<grid_of(p.rows, 8), kThreads, 0, st>>>(p);
     return launch_status("rms_norm_quant_any_kernel");
   }
-  const bool waves = p.cols <= 512 || (p.cols <= 4096 && p.rows >= 2048);
-  const long groups = waves ? (p.rows + 3) / 4 : p.rows;
-  const int grid = (int)(groups < most ? groups : most);
-  if (waves && p.cols <= 1024) rms_norm_quant_kernel<T, FP8, 64, 2><<<grid, kThreads, 0, st>>>(p);
-  else if (waves) rms_norm_quant_kernel<T, FP8, 64, 8><<<grid, kThreads, 0, st>>>(p);
+  // Columns that a row's threads keep: as few turns as the row needs.  Rows of up to 1024: a wavefront each (4096 x 1024 with
+  // a residual 8.5 us, a workgroup each 11.2), but a workgroup each where they are few (64 x 1024 3.48 and 3.32, even at 512).
+  // Over 8192: 1024 threads and two workgroups a compute unit, which load ahead (4096 x 16384 88 us, with eight 102;
+  // 256 threads that read half of the row again 121).
+  const long fours = (p.rows + 3) / 4;
+  const int grid = grid_of(p.rows, 128);
+  if (p.cols <= 512) rms_norm_quant_kernel<T, FP8, 64, 1><<<grid_of(fours, 128), kThreads, 0, st>>>(p);
+  else if (p.cols <= 1024 && p.rows >= 512) rms_norm_quant_kernel<T, FP8, 64, 2><<<grid_of(fours, 128), kThreads, 0, st>>>(p);
+  else if (p.cols <= 2048) rms_norm_quant_kernel<T, FP8, 256, 1><<<grid, kThreads, 0, st>>>(p);
   else if (p.cols <= 4096) rms_norm_quant_kernel<T, FP8, 256, 2><<<grid, kThreads, 0, st>>>(p);
-  else rms_norm_quant_kernel<T, FP8, 256, 8><<<grid, kThreads, 0, st>>>(p);
+  else if (p.cols <= 8192) rms_norm_quant_kernel<T, FP8, 256, 4><<<grid, kThreads, 0, st>>>(p);
+  else rms_norm_quant_kernel<T, FP8, 1024, 2><<<grid_of(p.rows, 2), 1024, 0, st>>>(p);
   return launch_status("rms_norm_quant_kernel");
 }
 
@@ -290,7 +315,7 @@ extern "C" int sonar_rms_norm_per_token_quant(const void* x, int64_t x_row_strid
   SONAR_REQUIRE(x && weight && q && scales, "x, weight, q and scales must not be NULL");
   SONAR_REQUIRE((residual == nullptr) == (residual_out == nullptr), "residual and residual_out go together");
   const NormParams p{x, residual, weight, residual_out, norm_out, (uint8_t*)q, scales, x_row_stride, residual ? residual_row_stride : 0,
-                     rows, (int)cols, epsilon};
+                     rows, (int)cols, 1.0 / (double)cols, epsilon};
   hipStream_t st = (hipStream_t)stream;
   const bool fp8 = q_dtype == SONAR_ADTYPE_FP8;
   if (dtype == SONAR_DTYPE_F16) return fp8 ? launch<_Float16, true>(p, st) : launch<_Float16, false>(p, st);

@@ -81,6 +81,27 @@ def test_many_rows(rows, cols):
     check(ops.rms_norm_per_token_quant(dx, dw, EPS, torch.int8, dres, True), x, w, res, "bf16", "int8", True)
 
 
+@pytest.mark.parametrize("rows,cols", [(131081, 64), (131081, 520), (32773, 1032), (32773, 2056), (32773, 4104), (517, 8200), (1030, 20000), (5000, 77)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_more_rows_than_workgroups(rows, cols, residual):
+    """Workgroups that go on to further rows: bit for bit what the rows give in pieces that the grid holds."""
+    from sonar_amd import ops
+    gen = torch.Generator(device=DEV).manual_seed(cols)
+    x = torch.randn((rows, cols), generator=gen, device=DEV, dtype=torch.bfloat16)
+    w = torch.randn(cols, generator=gen, device=DEV, dtype=torch.bfloat16)
+    res = torch.randn((rows, cols), generator=gen, device=DEV, dtype=torch.bfloat16) if residual else None
+    got = ops.rms_norm_per_token_quant(x, w, EPS, torch.int8, res, True)
+    some = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device=DEV)
+    check([None if t is None else t[some] for t in got], x[some].cpu(), w.cpu(), res[some].cpu() if residual else None, "bf16", "int8", True)
+    step = rows // 5 if cols > 77 else 500
+    if cols > 8192:
+        step = 200
+    for i in range(0, rows, step):
+        want = ops.rms_norm_per_token_quant(x[i:i + step], w, EPS, torch.int8, res[i:i + step] if residual else None, True)
+        for a, b in zip(got, want):
+            assert a is None and b is None or torch.equal(a[i:i + step], b)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("cols,pitch,shift", [(512, 520, 0), (512, 513, 0), (512, 512, 1), (500, 512, 4), (4096, 4100, 0), (24, 64, 8)])
 def test_strides_and_alignment(dtype, cols, pitch, shift):

@@ -228,7 +228,7 @@ def test_oracle_values():
     assert c.tolist() == [[-1.5, -382.0]]
 
 
-KERNEL_FORMS = {"rms_norm_quant_kernel": 24, "rms_norm_quant_any_kernel": 6, "int8_general_kernel": 2, "topk_routing_kernel": 16, "int8_stream_kernel": 12,
+KERNEL_FORMS = {"rms_norm_quant_kernel": 36, "rms_norm_quant_any_kernel": 6, "int8_general_kernel": 2, "topk_routing_kernel": 16, "int8_stream_kernel": 12,
                 "int8_tile_kernel": 10, "int8_join_kernel": 10, "int8_pad_kernel": 1}
 
 
