@@ -9,9 +9,13 @@
 // the largest first word over the token's lanes by lane moves, asks which lanes have it (and looks at the second words
 // only if several have), takes the lowest lane's lowest expert, and that lane looks for its next.  Word 0 is below every
 // number's: an expert that is taken, left out or not there.
-// Bound by the vector instructions of the rounds, and by the latency of their chains where tokens are few.  16384 x 256, sigmoid,
-// bias, 4 of 8 groups: 132 us with choices and 64-bit maxima in LDS, 28.5 so.  (Choices in float32 first, and in 64 bits only
-// for the tokens where two come near each other: 31.6.)
+// Groups whose experts lie in 2^n whole lanes are judged from registers, others through LDS.
+// Bound by the vector instructions (the 64-bit exponentials and the rounds; 4 to 8 wavefronts a SIMD take the same time), and by
+// the latency of their chains where tokens are few.  16384 x 256, sigmoid, bias, 4 of 8 groups: 132 us with choices and 64-bit
+// maxima in LDS; 28.6 by lane moves; 21.4 with no loop over tokens around it all (which kept constants in 80 registers), the
+// scoring's branch outside the experts' loop (their chains side by side, one set of constants), which of a lane's experts it is
+// as lane masks, and the groups from registers.  (Choices in float32 first, and in 64 bits only for the tokens where two come
+// near each other: no gain.)
 #include "common.hpp"
 #include "lane_reduce.hpp"
 #include "sonar_layer.h"
@@ -20,7 +24,6 @@ namespace sonar {
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxGroups = 64, kMaxTopk = 64, kWaves = 4;
-
 
 struct RouterParams {
   const void* logits;
@@ -122,160 +125,187 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = lane % LANES, seg = lane / LANES, E = p.experts, e0 = l * R;
   const float inf = __builtin_inff();
+  // 2^shift lanes a group, as many as there are; `in_lanes`: those hold just its experts
+  const int size = E / p.groups, shift = 31 - __builtin_clz(LANES / p.groups);
+  const bool in_lanes = size == R << shift;
   auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
   auto add = [](double a, double b) { return a + b; };
-  for (long first = ((long)blockIdx.x * kWaves + wave) * kTokens; first < p.tokens; first += (long)gridDim.x * kWaves * kTokens) {
-    const long token = first + seg;
-    const bool there = token < p.tokens;
-    const long at = (there ? token : p.tokens - 1) * p.row_stride;
-    float x[R];
-    uint32_t key[R], low[R];   // of the choices
-    if (p.dtype == SONAR_DTYPE_F32) load_logits((const float*)p.logits + at, e0, E, vectors, x);
-    else if (p.dtype == SONAR_DTYPE_BF16) load_logits((const __bf16*)p.logits + at, e0, E, vectors, x);
-    else load_logits((const _Float16*)p.logits + at, e0, E, vectors, x);
-    const bool softmax = p.scoring == SONAR_SCORING_SOFTMAX;
-    float top = 0;
-    if (softmax) {
-      uint32_t top_key = 0;
+  const long first = ((long)blockIdx.x * kWaves + wave) * kTokens;
+  if (first >= p.tokens) return;
+  const long token = first + seg;
+  const bool there = token < p.tokens;
+  const long at = (there ? token : p.tokens - 1) * p.row_stride;
+  float x[R];
+  uint32_t key[R], low[R];   // of the choices
+  if (p.dtype == SONAR_DTYPE_F32) load_logits((const float*)p.logits + at, e0, E, vectors, x);
+  else if (p.dtype == SONAR_DTYPE_BF16) load_logits((const __bf16*)p.logits + at, e0, E, vectors, x);
+  else load_logits((const _Float16*)p.logits + at, e0, E, vectors, x);
+  const bool softmax = p.scoring == SONAR_SCORING_SOFTMAX;
+  float top = 0;
+  if (softmax) {
+    uint32_t top_key = 0;
 #pragma unroll
-      for (int r = 0; r < R; ++r) top_key = larger(top_key, ordered(x[r]));
-      top = number_of(over_lanes<LANES>(top_key, larger));
-    }
-    double sum = 0;   // of a token's terms
-    if (BIASED) {
-      double score[R];
+    for (int r = 0; r < R; ++r) top_key = larger(top_key, ordered(x[r]));
+    top = number_of(over_lanes<LANES>(top_key, larger));
+  }
+  double sum = 0;   // of a token's terms
+  double choice[R];   // (with a bias; else x)
+  if (BIASED) {
+    if (softmax) {   // (branches outside the loops: the experts' chains of instructions side by side)
 #pragma unroll
-      for (int r = 0; r < R; ++r) sum += score[r] = softmax ? term(x[r], top) : sigmoid(x[r]);
-      if (softmax) sum = over_lanes<LANES>(sum, add);
-      if (softmax && sum > 0) {
+      for (int r = 0; r < R; ++r) sum += choice[r] = term(x[r], top);
+      sum = over_lanes<LANES>(sum, add);
+      if (sum > 0) {
         const double scale = inverse(sum);
 #pragma unroll
-        for (int r = 0; r < R; ++r) score[r] *= scale;
-      }
-      float bias[R];
-      load_logits(p.bias, e0, E, vectors, bias);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        double choice = score[r] + (double)bias[r];
-        if (choice != choice) choice = -(double)inf;
-        const float near = (float)choice, rest = (float)(choice - (double)near);
-        key[r] = ordered(near), low[r] = ordered(rest == rest ? rest : 0.0f);
-        if (p.groups > 1 && e0 + r < E) all_choices[(wave * kTokens + seg) * E + e0 + r] = choice;
+        for (int r = 0; r < R; ++r) choice[r] *= scale;
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        key[r] = ordered(x[r]);
-        if (p.groups > 1 && e0 + r < E) all_choices[(wave * kTokens + seg) * E + e0 + r] = (double)x[r];
-      }
-      if (softmax && !p.renormalize) {   // (renormalised weights need no sum over all)
-        float terms = 0;
-#pragma unroll
-        for (int r = 0; r < R; ++r) terms += x[r] == -inf ? 0.0f : x[r] == top ? 1.0f : __expf(x[r] - top);
-        sum = over_lanes<LANES>((double)terms, add);
-      }
+      for (int r = 0; r < R; ++r) choice[r] = sigmoid(x[r]);
     }
+    float bias[R];
+    load_logits(p.bias, e0, E, vectors, bias);
 #pragma unroll
-    for (int r = 0; r < R; ++r) key[r] = e0 + r < E ? key[r] : 0;
+    for (int r = 0; r < R; ++r) {
+      choice[r] += (double)bias[r];
+      if (choice[r] != choice[r]) choice[r] = -(double)inf;
+      const float near = (float)choice[r], rest = (float)(choice[r] - (double)near);
+      key[r] = ordered(near), low[r] = ordered(rest == rest ? rest : 0.0f);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = ordered(x[r]);
+    if (softmax && !p.renormalize) {   // (renormalised weights need no sum over all)
+      float terms = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) terms += x[r] == -inf ? 0.0f : x[r] == top ? 1.0f : __expf(x[r] - top);
+      sum = over_lanes<LANES>((double)terms, add);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = e0 + r < E ? key[r] : 0;
 
-    if (p.groups > 1) {
-      // 2^n lanes a group, as many as there are: the two largest choices of each, a lane's share first
+  if (p.groups > 1) {
+    const int g = l >> shift, share = 1 << shift;
+    double best = -(double)inf, second = best;   // of the lane's share of its group
+    auto count = [&](double c) {
+      second = fmax(second, fmin(best, c));
+      best = fmax(best, c);
+    };
+    if (in_lanes) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) count(BIASED ? choice[r] : (double)x[r]);
+    } else {
+      double* choices = all_choices + (wave * kTokens + seg) * E;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (e0 + r < E) choices[e0 + r] = BIASED ? choice[r] : (double)x[r];
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const int size = E / p.groups, shift = 31 - __builtin_clz(LANES / p.groups), g = l >> shift, share = 1 << shift;
-      const double* choices = all_choices + (wave * kTokens + seg) * E;
-      double best = -(double)inf, second = best;
       if (g < p.groups)
-        for (int j = l & (share - 1); j < size; j += share) {
-          const double c = choices[g * size + j];
-          second = fmax(second, fmin(best, c));
-          best = fmax(best, c);
-        }
-      for (int step = 1; step < share; step <<= 1) {
-        const double b = __shfl_xor(best, step, 64), s = __shfl_xor(second, step, 64);
-        second = fmax(fmin(best, b), fmax(second, s));
-        best = fmax(best, b);
-      }
-      if (BIASED && size > 1) best += second;
-      if (best != best) best = -(double)inf;
-      int rank = 0;   // groups before this one
-      for (int other = 0; other < p.groups; ++other) {
-        const double b = __shfl(best, seg * LANES + (other << shift), 64);
-        rank += b > best || (b == best && other < g) ? 1 : 0;
-      }
-      const unsigned long long open = __ballot(g < p.groups && rank < p.kept_groups) >> (seg * LANES);
+        for (int j = l & (share - 1); j < size; j += share) count(choices[g * size + j]);
+    }
+    for (int step = 1; step < share; step <<= 1) {
+      const double b = __shfl_xor(best, step, 64), s = __shfl_xor(second, step, 64);
+      second = fmax(fmin(best, b), fmax(second, s));
+      best = fmax(best, b);
+    }
+    if (BIASED && size > 1) best += second;
+    if (best != best) best = -(double)inf;
+    int rank = 0;   // groups before this one
+#pragma unroll 4
+    for (int other = 0; other < p.groups; ++other) {
+      const double b = __shfl(best, seg * LANES + (other << shift), 64);
+      rank += b > best || (b == best && other < g) ? 1 : 0;
+    }
+    const bool kept = g < p.groups && rank < p.kept_groups;
+    if (in_lanes) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) key[r] = kept ? key[r] : 0;
+    } else {
+      const unsigned long long open = __ballot(kept) >> (seg * LANES);
       const float per_group = 1.0f / (float)size;   // (e + 1 / 2) / size is 2^-11 from a whole number at least
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int of = (int)(((float)(e0 + r) + 0.5f) * per_group);
         if (!(open >> ((of << shift) & 63) & 1)) key[r] = 0;
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-
-    uint32_t best;   // of this lane's experts, by the first word
-    auto look = [&]() {
-      best = key[0];
-#pragma unroll
-      for (int r = 1; r < R; ++r) best = larger(best, key[r]);
-    };
-    auto low_of_best = [&]() {
-      uint32_t most = 0;
-#pragma unroll
-      for (int r = 0; r < R; ++r) most = larger(most, key[r] == best ? low[r] : 0);
-      return most;
-    };
-    look();
-    for (int k = 0; k < p.topk; ++k) {
-      const uint32_t most = over_lanes<LANES>(best, larger);
-      bool has = best == most;
-      unsigned long long have = __ballot(has);
-      if (BIASED && __popcll(have) != kTokens) {   // several lanes with the same first word
-        const uint32_t mine_low = has ? low_of_best() : 0, rest = over_lanes<LANES>(mine_low, larger);
-        has = has && mine_low == rest;
-        have = __ballot(has);
-      }
-      bool mine;
-      if (LANES == 64) mine = lane == __builtin_ctzll(have);
-      else mine = l == __builtin_ctz((uint32_t)(have >> (seg * LANES)) | 0x80000000u);   // (a lane of the token has it: the lowest is the token's)
-      if (mine) {
-        int at_r = 0;
-#pragma unroll
-        for (int r = R - 1; r > 0; --r) at_r = key[r] == best ? r : at_r;
-        at_r = key[0] == best ? 0 : at_r;
-        if (BIASED && R > 1) {
-          int same = 0;
-#pragma unroll
-          for (int r = 0; r < R; ++r) same += key[r] == best ? 1 : 0;
-          if (same > 1) {   // several here with the same first word: by the second
-            const uint32_t rest = low_of_best();
-#pragma unroll
-            for (int r = R - 1; r >= 0; --r) at_r = key[r] == best && low[r] == rest ? r : at_r;
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) key[r] = r == at_r ? 0 : key[r];
-        chosen[wave][seg * kMaxTopk + k] = e0 + at_r;
-        look();
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    double total = 0;
-    for (int pass = p.renormalize ? 0 : 1; pass < 2; ++pass)   // the sum of the chosen scores, then the weights
-      for (int k = l; k < (p.topk + LANES - 1) / LANES * LANES; k += LANES) {
-        const int expert = chosen[wave][seg * kMaxTopk + min(k, p.topk - 1)];
-        const float logit = logit_at(p, at + expert);
-        double w = softmax ? term(logit, top) : sigmoid(logit);
-        if (softmax && sum > 0) w /= sum;
-        if (pass == 0) {
-          total += over_lanes<LANES>(k < p.topk ? w : 0.0, add);
-        } else if (there && k < p.topk) {
-          if (total > 0) w /= total;
-          p.weights[token * p.topk + k] = (float)(w * p.factor);
-          p.ids[token * p.topk + k] = expert;
-        }
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
+
+  uint32_t best;   // of this lane's experts, by the first word
+  auto look = [&]() {
+    best = key[0];
+#pragma unroll
+    for (int r = 1; r < R; ++r) best = larger(best, key[r]);
+  };
+  auto low_of_best = [&]() {
+    uint32_t most = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) most = larger(most, key[r] == best ? low[r] : 0);
+    return most;
+  };
+  look();
+  for (int k = 0; k < p.topk; ++k) {
+    const uint32_t most = over_lanes<LANES>(best, larger);
+    bool has = best == most;
+    unsigned long long have = __ballot(has);
+    if (BIASED && __popcll(have) != kTokens) {   // several lanes with the same first word
+      const uint32_t mine_low = has ? low_of_best() : 0, rest = over_lanes<LANES>(mine_low, larger);
+      has = has && mine_low == rest;
+      have = __ballot(has);
+    }
+    bool mine;
+    if (LANES == 64) mine = lane == __builtin_ctzll(have);
+    else mine = l == __builtin_ctz((uint32_t)(have >> (seg * LANES)) | 0x80000000u);   // (a lane of the token has it: the lowest is the token's)
+    if (mine) {
+      bool seen = false, several = false;   // (lane masks: scalar instructions)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool is = key[r] == best;
+        several = several || (seen && is);
+        seen = seen || is;
+      }
+      int at_r = 0;
+      seen = false;
+      if (BIASED && R > 1 && __ballot(several)) {   // several here with the same first word: by the second
+        const uint32_t rest = low_of_best();
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const bool it = !seen && key[r] == best && low[r] == rest;
+          at_r = it ? r : at_r;
+          key[r] = it ? 0 : key[r];
+          seen = seen || it;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const bool it = !seen && key[r] == best;
+          at_r = it ? r : at_r;
+          key[r] = it ? 0 : key[r];
+          seen = seen || it;
+        }
+      }
+      chosen[wave][seg * kMaxTopk + k] = e0 + at_r;
+      look();
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  double total = 0;
+  for (int pass = p.renormalize ? 0 : 1; pass < 2; ++pass)   // the sum of the chosen scores, then the weights
+    for (int k = l; k < (p.topk + LANES - 1) / LANES * LANES; k += LANES) {
+      const int expert = chosen[wave][seg * kMaxTopk + min(k, p.topk - 1)];
+      const float logit = logit_at(p, at + expert);
+      double w = softmax ? term(logit, top) : sigmoid(logit);
+      if (softmax && sum > 0) w /= sum;
+      if (pass == 0) {
+        total += over_lanes<LANES>(k < p.topk ? w : 0.0, add);
+      } else if (there && k < p.topk) {
+        if (total > 0) w /= total;
+        p.weights[token * p.topk + k] = (float)(w * p.factor);
+        p.ids[token * p.topk + k] = expert;
+      }
+    }
 }
 
 template <int LANES, int R, bool BIASED>
@@ -283,15 +313,22 @@ void launch(const RouterParams& p, hipStream_t st) {
   const long size = p.dtype == SONAR_DTYPE_F32 ? 4 : 2;
   const bool vectors = (uintptr_t)p.logits % 16 == 0 && p.row_stride * size % 16 == 0 && p.experts * size % 16 == 0 &&
                        (uintptr_t)p.bias % 16 == 0;   // (experts: a multiple of four, whole vectors of the bias too)
-  const long waves = (p.tokens + 64 / LANES - 1) / (64 / LANES), groups = (waves + kWaves - 1) / kWaves;
-  const int grid = (int)(groups < (1 << 20) ? groups : 1 << 20);
-  const size_t lds = p.groups > 1 ? (size_t)kWaves * (64 / LANES) * p.experts * sizeof(double) : 0;
-  topk_routing_kernel<LANES, R, BIASED><<<grid, 64 * kWaves, lds, st>>>(p, vectors);
+  const bool in_lanes = p.experts / p.groups == R << (31 - __builtin_clz(LANES / p.groups));   // (as the kernel)
+  const size_t lds = p.groups > 1 && !in_lanes ? (size_t)kWaves * (64 / LANES) * p.experts * sizeof(double) : 0;
+  const long most = (1L << 20) * kWaves * (64 / LANES);   // tokens of a launch: a loop in the kernel would keep its constants in registers
+  for (long from = 0; from < p.tokens; from += most) {
+    RouterParams q = p;
+    q.tokens = p.tokens - from < most ? p.tokens - from : most;
+    q.logits = (const char*)p.logits + from * p.row_stride * size;
+    q.weights += from * p.topk, q.ids += from * p.topk;
+    const int grid = (int)((q.tokens + kWaves * (64 / LANES) - 1) / (kWaves * (64 / LANES)));
+    topk_routing_kernel<LANES, R, BIASED><<<grid, 64 * kWaves, lds, st>>>(q, vectors);
+  }
 }
 
-// Few tokens: a wavefront each, for its latency.  From 4096 on, where every SIMD has some, several share one (16384 x 128, top 8:
-// 8.0 us, 17.6 with a wavefront each; x 256 13.5 and 17.8).  With a bias and more than 128 experts two instead of four: the
-// 64-bit sums take the registers (16384 x 256, 4 of 8 groups: 28.5 us, 31.7 with four).
+// Few tokens: a wavefront each, for its latency.  From 4096 on, where every SIMD has some, several share one (8192 x 128, top 8:
+// 5.5 us, 9.5 with a wavefront each; at 2048 tokens x 256 4.9 and, shared, 6.0).  With a bias and more than 128 experts two
+// instead of four (4096 x 256, 4 of 8 groups: 11.0 us, 13.6 with four; the same from 16384 on).
 template <bool BIASED>
 void launch_form(const RouterParams& p, hipStream_t st) {
   const bool many = p.tokens >= 4096;

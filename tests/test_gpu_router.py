@@ -142,6 +142,19 @@ def test_many_tokens(experts, groups, kept, topk, scoring, biased, dtype):
         np.testing.assert_allclose(w.cpu().double().numpy()[rows], want_w, rtol=RTOL, atol=1e-40)
 
 
+def test_more_tokens_than_a_launch_takes():
+    """2^25 tokens of 8 experts are a launch; the next one's results lie behind the first one's."""
+    from sonar_amd import ops
+    tokens = (1 << 25) + 1000
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn((tokens, 8), generator=gen, device=DEV, dtype=torch.bfloat16)
+    got = ops.topk_routing(x, 2, renormalize=True)
+    for start in (0, (1 << 25) - 500, tokens - 900):
+        want = ops.topk_routing(x[start:start + 900], 2, renormalize=True)
+        assert all(torch.equal(a[start:start + 900], b) for a, b in zip(got, want))
+    check(x[-64:].cpu(), 2, "softmax", True, None)
+
+
 def test_a_bias_that_masks():
     """Experts that the bias switches off, and choices that differ in the last bits of the sum."""
     x, _ = make(8, 12, 64)
