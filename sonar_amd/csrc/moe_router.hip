@@ -12,7 +12,7 @@
 // Groups whose experts lie in 2^n whole lanes are judged from registers, others through LDS.
 // Bound by the vector instructions (the 64-bit exponentials and the rounds; 4 to 8 wavefronts a SIMD take the same time), and by
 // the latency of their chains where tokens are few.  16384 x 256, sigmoid, bias, 4 of 8 groups: 132 us with choices and 64-bit
-// maxima in LDS; 28.6 by lane moves; 21.4 with no loop over tokens around it all (which kept constants in 80 registers), the
+// maxima in LDS; 28.6 by lane moves; 21.2 with no loop over tokens around it all (which kept constants in 80 registers), the
 // scoring's branch outside the experts' loop (their chains side by side, one set of constants), which of a lane's experts it is
 // as lane masks, and the groups from registers.  (Choices in float32 first, and in 64 bits only for the tokens where two come
 // near each other: no gain.)
@@ -327,8 +327,8 @@ void launch(const RouterParams& p, hipStream_t st) {
 }
 
 // Few tokens: a wavefront each, for its latency.  From 4096 on, where every SIMD has some, several share one (8192 x 128, top 8:
-// 5.5 us, 9.5 with a wavefront each; at 2048 tokens x 256 4.9 and, shared, 6.0).  With a bias and more than 128 experts two
-// instead of four (4096 x 256, 4 of 8 groups: 11.0 us, 13.6 with four; the same from 16384 on).
+// 5.5 us, 9.3 with a wavefront each; 2048 x 256 4.9 and, shared, 6.6).  With a bias and more than 128 experts two instead of
+// four (4096 x 256, sigmoid, 4 of 8 groups: 9.2 us, 11.5 with four; without a bias, 16384 x 256: 12.0 with two, 11.3 with four).
 template <bool BIASED>
 void launch_form(const RouterParams& p, hipStream_t st) {
   const bool many = p.tokens >= 4096;

@@ -258,8 +258,9 @@ def topk_routing(gating_output: torch.Tensor, topk: int, scoring_func: str = "so
     With num_expert_group > 1 neighbouring experts form groups, and only those of the topk_group best groups may be
     chosen; a group counts by its best expert or, with a bias, by the sum of its two best.  The weights are the scores of
     the chosen, divided by their sum if `renormalize`, times routed_scaling_factor.  A NaN logit counts as -inf; a token
-    whose logits are all -inf gets the lowest experts that may be chosen, with softmax weights 0.  At most 1024 experts,
-    64 groups, 64 choices."""
+    whose logits are all -inf gets the lowest experts that may be chosen, with softmax weights 0.  With a bias an expert of
+    logit -inf has the score 0 and may still be chosen, by its bias: a bias of -inf leaves it out (a NaN bias does too).
+    At most 1024 experts, 64 groups, 64 choices."""
     return _topk_routing(gating_output, topk, scoring_func, renormalize, bias, num_expert_group, topk_group,
                          routed_scaling_factor)
 
