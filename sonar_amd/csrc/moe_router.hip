@@ -4,15 +4,15 @@
 // Equal choices go to the lowest expert.  What decides, s + bias and the groups' sums, is taken in 64 bits: two experts whose
 // float32 sums are equal are told apart, as a 64-bit program would.
 //
-// A choice is kept as two words whose unsigned order is that of the numbers: its float32 rounding and what that leaves (no
-// second word without a bias).  A lane holds R neighbouring experts of a token and knows the largest of them.  Every round finds
+// A choice is kept as two words whose unsigned order is that of the numbers: its float32 rounding and what that leaves (formed
+// where first words are equal; none without a bias).  A lane holds R neighbouring experts of a token and knows the largest of them.  Every round finds
 // the largest first word over the token's lanes by lane moves, asks which lanes have it (and looks at the second words
 // only if several have), takes the lowest lane's lowest expert, and that lane looks for its next.  Word 0 is below every
 // number's: an expert that is taken, left out or not there.
 // Groups whose experts lie in 2^n whole lanes are judged from registers, others through LDS.
 // Bound by the vector instructions (the 64-bit exponentials and the rounds; 4 to 8 wavefronts a SIMD take the same time), and by
 // the latency of their chains where tokens are few.  16384 x 256, sigmoid, bias, 4 of 8 groups: 132 us with choices and 64-bit
-// maxima in LDS; 28.6 by lane moves; 21.2 with no loop over tokens around it all (which kept constants in 80 registers), the
+// maxima in LDS; 28.6 by lane moves; 20.9 with no loop over tokens around it all (which kept constants in 80 registers), the
 // scoring's branch outside the experts' loop (their chains side by side, one set of constants), which of a lane's experts it is
 // as lane masks, and the groups from registers.  (Choices in float32 first, and in 64 bits only for the tokens where two come
 // near each other: no gain.)
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
   const bool there = token < p.tokens;
   const long at = (there ? token : p.tokens - 1) * p.row_stride;
   float x[R];
-  uint32_t key[R], low[R];   // of the choices
+  uint32_t key[R];   // of the choices
   if (p.dtype == SONAR_DTYPE_F32) load_logits((const float*)p.logits + at, e0, E, vectors, x);
   else if (p.dtype == SONAR_DTYPE_BF16) load_logits((const __bf16*)p.logits + at, e0, E, vectors, x);
   else load_logits((const _Float16*)p.logits + at, e0, E, vectors, x);
@@ -170,8 +170,7 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
     for (int r = 0; r < R; ++r) {
       choice[r] += (double)bias[r];
       if (choice[r] != choice[r]) choice[r] = -(double)inf;
-      const float near = (float)choice[r], rest = (float)(choice[r] - (double)near);
-      key[r] = ordered(near), low[r] = ordered(rest == rest ? rest : 0.0f);
+      key[r] = ordered((float)choice[r]);
     }
   } else {
 #pragma unroll
@@ -239,10 +238,14 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
 #pragma unroll
     for (int r = 1; r < R; ++r) best = larger(best, key[r]);
   };
+  auto low = [&](int r) {   // the second word: what the first leaves of the choice
+    const float rest = (float)(choice[r] - (double)(float)choice[r]);
+    return ordered(rest == rest ? rest : 0.0f);
+  };
   auto low_of_best = [&]() {
     uint32_t most = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) most = larger(most, key[r] == best ? low[r] : 0);
+    for (int r = 0; r < R; ++r) most = larger(most, key[r] == best ? low(r) : 0);
     return most;
   };
   look();
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
         const uint32_t rest = low_of_best();
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const bool it = !seen && key[r] == best && low[r] == rest;
+          const bool it = !seen && key[r] == best && low(r) == rest;
           at_r = it ? r : at_r;
           key[r] = it ? 0 : key[r];
           seen = seen || it;
@@ -291,21 +294,30 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  double total = 0;
-  for (int pass = p.renormalize ? 0 : 1; pass < 2; ++pass)   // the sum of the chosen scores, then the weights
-    for (int k = l; k < (p.topk + LANES - 1) / LANES * LANES; k += LANES) {
-      const int expert = chosen[wave][seg * kMaxTopk + min(k, p.topk - 1)];
-      const float logit = logit_at(p, at + expert);
-      double w = softmax ? term(logit, top) : sigmoid(logit);
-      if (softmax && sum > 0) w /= sum;
-      if (pass == 0) {
-        total += over_lanes<LANES>(k < p.topk ? w : 0.0, add);
-      } else if (there && k < p.topk) {
-        if (total > 0) w /= total;
-        p.weights[token * p.topk + k] = (float)(w * p.factor);
-        p.ids[token * p.topk + k] = expert;
-      }
+  // the chosen scores, their sum if it divides them, then the weights; a choice a lane, and again from the first for more
+  double total = 0, w = 0;
+  int expert = 0;
+  auto take = [&](int k) {
+    expert = chosen[wave][seg * kMaxTopk + min(k, p.topk - 1)];
+    const float logit = logit_at(p, at + expert);
+    w = softmax ? term(logit, top) : sigmoid(logit);
+    if (softmax && sum > 0) w /= sum;
+  };
+  const int end = (p.topk + LANES - 1) / LANES * LANES;
+  if (p.renormalize)
+    for (int k = l; k < end; k += LANES) {
+      take(k);
+      total += over_lanes<LANES>(k < p.topk ? w : 0.0, add);
     }
+  const bool held = p.renormalize && end == LANES;
+  for (int k = l; k < end; k += LANES) {
+    if (!held) take(k);
+    if (there && k < p.topk) {
+      if (total > 0) w /= total;
+      p.weights[token * p.topk + k] = (float)(w * p.factor);
+      p.ids[token * p.topk + k] = expert;
+    }
+  }
 }
 
 template <int LANES, int R, bool BIASED>
