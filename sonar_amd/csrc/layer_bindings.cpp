@@ -8,6 +8,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -145,8 +146,9 @@ std::tuple<Tensor, Tensor> topk_routing(const Tensor& logits, int64_t topk, c10:
   int64_t stride = experts;
   const Tensor rows = experts > 0 ? rows_of(logits, experts, stride) : logits;
   const Tensor bc = bias.has_value() ? bias->contiguous() : Tensor();
-  Tensor weights = new_tensor(logits, {logits.size(0), std::max<int64_t>(topk, 0)}, at::kFloat);
-  Tensor ids = new_tensor(logits, {logits.size(0), std::max<int64_t>(topk, 0)}, at::kInt);
+  const int64_t columns = std::max<int64_t>(std::min(topk, experts), 0);   // (of a call that is refused below, none too many)
+  Tensor weights = new_tensor(logits, {logits.size(0), columns}, at::kFloat);
+  Tensor ids = new_tensor(logits, {logits.size(0), columns}, at::kInt);
   raise_if_failed(sonar_topk_routing(
       rows.const_data_ptr(), dtype, stride, bias.has_value() ? static_cast<const float*>(bc.const_data_ptr()) : nullptr,
       static_cast<float*>(weights.mutable_data_ptr()), static_cast<int32_t*>(ids.mutable_data_ptr()), logits.size(0), experts, topk,

@@ -78,6 +78,8 @@ def _route(hidden_states, logits, topk, scoring_func, renormalize, bias, groups,
         bias = bias.to(torch.float32)
     if logits.is_cuda:
         return ops.topk_routing(logits, topk, scoring_func, renormalize, bias, groups, kept_groups, factor)
+    if bias is not None:
+        bias = bias.reshape(experts)
     return _topk_routing_torch(logits, topk, scoring_func, renormalize, bias, groups, kept_groups, factor)
 
 

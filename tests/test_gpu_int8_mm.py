@@ -171,6 +171,20 @@ def test_empty():
     assert torch.equal(c, bias.expand(5, 48))
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 600000), (40, 4096, 600000), (300, 4096, 600000), (300, 64, 8400000), (70, 63, 33000000), (300, 63, 8400000)])
+def test_offsets_past_32_bits(m, k, n):
+    """Weights of more than 2^31 bytes, results of more than 2^31 numbers: the first and last channels are those of a call of their own."""
+    from sonar_amd import ops
+    gen = torch.Generator(device=DEV).manual_seed(m + k)
+    a = torch.randint(-127, 128, (m, k), device=DEV, generator=gen, dtype=torch.int8)
+    b = torch.randint(-127, 128, (n, k), device=DEV, generator=gen, dtype=torch.int8)
+    sa, sb = torch.rand(m, device=DEV, generator=gen), torch.rand(n, device=DEV, generator=gen)
+    got = ops.scaled_mm_int8(a, b.t(), sa, sb, torch.bfloat16)
+    for start in (0, n // 2 - 100, n - 700):
+        want = ops.scaled_mm_int8(a, b[start:start + 700].t(), sa, sb[start:start + 700], torch.bfloat16)
+        assert torch.equal(got[:, start:start + 700], want)
+
+
 def test_scales_that_are_no_numbers():
     """A NaN or infinite scale reaches its own row or column and no other."""
     from sonar_amd import ops

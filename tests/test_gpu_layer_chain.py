@@ -108,6 +108,33 @@ def test_layer_in_a_graph(layer):
                 assert torch.equal(a, b), i
 
 
+def test_two_graphs_that_share_a_pool():
+    """Replayed in turn, with eager calls between them, each gives what eager calls give."""
+    from sonar_amd import ops
+    xs, graphs, held = [], [], []
+    pool = torch.cuda.graph_pool_handle()
+    b = torch.randint(-127, 128, (512, 14336), device=DEV, dtype=torch.int8)
+    sb = torch.rand(512, device=DEV)
+    w = torch.ones(14336, device=DEV, dtype=torch.bfloat16)
+    def call(x):
+        q, s, _, y = ops.rms_norm_per_token_quant(x, w, 1e-5, with_norm=True)
+        return ops.scaled_mm_int8(q, b.t(), s, sb, torch.bfloat16), *ops.topk_routing(y[:, :256], 8, "sigmoid", True, sb[:256], 8, 4)
+    for m in (40, 200):   # (both split K)
+        xs.append(torch.randn((m, 14336), device=DEV, dtype=torch.bfloat16))
+        call(xs[-1])
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=pool):
+            out = call(xs[-1])
+            held.append([t.clone() for t in out])
+    for turn in range(4):
+        for x, graph, mine in zip(xs, graphs, held):
+            x.normal_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(mine, call(x))), turn
+
+
 def test_opcheck():
     """Schema, fake results, no autograd formula, dynamic shapes: what the ops declare is what they do."""
     from sonar_amd import ops  # noqa: F401

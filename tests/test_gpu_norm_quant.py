@@ -102,6 +102,18 @@ def test_more_rows_than_workgroups(rows, cols, residual):
             assert a is None and b is None or torch.equal(a[i:i + step], b)
 
 
+@pytest.mark.parametrize("rows,cols", [(600000, 4096), (2150000, 1003)])
+def test_offsets_past_32_bits(rows, cols):
+    from sonar_amd import ops
+    x = torch.empty((rows, cols), device=DEV, dtype=torch.float16).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    w = torch.ones(cols, device=DEV, dtype=torch.float16)
+    got = ops.rms_norm_per_token_quant(x, w, EPS, torch.int8, x, True)
+    for start in (0, rows // 2, rows - 50):
+        want = ops.rms_norm_per_token_quant(x[start:start + 50], w, EPS, torch.int8, x[start:start + 50], True)
+        for a, b in zip(got, want):
+            assert torch.equal(a[start:start + 50], b)
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("cols,pitch,shift", [(512, 520, 0), (512, 513, 0), (512, 512, 1), (500, 512, 4), (4096, 4100, 0), (24, 64, 8)])
 def test_strides_and_alignment(dtype, cols, pitch, shift):

@@ -155,6 +155,19 @@ def test_more_tokens_than_a_launch_takes():
     check(x[-64:].cpu(), 2, "softmax", True, None)
 
 
+@pytest.mark.parametrize("groups,kept", [(1, 1), (8, 4), (5, 2)])
+def test_offsets_past_32_bits(groups, kept):
+    from sonar_amd import ops
+    tokens, experts = 8400000, 260 if groups == 5 else 256
+    x = torch.empty((tokens, experts), device=DEV, dtype=torch.bfloat16).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    bias = torch.linspace(-0.1, 0.1, experts, device=DEV)
+    args = 8, "sigmoid", True, bias, groups, kept, 2.5
+    got = ops.topk_routing(x, *args)
+    for start in (0, tokens // 2, tokens - 5000):
+        want = ops.topk_routing(x[start:start + 5000], *args)
+        assert all(torch.equal(a[start:start + 5000], b) for a, b in zip(got, want))
+
+
 def test_a_bias_that_masks():
     """Experts that the bias switches off, and choices that differ in the last bits of the sum."""
     x, _ = make(8, 12, 64)
