@@ -82,7 +82,7 @@ int sonar_topk_routing(const void* logits, int dtype, int64_t row_stride, const 
                        int renormalize, int64_t groups, int64_t kept_groups, double factor, void* stream);
 
 /* Diagnostics for tests.  sonar_debug_int8_choice: the number of the kernel form that sonar_scaled_mm_int8 takes for a call
- * (0 general, 1 to 3 streams of up to 16, 16 and 32 rows, 4 to 8 tiles of 64 x 64, 64 x 128, 128 x 128, 256 x 128, 256 x 256) and
+ * (0 general, 1 and 2 streams of up to 16 rows, 3 streams of blocks of 32, 4 to 8 tiles of 64 x 64, 64 x 128, 128 x 128, 256 x 128, 256 x 256) and
  * in how many parts it splits K; runs on the host.  sonar_debug_int8_form: the calling thread's calls take that form (-1: the
  * rule's again); a call that a stream form has too many rows for is refused. */
 int sonar_debug_int8_choice(int64_t size_m, int64_t size_n, int64_t size_k, int aligned, int* splits);

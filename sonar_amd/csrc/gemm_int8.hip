@@ -3,7 +3,7 @@
 // Both operands lie along K, as a checkpoint and a quantiser leave them, and both are read as they lie: nothing is laid
 // out anew.  The sums are integers, so every kernel, split and order gives the same bits.
 //
-//   int8_stream_kernel   up to 16 (32) rows: bound by the bytes of the weight
+//   int8_stream_kernel   up to 16 (32) rows: bound by the bytes of the weight; few rows of any alignment in blocks of 32
 //   int8_tile_kernel     more rows, five tile sizes: bound by the matrix pipes from a few hundred rows on
 //   int8_join_kernel     sums of a K that was split over workgroups
 //   int8_pad_kernel      rows that no 16-byte vector is aligned to, laid down aligned for the tiles
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(512) void int8_general_kernel(const Int8Params p, i
 }
 
 // ---- few rows
-// Up to 16 MB tokens: the weight is read once, past LDS, straight into the operand registers of 16 x 16 x 64 matrix
+// Up to 16 MB tokens (or blocks of as many): the weight is read once a block, past LDS, straight into the operand registers of 16 x 16 x 64 matrix
 // instructions (its 16 channels the first operand), 64 bytes of a row an instruction; rows of any alignment (ODD: not of words).  A workgroup owns 16 NB
 // channels; its wavefronts take steps of 128 bytes of K in turn, so that together they read a run of each row, and join their
 // sums through LDS.  A wavefront has DEEP steps of loads in flight, 4 KB at DEEP = 2: with 16 wavefronts on each compute unit
@@ -226,11 +226,11 @@ __global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8P
   __shared__ intx4_t sums[kWaves][NB * MB][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, at = 16 * (lane >> 4);   // an operand's row, and its 16 bytes of 64
-  const long n0 = (long)blockIdx.x * (16 * NB);
+  const long n0 = (long)blockIdx.x * (16 * NB), m0 = (long)blockIdx.y * (16 * MB);
   const int8_t* a_rows[MB];
   const int8_t* b_rows[NB];
 #pragma unroll
-  for (int i = 0; i < MB; ++i) a_rows[i] = p.a + min((long)(16 * i + r), (long)p.m - 1) * p.lda;   // (tokens past the end: the last one's)
+  for (int i = 0; i < MB; ++i) a_rows[i] = p.a + min(m0 + 16 * i + r, (long)p.m - 1) * p.lda;   // (tokens past the end: the last one's)
 #pragma unroll
   for (int j = 0; j < NB; ++j) b_rows[j] = p.b + min(n0 + 16 * j + r, (long)p.n - 1) * p.ldb;
   intx4_t acc[NB][MB] = {};
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void int8_stream_kernel(const Int8P
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) v += sums[w][x][lane];
     // a lane has token 16 i + lane % 16 and channels 4 (lane / 16) + 0 .. 3 of the sixteen
-    const long m = 16 * (x % MB) + r, n = n0 + 16 * (x / MB) + 4 * (lane >> 4);
+    const long m = m0 + 16 * (x % MB) + r, n = n0 + 16 * (x / MB) + 4 * (lane >> 4);
     if (m >= p.m) continue;
     const float sa = p.a_scales[p.a_many ? m : 0];
     T* out = (T*)p.c + m * p.n + n;
@@ -663,13 +663,15 @@ struct FormCost {
   int rows, cols;
   float round, per_k;
 };
-constexpr FormCost kCosts[kForms] = {{64, 64, 4.0f, 5.5f},      {16, 32, 0, 0},        {16, 16, 0, 0},        {32, 16, 0, 0}, {64, 64, 4.4f, 1.3f},
+constexpr FormCost kCosts[kForms] = {{64, 64, 4.0f, 5.5f},      {16, 32, 0, 0},        {16, 16, 0, 0},        {32, 16, 0.35f, 2.5f}, {64, 64, 4.4f, 1.3f},
                                      {64, 128, 5.0f, 2.0f}, {128, 128, 5.0f, 3.1f}, {256, 128, 6.5f, 4.6f}, {256, 256, 8.1f, 8.3f}};
+constexpr float kStreamUs = 3.0f;   // start and end of the streams' rounds, which overlap
 constexpr float kLaunchUs = 4.5f, kBytesPerUs = 4.5e6f;   // a launch more, for partial sums or aligned copies; their bytes
 
 struct Int8Choice {
   int form, splits;
 };
+constexpr int64_t kStreamRows = 32 * 65535;   // a grid's second dimension
 thread_local Int8Choice g_forced = {-1, 1};
 
 int64_t tiles_of(int form, int64_t m, int64_t n) {
@@ -694,6 +696,11 @@ Int8Choice choose_form(int64_t m, int64_t n, int64_t k, bool aligned) {
     best = {kGeneral, 1};
     least = (float)((tiles_of(kGeneral, m, n) + 255) / 256) * (kCosts[kGeneral].round + kCosts[kGeneral].per_k * (float)k / 1024);
     copies = kLaunchUs + 2.0f * (float)(m + n) * (float)k / kBytesPerUs;
+    // The stream in blocks of 32 rows reads the weight once a block, but has sixteen wavefronts on 16 channels: 77 x 1003 x 1537
+    // 7.9 us, the general kernel 9.8; 200 x 2047 x 513 8.3 and 12.1; 200 x 1003 x 1537 12.9 and 10.1.
+    const float streams = kStreamUs + (float)((tiles_of(kStreamTwo, m, n) + 255) / 256) *
+                                          (kCosts[kStreamTwo].round + kCosts[kStreamTwo].per_k * (float)k / 1024);
+    if (m <= kStreamRows && streams < least) least = streams, best = {kStreamTwo, 1};
   }
   for (int form = kTile64; form <= kTile256; ++form)
     for (int splits = 1; splits <= 8 && may_split(splits, k); splits *= 2) {
@@ -745,7 +752,7 @@ int launch_tiles(const Int8Params& p, int splits, int* partial, bool vectors, hi
 
 template <typename T, int kWaves, int MB, int NB, int DEEP>
 void launch_stream(const Int8Params& p, bool vectors, hipStream_t st) {
-  const int grid = (p.n + 16 * NB - 1) / (16 * NB);
+  const dim3 grid((p.n + 16 * NB - 1) / (16 * NB), (p.m + 16 * MB - 1) / (16 * MB));
   if (((uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.lda | (uintptr_t)p.ldb) % 4 != 0)
     int8_stream_kernel<T, true, kWaves, MB, NB, DEEP < 2 ? DEEP : 2><<<grid, 64 * kWaves, 0, st>>>(p, vectors);
   else
@@ -823,7 +830,8 @@ extern "C" int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const
   if (scratch == nullptr) scratch_bytes = 0;
   Int8Choice s = choose_form(size_m, size_n, size_k, aligned);
   if (is_tile(s.form) && size_k < 16) s = {kGeneral, 1};
-  SONAR_REQUIRE(is_tile(s.form) || s.form == kGeneral || size_m <= kCosts[s.form].rows, "form %d takes %d rows", s.form, kCosts[s.form].rows);
+  SONAR_REQUIRE(is_tile(s.form) || s.form == kGeneral || size_m <= (s.form == kStreamTwo ? kStreamRows : kCosts[s.form].rows),
+                "form %d does not take %ld rows", s.form, (long)size_m);
   const size_t padded = padded_bytes(s, size_m, size_n, size_k, aligned);
   if (padded > scratch_bytes) s = {kGeneral, 1};
   if (is_tile(s.form) && padded > 0) {

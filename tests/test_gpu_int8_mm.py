@@ -66,12 +66,12 @@ def test_columns(n, m, k):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 4096, 4096), (16, 4096, 6144), (64, 2880, 5760), (200, 4096, 6144), (333, 2880, 5760),
-                                   (700, 14336, 512), (1500, 1024, 4096), (2050, 4096, 1030), (77, 1003, 1537)])
+                                   (700, 14336, 512), (1500, 1024, 4096), (2050, 4096, 1030), (77, 1003, 1537), (200, 1003, 1537)])
 def test_larger(m, k, n):
     run(m, k, n, bias=True)
 
 
-FORMS = {0: 1 << 20, 1: 16, 2: 16, 3: 32, 4: 1 << 20, 5: 1 << 20, 6: 1 << 20, 7: 1 << 20, 8: 1 << 20}   # and the rows each takes
+FORMS = {0: 1 << 20, 1: 16, 2: 16, 3: 1 << 20, 4: 1 << 20, 5: 1 << 20, 6: 1 << 20, 7: 1 << 20, 8: 1 << 20}   # and the rows each takes
 
 
 @pytest.fixture

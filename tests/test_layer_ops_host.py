@@ -100,7 +100,8 @@ def test_the_rule_of_the_int8_product():
     assert choice(1, 4096, 4096) == (2, 1) and choice(16, 4097, 4096) == (1, 1)
     assert choice(17, 4096, 6144) == (3, 1) and choice(32, 4112, 4096)[0] >= 4 and choice(32, 4112, 4096, 0) == (3, 1)
     assert choice(17, 28672, 100) == (3, 1)           # K is no multiple of 16: unaligned whatever the strides are
-    assert choice(33, 100, 15) == (0, 1) and choice(77, 1537, 1003) == (0, 1) and choice(77, 1537, 4095)[0] >= 4
+    assert choice(33, 100, 15) == (0, 1) and choice(77, 1537, 1003) == (3, 1) and choice(200, 1537, 1003) == (0, 1)
+    assert choice(77, 1537, 4095)[0] >= 4 and choice(1 << 24, 1, 17)[0] >= 4
     assert choice(8192, 28672, 4096) == (8, 1) and choice(2048, 4096, 14336) == (7, 1)
     form, splits = choice(64, 256, 14336)
     assert form == 4 and splits > 1
