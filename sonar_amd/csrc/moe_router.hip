@@ -2,19 +2,19 @@
 //   s = softmax(x) or 1 / (1 + exp(-x));  c = s + bias, or x itself, which has the order of s, without a bias
 //   ids: the topk largest c, of the experts in the best groups where there are groups;  weights: s of them
 // Equal choices go to the lowest expert.  What decides, s + bias and the groups' sums, is taken in 64 bits: two experts whose
-// float32 sums are equal are told apart, as a 64-bit program would.
+// float32 sums are equal, or whose scores are below float32's range, are told apart.
 //
-// A choice is kept as two words whose unsigned order is that of the numbers: its float32 rounding and what that leaves (formed
-// where first words are equal; none without a bias).  A lane holds R neighbouring experts of a token and knows the largest of them.  Every round finds
-// the largest first word over the token's lanes by lane moves, asks which lanes have it (and looks at the second words
-// only if several have), takes the lowest lane's lowest expert, and that lane looks for its next.  Word 0 is below every
-// number's: an expert that is taken, left out or not there.
+// A choice is kept as words whose unsigned order is that of the numbers: without a bias one, of the float32 logit; with a bias
+// the two of the double, the lower one looked at only where upper ones are equal.  A lane holds R neighbouring experts of a
+// token and knows the largest of them.  Every round finds the largest first word over the token's lanes by lane moves, asks which
+// lanes have it (and looks at the second words only if several have), takes the lowest lane's lowest expert, and that lane looks
+// for its next.  Word 0 is below every number's: an expert that is taken, left out or not there.
 // Groups whose experts lie in 2^n whole lanes are judged from registers, others through LDS.
 // Bound by the vector instructions (the 64-bit exponentials and the rounds; 4 to 8 wavefronts a SIMD take the same time), and by
 // the latency of their chains where tokens are few.  16384 x 256, sigmoid, bias, 4 of 8 groups: 132 us with choices and 64-bit
 // maxima in LDS; 28.6 by lane moves; 20.9 with no loop over tokens around it all (which kept constants in 80 registers), the
 // scoring's branch outside the experts' loop (their chains side by side, one set of constants), which of a lane's experts it is
-// as lane masks, and the groups from registers.  (Choices in float32 first, and in 64 bits only for the tokens where two come
+// as lane masks, and the groups from registers; 19.6 with the words of the double itself (float32 and what it leaves before).  (Choices in float32 first, and in 64 bits only for the tokens where two come
 // near each other: no gain.)
 #include "common.hpp"
 #include "lane_reduce.hpp"
@@ -43,6 +43,16 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 }
 __device__ __forceinline__ float number_of(uint32_t w) {
   return __builtin_bit_cast(float, w ^ (w & 0x80000000u ? 0x80000000u : 0xffffffffu));
+}
+// double -> two words, by the first of which and, where equal, the second it is ordered; the first is above 0 (numbers and
+// infinities, no negative zero)
+__device__ __forceinline__ uint32_t upper_ordered(double d) {
+  const TwoWords w = __builtin_bit_cast(TwoWords, d);
+  return (uint32_t)w.hi ^ ((uint32_t)(w.hi >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint32_t lower_ordered(double d) {
+  const TwoWords w = __builtin_bit_cast(TwoWords, d);
+  return (uint32_t)(w.lo ^ (w.hi >> 31));
 }
 
 // The logits of experts e0 .. e0 + R - 1 of a row; -infinity for a NaN and behind the end.  `vectors`: 16 bytes at a time lie
@@ -168,9 +178,9 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
     load_logits(p.bias, e0, E, vectors, bias);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      choice[r] += (double)bias[r];
+      choice[r] += (double)bias[r];   // (scores are 0 or above: no sum is a negative zero)
       if (choice[r] != choice[r]) choice[r] = -(double)inf;
-      key[r] = ordered((float)choice[r]);
+      key[r] = upper_ordered(choice[r]);
     }
   } else {
 #pragma unroll
@@ -238,10 +248,7 @@ __global__ __launch_bounds__(64 * kWaves) void topk_routing_kernel(const RouterP
 #pragma unroll
     for (int r = 1; r < R; ++r) best = larger(best, key[r]);
   };
-  auto low = [&](int r) {   // the second word: what the first leaves of the choice
-    const float rest = (float)(choice[r] - (double)(float)choice[r]);
-    return ordered(rest == rest ? rest : 0.0f);
-  };
+  auto low = [&](int r) { return lower_ordered(choice[r]); };   // the second word
   auto low_of_best = [&]() {
     uint32_t most = 0;
 #pragma unroll
