@@ -27,7 +27,7 @@ const char* sonar_layer_last_error(void);
  *   z = T(x + residual) (x itself without a residual), y = z * r * weight in fp32, r = 1 / sqrt(mean(z^2) + epsilon),
  *   int8: scale = max(max|y|, 1e-10) / 127, code = y * (127 / max|y|) rounded half away from zero,
  *   fp8:  scale = max(max|y| / 448, 1 / (448 * 512)), code = float8_e4m3fn(clamp(y * (1 / scale), -448, 448)).
- * The codes and scales are those of sonar_per_token_quant_int8 / _fp8 of the fp32 numbers y.
+ * The codes and scales are those of sonar_per_token_quant_int8 / _fp8 of the fp32 numbers y where all of them are numbers.
  *   x             dtype[rows][x_row_stride]
  *   residual      dtype[rows][residual_row_stride] or NULL
  *   weight        dtype[cols]
@@ -37,7 +37,8 @@ const char* sonar_layer_last_error(void);
  *   q             int8 or float8_e4m3fn [rows][cols] (q_dtype: SONAR_ADTYPE_INT8 / _FP8)
  *   scales        float[rows]
  *   epsilon       at least 2^-126, so that rows of zeros stay zeros
- * A row with an infinity or a NaN in z has the scale NaN. */
+ * A row of y with a NaN (z holds one or an infinity, or weight holds a NaN) has the scale NaN and codes 0 (int8) or NaN (fp8);
+ * an infinite weight gives the scale infinity, or NaN where z is 0 at its column. */
 int sonar_rms_norm_per_token_quant(const void* x, int64_t x_row_stride, const void* residual,
                                    int64_t residual_row_stride, const void* weight, void* residual_out,
                                    void* norm_out, void* q, int q_dtype, float* scales, int dtype,

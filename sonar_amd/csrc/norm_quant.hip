@@ -56,21 +56,24 @@ __device__ __forceinline__ float inverse_root(double x) {
   return x <= 1.7976931348623157e308 ? (float)y : (float)(x - x);   // (infinities and NaN: NaN)
 }
 
-// A row's scale, and what its numbers are multiplied by; `r` NaN marks a row whose sum is none.
+// A NaN stays one in these (the instructions of three operands; fmaxf and fminf would drop it).
+__device__ __forceinline__ float larger_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float smaller_of(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+
+// A row's scale, and what its numbers are multiplied by; both NaN where one of its numbers is.
 template <bool FP8>
-__device__ __forceinline__ void scale_of(float most, float r, float& scale, float& by) {
+__device__ __forceinline__ void scale_of(float most, float& scale, float& by) {
   if (FP8) {
-    scale = fmaxf(most / 448.0f, 1.0f / (448.0f * 512.0f));
+    scale = larger_of(most / 448.0f, 1.0f / (448.0f * 512.0f));
     by = 1.0f / scale;
   } else {
-    most = fmaxf(most, 1e-10f);
+    most = larger_of(most, 1e-10f);
     scale = most / 127.0f;
     by = 127.0f / most;
   }
-  if (r != r) scale = r;
 }
 
-// A code in the low byte: halves away from zero (int8), the nearest float8_e4m3fn.  A NaN's is 0 (int8).
+// A code in the low byte: halves away from zero (int8), the nearest float8_e4m3fn.  A NaN's is 0 (int8), the type's NaN (fp8).
 __device__ __forceinline__ int int8_code(float y, float by) {
 #pragma clang fp contract(off)
   const float t = y * by;
@@ -79,7 +82,7 @@ __device__ __forceinline__ int int8_code(float y, float by) {
 __device__ __forceinline__ float fp8_number(float y, float by) {
 #pragma clang fp contract(off)
   const float t = y * by;
-  return fminf(fmaxf(t, -448.0f), 448.0f);
+  return smaller_of(larger_of(t, -448.0f), 448.0f);
 }
 
 // Eight neighbouring numbers.
@@ -171,7 +174,7 @@ __global__ __launch_bounds__(THREADS > kThreads ? THREADS : kThreads) void rms_n
     float most = 0.0f;
     auto larger = [&](const Eight<T>& v, const Eight<T>& w) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v.at(e) * r * w.at(e)));
+      for (int e = 0; e < 8; ++e) most = larger_of(most, fabsf(v.at(e) * r * w.at(e)));
     };
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
@@ -182,10 +185,10 @@ __global__ __launch_bounds__(THREADS > kThreads ? THREADS : kThreads) void rms_n
         v.load(again + c), w.load((const T*)p.weight + c);
         larger(v, w);
       }
-    auto max_of = [](float a, float b) { return fmaxf(a, b); };
+    auto max_of = [](float a, float b) { return larger_of(a, b); };
     most = THREADS == 64 ? over_wave(most, 0.0f, max_of) : over_block<THREADS>(most, 0.0f, mosts, max_of);
     float scale, by;
-    scale_of<FP8>(most, r, scale, by);
+    scale_of<FP8>(most, scale, by);
     if (first == 0) p.scales[row] = scale;
     auto code = [&](const Eight<T>& v, const Eight<T>& w, uint32_t c) {
       float y[8];
@@ -249,10 +252,10 @@ __global__ __launch_bounds__(kThreads) void rms_norm_quant_any_kernel(const Norm
     sum = over_block<kThreads>(sum, 0.0, sums, [](double a, double b) { return a + b; });
     const float r = inverse_root(__builtin_fma(sum, p.inverse_cols, p.epsilon));
     float most = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += kThreads) most = fmaxf(most, fabsf((float)z[c] * r * (float)weight[c]));
-    most = over_block<kThreads>(most, 0.0f, mosts, [](float a, float b) { return fmaxf(a, b); });
+    for (int c = threadIdx.x; c < cols; c += kThreads) most = larger_of(most, fabsf((float)z[c] * r * (float)weight[c]));
+    most = over_block<kThreads>(most, 0.0f, mosts, [](float a, float b) { return larger_of(a, b); });
     float scale, by;
-    scale_of<FP8>(most, r, scale, by);
+    scale_of<FP8>(most, scale, by);
     if (threadIdx.x == 0) p.scales[row] = scale;
     for (int c = threadIdx.x; c < cols; c += kThreads) {
       const float y = (float)z[c] * r * (float)weight[c];

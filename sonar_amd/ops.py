@@ -231,7 +231,8 @@ def rms_norm_per_token_quant(x: torch.Tensor, weight: torch.Tensor, epsilon: flo
     (..., 1) of y as per_token_quant_int8 / _fp8 make them, what `marlin_gemm` and `scaled_mm_int8` take as `a` and
     `a_scales`; z where a residual was given, the next residual, else None; y rounded to x's type where `with_norm`
     (for a router, which reads 16 bits), else None.  The codes are those of y itself, not of the rounded norm.
-    epsilon is at least 2^-126, so that rows of zeros stay zeros.  A row with an infinity or a NaN in z has the scale NaN."""
+    epsilon is at least 2^-126, so that rows of zeros stay zeros.  A row with an infinity or a NaN in z has the scale NaN, and
+    so has every row where the weight holds a NaN; the codes are then 0 (int8) or NaN (fp8)."""
     got = _rms_norm_per_token_quant(x, weight, residual, epsilon, quant_dtype, with_norm)
     return got[0], got[1], got[2] if residual is not None else None, got[-1] if with_norm else None
 
