@@ -148,6 +148,10 @@ def lib_path() -> str:
     return _LIB_PATH
 
 
+def layer_path() -> str:
+    return _LAYER_PATH
+
+
 def _open(path: str, prototypes) -> ctypes.CDLL:
     if not os.path.exists(path):
         raise ImportError(

@@ -1,7 +1,9 @@
 """Python op wrappers with the names and signatures of the reference's
 aphrodite/_custom_ops.py (:1363-1461 repack, :1472-1543 marlin_gemm,
 :3046-3141 moe_wna16_marlin_gemm).  Importing this module loads the HIP library
-and the torch op registration layer; it raises if either is missing."""
+and the torch op registration layer; it raises if either is missing.  The
+operators around the GEMMs are two libraries more: without those the module
+serves the rest, and a call of theirs raises."""
 from __future__ import annotations
 
 import os
@@ -16,19 +18,44 @@ _LAYER_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib"
 
 
 def _load_ops() -> None:
-    def load(library, path):
-        library()  # raises with build instructions when the HIP library is missing
-        if not os.path.exists(path):
-            raise ImportError(f"{path} is missing: build it with `python -m sonar_amd.build`")
-        torch.ops.load_library(path)
+    if hasattr(torch.ops._C, "marlin_gemm") and hasattr(torch.ops._C, "marlin_to_gfx950"):
+        return
+    _lib.load()  # raises with build instructions when the HIP library is missing
+    if not os.path.exists(_OPS_PATH):
+        raise ImportError(f"{_OPS_PATH} is missing: build it with `python -m sonar_amd.build`")
+    torch.ops.load_library(_OPS_PATH)
 
-    if not (hasattr(torch.ops._C, "marlin_gemm") and hasattr(torch.ops._C, "marlin_to_gfx950")):
-        load(_lib.load, _OPS_PATH)
-    if not hasattr(torch.ops.sonar_amd, "scaled_mm_int8"):
-        load(_lib.load_layer, _LAYER_OPS_PATH)
+
+def _load_layer_ops() -> list[str]:
+    """Loads the operators around the GEMMs; returns the files that this takes and that are missing."""
+    if hasattr(torch.ops.sonar_amd, "scaled_mm_int8"):
+        return []
+    missing = [path for path in (_lib.layer_path(), _LAYER_OPS_PATH) if not os.path.exists(path)]
+    if not missing:
+        _lib.load_layer()
+        torch.ops.load_library(_LAYER_OPS_PATH)
+    return missing
 
 
 _load_ops()
+_LAYER_MISSING = _load_layer_ops()
+
+
+def _register_layer_fakes(reg, quant_fake) -> None:
+    @reg("sonar_amd::rms_norm_per_token_quant")
+    def _(x, weight, residual, epsilon, quant_dtype, with_norm):
+        more = (residual is not None) + bool(with_norm)
+        return [*quant_fake(quant_dtype)(x), *(torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(more))]
+
+    @reg("sonar_amd::scaled_mm_int8")
+    def _(a, b, a_scales, b_scales, out_dtype, bias):
+        return torch.empty(a.shape[:-1] + (b.shape[1],), dtype=out_dtype, device=a.device)
+
+    @reg("sonar_amd::topk_routing")
+    def _(logits, topk, scoring_func, renormalize, bias, num_expert_group, topk_group, routed_scaling_factor):
+        shape = (logits.shape[0], topk)
+        return (torch.empty(shape, dtype=torch.float32, device=logits.device),
+                torch.empty(shape, dtype=torch.int32, device=logits.device))
 
 
 def _register_fakes() -> None:
@@ -65,21 +92,8 @@ def _register_fakes() -> None:
 
     reg("sonar_amd::per_token_quant_int8")(quant_fake(torch.int8))
     reg("sonar_amd::per_token_quant_fp8")(quant_fake(torch.float8_e4m3fn))
-
-    @reg("sonar_amd::rms_norm_per_token_quant")
-    def _(x, weight, residual, epsilon, quant_dtype, with_norm):
-        more = (residual is not None) + bool(with_norm)
-        return [*quant_fake(quant_dtype)(x), *(torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(more))]
-
-    @reg("sonar_amd::scaled_mm_int8")
-    def _(a, b, a_scales, b_scales, out_dtype, bias):
-        return torch.empty(a.shape[:-1] + (b.shape[1],), dtype=out_dtype, device=a.device)
-
-    @reg("sonar_amd::topk_routing")
-    def _(logits, topk, scoring_func, renormalize, bias, num_expert_group, topk_group, routed_scaling_factor):
-        shape = (logits.shape[0], topk)
-        return (torch.empty(shape, dtype=torch.float32, device=logits.device),
-                torch.empty(shape, dtype=torch.int32, device=logits.device))
+    if not _LAYER_MISSING:
+        _register_layer_fakes(reg, quant_fake)
 
     @reg("sonar_amd::gptq_marlin_moe_repack")
     def _(b_q_weight, perm, size_k, size_n):
@@ -213,10 +227,20 @@ def per_token_quant_fp8(x: torch.Tensor):
     return torch.ops.sonar_amd.per_token_quant_fp8(x)
 
 
-# (the ops themselves, not the names that look for an overload at every call)
-_rms_norm_per_token_quant = torch.ops.sonar_amd.rms_norm_per_token_quant.default
-_scaled_mm_int8 = torch.ops.sonar_amd.scaled_mm_int8.default
-_topk_routing = torch.ops.sonar_amd.topk_routing.default
+def _layer_op(name: str):
+    """An op of the layer library itself, not the name that looks for an overload at every call."""
+    if not _LAYER_MISSING:
+        return getattr(torch.ops.sonar_amd, name).default
+
+    def absent(*args):
+        raise ImportError(f"{' and '.join(_LAYER_MISSING)} missing: build with `python -m sonar_amd.build`; there is no "
+                          f"other implementation of {name}")
+    return absent
+
+
+_rms_norm_per_token_quant = _layer_op("rms_norm_per_token_quant")
+_scaled_mm_int8 = _layer_op("scaled_mm_int8")
+_topk_routing = _layer_op("topk_routing")
 
 
 def rms_norm_per_token_quant(x: torch.Tensor, weight: torch.Tensor, epsilon: float,
