@@ -56,7 +56,8 @@ int sonar_rms_norm_per_token_quant(const void* x, int64_t x_row_stride, const vo
  *             where K is split, aligned copies of rows that are not.  A smaller one or none is allowed and slower, with the
  *             same results.  Calls that overlap in time need scratches of their own.
  *   aligned   whether a, b and both row strides are multiples of 16 bytes, the strides below 2^23
- * size_m and size_n below 2^25. */
+ * size_m and size_n below 2^25.  A call of 2^22 tiles or more is refused: of 256 x 256 results, which are more than the card
+ * holds, or, where size_k is below 16 and where rows that are not aligned have no scratch, of 64 x 64. */
 size_t sonar_scaled_mm_int8_scratch_bytes(int64_t size_m, int64_t size_n, int64_t size_k, int aligned);
 int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const int8_t* b, int64_t b_row_stride, void* c,
                          const float* a_scales, int64_t a_scales_len, const float* b_scales,

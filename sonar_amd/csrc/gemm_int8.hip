@@ -672,6 +672,7 @@ struct Int8Choice {
   int form, splits;
 };
 constexpr int64_t kStreamRows = 32 * 65535;   // a grid's second dimension
+constexpr int64_t kMostTiles = (1 << 22) - 1;   // of a launch, the parts of K counted: 512 threads each are fewer than 2^32
 thread_local Int8Choice g_forced = {-1, 1};
 
 int64_t tiles_of(int form, int64_t m, int64_t n) {
@@ -736,8 +737,7 @@ int launch_tiles(const Int8Params& p, int splits, int* partial, bool vectors, hi
   TilePlan t;
   t.tiles_m = (int)(((int64_t)p.m + BM - 1) / BM), t.tiles_n = (int)(((int64_t)p.n + BN - 1) / BN);
   t.splits = splits;
-  const int64_t units = (int64_t)t.tiles_m * t.tiles_n * splits;
-  SONAR_REQUIRE(units < (1 << 22), "size_m = %d, size_n = %d: more tiles than a launch takes", p.m, p.n);
+  const int64_t units = (int64_t)t.tiles_m * t.tiles_n * splits;   // (kMostTiles at most)
   t.per_xcd = (int)((units + 7) / 8);
   if (kLds > 65536)
     SONAR_HIP(hipFuncSetAttribute((const void*)int8_tile_kernel<T, WM, MT, NT, KG, kStageK, kRing>,
@@ -772,7 +772,6 @@ int run_form(const Int8Params& p, const Int8Choice& s, int* partial, bool vector
     case kStreamTwo: launch_stream<T, 16, 2, 1, 2>(p, vectors, st); break;
     default: {
       const int64_t rows = ((int64_t)p.m + 63) / 64, cols = ((int64_t)p.n + 63) / 64;
-      SONAR_REQUIRE(rows * cols < (1 << 22), "size_m = %d, size_n = %d: more tiles than a launch takes", p.m, p.n);
       constexpr int kLds = 65536;
       int8_general_kernel<T><<<(int)(rows * cols), 512, kLds, st>>>(p, (int)cols, vectors);
     }
@@ -834,14 +833,16 @@ extern "C" int sonar_scaled_mm_int8(const int8_t* a, int64_t a_row_stride, const
                 "form %d does not take %ld rows", s.form, (long)size_m);
   const size_t padded = padded_bytes(s, size_m, size_n, size_k, aligned);
   if (padded > scratch_bytes) s = {kGeneral, 1};
-  if (is_tile(s.form) && padded > 0) {
+  if (!is_tile(s.form) || !may_split(s.splits, size_k) || padded + partial_bytes(s, size_m, size_n) > scratch_bytes) s.splits = 1;
+  SONAR_REQUIRE((s.form != kGeneral && !is_tile(s.form)) || tiles_of(s.form, size_m, size_n) * s.splits <= kMostTiles,
+                "size_m = %ld, size_n = %ld: more tiles than a launch takes", (long)size_m, (long)size_n);
+  if (is_tile(s.form) && padded > 0) {   // (the first launch: nothing is refused behind it)
     const int pitch = (int)padded_k(size_k);
     int8_t* copies = (int8_t*)scratch;
     const int64_t groups = (size_m + size_n + 3) / 4;
     int8_pad_kernel<<<(int)(groups < 16384 ? groups : 16384), 256, 0, st>>>(p, copies, copies + size_m * pitch, pitch);
     p.a = copies, p.b = copies + size_m * pitch, p.lda = p.ldb = p.k = pitch;
   }
-  if (!is_tile(s.form) || !may_split(s.splits, size_k) || padded + partial_bytes(s, size_m, size_n) > scratch_bytes) s.splits = 1;
   int* partial = s.splits > 1 ? (int*)((char*)scratch + padded) : nullptr;
   return dtype == SONAR_DTYPE_F16 ? run_form<_Float16>(p, s, partial, vectors, st) : run_form<__bf16>(p, s, partial, vectors, st);
 }
