@@ -8,6 +8,7 @@
 //   int8_join_kernel     sums of a K that was split over workgroups
 //   int8_pad_kernel      rows that no 16-byte vector is aligned to, laid down aligned for the tiles
 //   int8_general_kernel  such rows as they lie, of short K, and anything without scratch
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -658,7 +659,8 @@ __global__ __launch_bounds__(256) void int8_pad_kernel(const Int8Params p, int8_
 enum Form { kGeneral, kStream32, kStream16, kStreamTwo, kTile64, kTile128Wide, kTile128, kTile256Tall, kTile256, kForms };
 // Rows and columns of a form's tile, and what it takes (us): a round of 256 workgroups, and 1024 of K in it.  Fitted to 140
 // shapes of 24 to 4096 rows, 256 to 28672 channels, K of 2048 to 14336; the choice they make is 0.2 % slower than the best one
-// (geometric mean; at most 5 %).
+// (geometric mean; at most 6 %).  Of 118 with rows of any alignment, K of 24 to 14336, 2.1 % (at most 64 %: 86 x 4148 x 1955
+// takes tiles, 20.2 us, where the stream would take 12.3).
 struct FormCost {
   int rows, cols;
   float round, per_k;
@@ -666,6 +668,10 @@ struct FormCost {
 constexpr FormCost kCosts[kForms] = {{64, 64, 4.0f, 5.5f},      {16, 32, 0, 0},        {16, 16, 0, 0},        {32, 16, 0.35f, 2.5f}, {64, 64, 4.4f, 1.3f},
                                      {64, 128, 5.0f, 2.0f}, {128, 128, 5.0f, 3.1f}, {256, 128, 6.5f, 4.6f}, {256, 256, 8.1f, 8.3f}};
 constexpr float kStreamUs = 3.0f;   // start and end of the streams' rounds, which overlap
+constexpr float kStreamRoundUs = 2.0f;   // a further round at least, however short K is (64 x 33 x 1048576: 996 us, 512 rounds)
+// A row of aligned copies at least, whatever its length.  The copies themselves take 0.22 ns a row (1048640 rows of 33 bytes
+// 240 us); less is counted because the general kernel's rounds are counted a third too high where there are many of them.
+constexpr float kCopyRowUs = 0.13e-3f;
 constexpr float kLaunchUs = 4.5f, kBytesPerUs = 4.5e6f;   // a launch more, for partial sums or aligned copies; their bytes
 
 struct Int8Choice {
@@ -675,6 +681,7 @@ constexpr int64_t kStreamRows = 32 * 65535;   // a grid's second dimension
 constexpr int64_t kMostTiles = (1 << 22) - 1;   // of a launch, the parts of K counted: 512 threads each are fewer than 2^32
 thread_local Int8Choice g_forced = {-1, 1};
 
+int64_t padded_k(int64_t k) { return (k + 255) / 256 * 256; }   // of aligned copies: whole rounds of every form
 int64_t tiles_of(int form, int64_t m, int64_t n) {
   return ((m + kCosts[form].rows - 1) / kCosts[form].rows) * ((n + kCosts[form].cols - 1) / kCosts[form].cols);
 }
@@ -696,19 +703,22 @@ Int8Choice choose_form(int64_t m, int64_t n, int64_t k, bool aligned) {
   if (!aligned) {   // the tiles would have to wait for copies
     best = {kGeneral, 1};
     least = (float)((tiles_of(kGeneral, m, n) + 255) / 256) * (kCosts[kGeneral].round + kCosts[kGeneral].per_k * (float)k / 1024);
-    copies = kLaunchUs + 2.0f * (float)(m + n) * (float)k / kBytesPerUs;
+    const float rows = (float)(m + n);
+    copies = kLaunchUs + std::max(rows * (float)(k + padded_k(k)) / kBytesPerUs, rows * kCopyRowUs);
     // The stream in blocks of 32 rows reads the weight once a block, but has sixteen wavefronts on 16 channels: 77 x 1003 x 1537
     // 7.9 us, the general kernel 9.8; 200 x 2047 x 513 8.3 and 12.1; 200 x 1003 x 1537 12.9 and 10.1.
-    const float streams = kStreamUs + (float)((tiles_of(kStreamTwo, m, n) + 255) / 256) *
-                                          (kCosts[kStreamTwo].round + kCosts[kStreamTwo].per_k * (float)k / 1024);
+    const float rounds = (float)((tiles_of(kStreamTwo, m, n) + 255) / 256);
+    const float streams = kStreamUs + std::max(rounds * (kCosts[kStreamTwo].round + kCosts[kStreamTwo].per_k * (float)k / 1024),
+                                               (rounds - 1) * kStreamRoundUs);
     if (m <= kStreamRows && streams < least) least = streams, best = {kStreamTwo, 1};
   }
+  const float tile_k = (float)(aligned ? k : padded_k(k));
   for (int form = kTile64; form <= kTile256; ++form)
     for (int splits = 1; splits <= 8 && may_split(splits, k); splits *= 2) {
       const int64_t tiles = tiles_of(form, m, n);
       if (splits > 1 && tiles * splits > 1024) break;
       const float rounds = (float)((tiles * splits + 255) / 256);
-      float us = rounds * (kCosts[form].round + kCosts[form].per_k * (float)k / splits / 1024);
+      float us = rounds * (kCosts[form].round + kCosts[form].per_k * tile_k / splits / 1024);
       if (splits > 1) us += kLaunchUs + (float)tiles * splits * kCosts[form].rows * kCosts[form].cols * 8 / kBytesPerUs;
       us += copies;
       if (us < least) least = us, best = {form, splits};
@@ -722,7 +732,6 @@ size_t partial_bytes(const Int8Choice& s, int64_t m, int64_t n) {
   if (!is_tile(s.form) || s.splits <= 1) return 0;
   return (size_t)tiles_of(s.form, m, n) * s.splits * kCosts[s.form].rows * kCosts[s.form].cols * 4;
 }
-int64_t padded_k(int64_t k) { return (k + 255) / 256 * 256; }   // whole rounds of every form
 size_t padded_bytes(const Int8Choice& s, int64_t m, int64_t n, int64_t k, bool aligned) {
   return is_tile(s.form) && !aligned ? (size_t)(m + n) * padded_k(k) : 0;
 }

@@ -1,5 +1,5 @@
-"""CPU: what the layer library launches, counted by a stand-in for the runtime's launch functions that the library finds first:
-no kernel runs.  A call that is refused launches nothing, whatever it is refused for."""
+"""CPU: which kernels the layer library takes and launches.  Launches are counted by a stand-in for the runtime's launch
+functions that the library finds first: no kernel runs."""
 import os
 import shutil
 import subprocess
@@ -71,3 +71,17 @@ def test_a_refused_product_launches_nothing(tmp_path):
     subprocess.run([gcc, "-shared", "-fPIC", "-o", library, str(tmp_path / "stand_in.c")], check=True, timeout=60)
     run = subprocess.run([sys.executable, "-c", CALLS, ROOT, library], capture_output=True, text=True, timeout=120)
     assert run.returncode == 0 and run.stdout.strip() == "done", run.stderr[-2000:]
+
+
+def test_the_rule_counts_what_aligned_copies_move():
+    """Rows that are laid down for the tiles are written to whole rounds of K, 256 bytes at least, and multiplied over them: for a
+    short K that is many times the operands.  What was measured to be fastest there, and near there."""
+    from sonar_amd import _lib
+    lib = _lib.load_layer()
+    for m, n, k in ((64, 1 << 20, 33), (64, 200000, 33), (48, 400000, 200), (64, 200000, 513), (100, 6144, 300)):
+        assert lib.sonar_debug_int8_choice(m, n, k, 0, None) == 0, (m, n, k)   # the general kernel, on the rows as they lie
+        assert lib.sonar_scaled_mm_int8_scratch_bytes(m, n, k, 0) == 0
+    for m, n, k in ((83, 802, 29), (113, 270, 164)):
+        assert lib.sonar_debug_int8_choice(m, n, k, 0, None) == 3, (m, n, k)   # the stream in blocks of 32 rows
+    for m, n, k in ((200, 100000, 100), (1000, 50000, 60), (1 << 18, 512, 40), (300, 4096, 4095)):
+        assert lib.sonar_debug_int8_choice(m, n, k, 0, None) >= 4, (m, n, k)   # tiles of copies
