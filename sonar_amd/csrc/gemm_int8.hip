@@ -54,7 +54,7 @@ __device__ __forceinline__ intx4_t load_16(const int8_t* row, int k0, int k) {
 }
 
 // A row that starts at any byte (ODD) is read by whole words: 16 bytes and the word behind them, and shifted by what is over.
-// Vectors at odd bytes take the hardware three times as long: 1 x 4095 x 28672 63 us, 25.8 with 4096.  No word is read that
+// Vectors at odd bytes take the hardware three times as long: 1 x 4095 x 28672 63 us, by words 37.5, 4096 columns 25.8.  No word is read that
 // holds none of the bytes asked for.
 template <bool ODD>
 struct Row {
@@ -346,10 +346,10 @@ __device__ __forceinline__ void tile_at(int tile, const TilePlan& t, int& tm, in
 // stands at c ^ (i / 2 & 7) (rows of 64: c ^ (i / 4 & 3)), so that lanes that read together find different banks: 548 bytes/ns
 // a compute unit, where c ^ (i & 7) reaches half and no turn a quarter of that.  Stages of 128 bytes because a copy of whole
 // 128-byte lines runs at 55 bytes a cycle and compute unit, one of half lines at 41 (2048 x 14336 x 4096: 133 -> 104 us); the
-// 256 x 256 tile has no room for three of them and takes four of 64 (859 us for 8192 x 4096 x 28672, 888 with two of 128).
+// 256 x 256 tile has no room for three of them and takes four of 64 (8192 x 4096 x 28672: two of 128 take 3 % longer).
 // Operands are read one step (32 of K) ahead of their matrix instructions.
 // Eight wavefronts for the tiles of 128 rows and up: while one waits at a barrier or issues its copies, the other of its
-// SIMD multiplies (four wavefronts with 128 x 128 each: 944 us instead of 859).
+// SIMD multiplies (four wavefronts with 128 x 128 each take 10 % longer).
 // KG: that many sets of wavefronts take stages in turn and join their sums through LDS, for tiles too small to keep a compute
 // unit busy otherwise (100 x 4096 x 4096: 9.7 -> 9.2 us).
 // What K is over whole rounds of stages is one more stage, whose pieces behind the end of a row are copied from its last
@@ -565,7 +565,7 @@ void int8_tile_kernel(const Int8Params p, const TilePlan t, int* __restrict__ pa
     }
   } else {
     // 32 rows at a time turn in LDS, so that they leave as whole lines, 64 NT bytes a row (in pieces of 32 bytes from where
-    // they are: 8192 x 4096 x 28672 926 us instead of 901)
+    // they are 8192 x 4096 x 28672 takes 3 % longer)
     constexpr int kPitch = 64 * NT + 16, kLanes = 4 * NT, kRowsOut = 64 / kLanes;
     typedef T eight_t __attribute__((ext_vector_type(8)));
     typedef T four_t __attribute__((ext_vector_type(4)));

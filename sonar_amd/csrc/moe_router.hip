@@ -14,8 +14,8 @@
 // the latency of their chains where tokens are few.  16384 x 256, sigmoid, bias, 4 of 8 groups: 132 us with choices and 64-bit
 // maxima in LDS; 28.6 by lane moves; 20.9 with no loop over tokens around it all (which kept constants in 80 registers), the
 // scoring's branch outside the experts' loop (their chains side by side, one set of constants), which of a lane's experts it is
-// as lane masks, and the groups from registers; 19.6 with the words of the double itself (float32 and what it leaves before).  (Choices in float32 first, and in 64 bits only for the tokens where two come
-// near each other: no gain.)
+// as lane masks, and the groups from registers; 19.6 with the words of the double itself (before, its float32 rounding and what
+// that leaves).  (Choices in float32 first, and in 64 bits only for the tokens where two come near each other: no gain.)
 #include "common.hpp"
 #include "lane_reduce.hpp"
 #include "sonar_layer.h"
@@ -88,12 +88,13 @@ __device__ __forceinline__ float logit_at(const RouterParams& p, long at) {
   return f == f ? f : -__builtin_inff();
 }
 
-// e^-d for d >= 0 (also infinite): 2^n e^r with |r| <= ln(2) / 2, and the series of e^r to r^13, whose rest is below 2^-57.
+// e^-d for d >= 0 (also infinite): 2^n e^r with |r| <= ln(2) / 2, and the series of e^r to r^13, whose rest is below 2^-57.  The
+// reduction is Cody and Waite's, with ln 2 in two parts, the first of so few bits that n times it is exact: those of fdlibm.
 // The relative error grows with d, by 2^-53 for each of its units; that of a score by less, since e^-d falls faster.
 __device__ __forceinline__ double exp_minus(double d) {
   const double t = -fmin(d, 800.0);
   const double n = __builtin_rint(t * 1.4426950408889634);
-  const double r = __builtin_fma(-n, 1.9082149292705877e-10, __builtin_fma(-n, 0.6931471803691238, t));   // ln 2 in two parts
+  const double r = __builtin_fma(-n, 1.9082149292705877e-10, __builtin_fma(-n, 0.6931471803691238, t));
   double e = 1.0 / 6227020800.0;
   e = __builtin_fma(e, r, 1.0 / 479001600.0);
   e = __builtin_fma(e, r, 1.0 / 39916800.0);
@@ -346,8 +347,8 @@ void launch(const RouterParams& p, hipStream_t st) {
 }
 
 // Few tokens: a wavefront each, for its latency.  From 4096 on, where every SIMD has some, several share one (8192 x 128, top 8:
-// 5.5 us, 9.3 with a wavefront each; 2048 x 256 4.9 and, shared, 6.6).  With a bias and more than 128 experts two instead of
-// four (4096 x 256, sigmoid, 4 of 8 groups: 9.2 us, 11.5 with four; without a bias, 16384 x 256: 12.0 with two, 11.3 with four).
+// 5.3 us, 9.3 with a wavefront each; 2048 x 256 4.6 and, shared, 6.6).  With a bias and more than 128 experts two instead of
+// four (4096 x 256, sigmoid, 4 of 8 groups: 8.8 us, 10.6 with four; without a bias, 16384 x 256: 12.0 with two, 11.3 with four).
 template <bool BIASED>
 void launch_form(const RouterParams& p, hipStream_t st) {
   const bool many = p.tokens >= 4096;

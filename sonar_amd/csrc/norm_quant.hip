@@ -1,8 +1,8 @@
 // Root-mean-square norm with the residual's addition before it and 8-bit codes with one scale a token behind it:
 //   z = T(x + residual);  r = 1 / sqrt(mean(z^2) + epsilon);  y = (z * r) * weight;  codes of y against its largest magnitude
 // The sum of squares and r are held in 64 bits and r is rounded once, y and the codes' arithmetic are float32, so that the
-// result does not depend on the order of the sum (but for one r in 2^24): a code is a rounding of y, and one last bit of r
-// would turn some.
+// result hardly depends on the order of the sum, which the forms below take differently: one r in about 2^24 comes out a last
+// bit apart, and that bit may turn a code of its row.
 //
 // One pass over memory: a row is read once, z stays in registers (16 bits a number where the type has 16), y is formed
 // twice, for the maximum and for the codes.  Bound by the bytes.
@@ -99,9 +99,9 @@ struct Eight {
 // workgroup, sums and maxima by lane moves, no barrier.  THREADS = 1024: rows of any length; turns beyond KEPT are read
 // again (as z).  A workgroup that goes on to a further row has its numbers loaded before it works on its own; the weight
 // stays in registers.
-// 16384 x 4096 bf16 to int8 with a residual (470 MB): 80 us, 5.8 TB/s; 92 with eight workgroups a compute unit that walk
-// the rows instead of a workgroup a row (fresh ones overlap their loads with the others' stores), 97 with a wavefront a row,
-// 220 element by element with three passes.  Registers decide: row bases in scalar registers with 32-bit offsets of the
+// 16384 x 4096 bf16 to int8 with a residual (470 MB): 80 us, 5.8 TB/s (float32 151 us, 5.8 TB/s); 92 with
+// eight workgroups a compute unit that walk the rows instead of a workgroup a row (fresh ones overlap their loads with the
+// others' stores), 97 with a wavefront a row, 220 element by element with three passes.  Registers decide: row bases in scalar registers with 32-bit offsets of the
 // columns, and no code of the repeated reads where no call needs them, took 107 registers to 68 and 16384 x 2880 without a
 // residual from 47 to 34 us.
 template <typename T, bool FP8, int THREADS, int KEPT>
@@ -226,7 +226,8 @@ __global__ __launch_bounds__(THREADS > kThreads ? THREADS : kThreads) void rms_n
   }
 }
 
-// Any column count, stride and alignment: a workgroup a row, element by element; z is read again in each pass.
+// Any column count, stride and alignment: a workgroup a row, element by element; z is read again in each pass (4096 x 4099 bf16
+// with a residual 55 us, 2.1 TB/s of the bytes it needs; 4096 columns 24).
 template <typename T, bool FP8>
 __global__ __launch_bounds__(kThreads) void rms_norm_quant_any_kernel(const NormParams p) {
 #pragma clang fp contract(off)
