@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABIs in include/sonar_marlin.h and include/sonar_layer.h.
+"""ctypes binding of the C ABIs in include/sonar_marlin.h, include/sonar_layer.h and
+include/sonar_attention.h.
 
 Loading fails loudly when the HIP library has not been built: there is no
 fallback path."""
@@ -6,10 +7,11 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_marlin.so")
 _LAYER_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_layer.so")
+_ATTENTION_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_attention.so")
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -133,9 +135,31 @@ LAYER_PROTOTYPES = {
                                    c_int, c_int64, c_int64, c_double, c_void_p]),
 }
 SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
+CACHE_FP8 = 3
+
+
+class KvCache(ctypes.Structure):
+    """sonar_kv_cache"""
+    _fields_ = [("data", c_void_p), ("page_stride", c_int64), ("slot_stride", c_int64), ("head_stride", c_int64),
+                ("scale", c_void_p), ("scale_len", c_int64)]
+
+
+# the same for include/sonar_attention.h
+ATTENTION_PROTOTYPES = {
+    "sonar_attention_last_error": (c_char_p, []),
+    "sonar_qk_norm_rope": (c_int, [c_void_p, c_int64, c_int64] * 3 + [c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p,
+                                   c_void_p, c_double, c_void_p, c_void_p, POINTER(KvCache), POINTER(KvCache), c_int, c_void_p, c_int,
+                                   c_int64, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p]),
+    "sonar_paged_attention_scratch_bytes": (c_size_t, [c_int64] * 7),
+    "sonar_paged_attention": (c_int, [c_void_p, c_int64, c_int64, POINTER(KvCache), POINTER(KvCache), c_int, c_int64, c_int64, c_void_p,
+                                      c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_double, c_double,
+                                      c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_int, c_int64, c_int64, c_int64,
+                                      c_int64, c_int64, c_int64, c_void_p]),
+}
 
 _lib = None
 _layer = None
+_attention = None
 
 
 class SonarMarlinError(RuntimeError):
@@ -150,6 +174,10 @@ def lib_path() -> str:
 
 def layer_path() -> str:
     return _LAYER_PATH
+
+
+def attention_path() -> str:
+    return _ATTENTION_PATH
 
 
 def _open(path: str, prototypes) -> ctypes.CDLL:
@@ -179,6 +207,13 @@ def load_layer() -> ctypes.CDLL:
     return _layer
 
 
+def load_attention() -> ctypes.CDLL:
+    global _attention
+    if _attention is None:
+        _attention = _open(_ATTENTION_PATH, ATTENTION_PROTOTYPES)
+    return _attention
+
+
 def _raise(rc: int, msg: bytes) -> None:
     text = msg.decode("utf-8", "replace")
     if rc == E_UNSUPPORTED:
@@ -194,3 +229,8 @@ def check(rc: int) -> None:
 def check_layer(rc: int) -> None:
     if rc != OK:
         _raise(rc, load_layer().sonar_layer_last_error())
+
+
+def check_attention(rc: int) -> None:
+    if rc != OK:
+        _raise(rc, load_attention().sonar_attention_last_error())

@@ -15,6 +15,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libsonar_marlin.so")
 OPS_PATH = os.path.join(LIB_DIR, "libsonar_marlin_torch.so")
 LAYER_PATH = os.path.join(LIB_DIR, "libsonar_layer.so")
 LAYER_OPS_PATH = os.path.join(LIB_DIR, "libsonar_layer_torch.so")
+ATTENTION_PATH = os.path.join(LIB_DIR, "libsonar_attention.so")
+ATTENTION_OPS_PATH = os.path.join(LIB_DIR, "libsonar_attention_torch.so")
 BENCH_PATH = os.path.join(LIB_DIR, "libsonar_bench.so")   # bench.py's yardstick kernels, not part of the product
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -22,6 +24,8 @@ HIP_SOURCES = ["repack.hip", "gemm_stream.hip", "gemm_tile.hip", "gemm_moe.hip",
                "gemm_mid.hip", "gemm_a8_block.hip"]
 # the operators around the GEMMs (include/sonar_layer.h): a library of their own
 LAYER_SOURCES = ["norm_quant.hip", "gemm_int8.hip", "moe_router.hip"]
+# the operators between the qkv and the output projection (include/sonar_attention.h): another one
+ATTENTION_SOURCES = ["qk_norm_rope.hip", "paged_attention.hip"]
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -85,6 +89,10 @@ def build_layer_library(verbose: bool = False, only=None) -> str:
     return build_hip_library(verbose, only, tuple(LAYER_SOURCES), LAYER_PATH)
 
 
+def build_attention_library(verbose: bool = False, only=None) -> str:
+    return build_hip_library(verbose, only, tuple(ATTENTION_SOURCES), ATTENTION_PATH)
+
+
 def build_bench_library(verbose: bool = False) -> str:
     """Compiles the yardstick kernels bench.py times beside the GEMMs (an empty kernel, a
     kernel that only streams bytes) into a library of their own."""
@@ -122,9 +130,10 @@ def build_torch_ops(verbose: bool = False, source: str = "torch_bindings.cpp", p
 
 
 def build_all(verbose: bool = False):
-    paths = [build_hip_library(verbose), build_layer_library(verbose)]
+    paths = [build_hip_library(verbose), build_layer_library(verbose), build_attention_library(verbose)]
     paths.append(build_torch_ops(verbose))
     paths.append(build_torch_ops(verbose, "layer_bindings.cpp", LAYER_OPS_PATH, "sonar_layer"))
+    paths.append(build_torch_ops(verbose, "attention_bindings.cpp", ATTENTION_OPS_PATH, "sonar_attention"))
     paths.append(build_bench_library(verbose))
     return paths
 
@@ -133,12 +142,15 @@ if __name__ == "__main__":
     if len(sys.argv) > 1:   # python -m sonar_amd.build gemm_stream.hip ...: recompile these, relink
         marlin = [f for f in sys.argv[1:] if f in HIP_SOURCES]
         layer = [f for f in sys.argv[1:] if f in LAYER_SOURCES]
-        if len(marlin) + len(layer) < len(sys.argv) - 1:
-            sys.exit("sources: %s" % " ".join(HIP_SOURCES + LAYER_SOURCES))
+        attention = [f for f in sys.argv[1:] if f in ATTENTION_SOURCES]
+        if len(marlin) + len(layer) + len(attention) < len(sys.argv) - 1:
+            sys.exit("sources: %s" % " ".join(HIP_SOURCES + LAYER_SOURCES + ATTENTION_SOURCES))
         if marlin:
             print("built", build_hip_library(verbose=True, only=marlin))
         if layer:
             print("built", build_layer_library(verbose=True, only=layer))
+        if attention:
+            print("built", build_attention_library(verbose=True, only=attention))
     else:
         for p in build_all(verbose=True):
             print("built", p)

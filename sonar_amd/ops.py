@@ -2,8 +2,8 @@
 aphrodite/_custom_ops.py (:1363-1461 repack, :1472-1543 marlin_gemm,
 :3046-3141 moe_wna16_marlin_gemm).  Importing this module loads the HIP library
 and the torch op registration layer; it raises if either is missing.  The
-operators around the GEMMs are two libraries more: without those the module
-serves the rest, and a call of theirs raises."""
+operators around the GEMMs are two libraries more, those of the attention another
+two: without those the module serves the rest, and a call of theirs raises."""
 from __future__ import annotations
 
 import os
@@ -15,6 +15,7 @@ from .scalar_type import ScalarType
 
 _OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_marlin_torch.so")
 _LAYER_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_layer_torch.so")
+_ATTENTION_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsonar_attention_torch.so")
 
 
 def _load_ops() -> None:
@@ -37,8 +38,20 @@ def _load_layer_ops() -> list[str]:
     return missing
 
 
+def _load_attention_ops() -> list[str]:
+    """The same for the operators between the qkv and the output projection."""
+    if hasattr(torch.ops.sonar_amd, "paged_attention"):
+        return []
+    missing = [path for path in (_lib.attention_path(), _ATTENTION_OPS_PATH) if not os.path.exists(path)]
+    if not missing:
+        _lib.load_attention()
+        torch.ops.load_library(_ATTENTION_OPS_PATH)
+    return missing
+
+
 _load_ops()
 _LAYER_MISSING = _load_layer_ops()
+_ATTENTION_MISSING = _load_attention_ops()
 
 
 def _register_layer_fakes(reg, quant_fake) -> None:
@@ -56,6 +69,28 @@ def _register_layer_fakes(reg, quant_fake) -> None:
         shape = (logits.shape[0], topk)
         return (torch.empty(shape, dtype=torch.float32, device=logits.device),
                 torch.empty(shape, dtype=torch.int32, device=logits.device))
+
+
+def _register_attention_fakes(reg) -> None:
+    @reg("sonar_amd::qk_norm_rope")
+    def _(query, key, positions, cos_sin_cache, q_weight, k_weight, epsilon, is_neox):
+        return (torch.empty(query.shape, dtype=query.dtype, device=query.device),
+                torch.empty(key.shape, dtype=query.dtype, device=query.device))
+
+    @reg("sonar_amd::qk_norm_rope_append")
+    def _(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin_cache, q_weight, k_weight, epsilon, is_neox,
+          k_scale, v_scale):
+        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+
+    @reg("sonar_amd::paged_attention")
+    def _(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, scale, causal, window, softcap, alibi_slopes,
+          tree_mask, k_scale, v_scale, max_seq_len):
+        return torch.empty(query.shape, dtype=query.dtype, device=query.device)
+
+    @reg("sonar_amd::paged_attention_out")
+    def _(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, scale, causal, window, softcap, alibi_slopes,
+          tree_mask, k_scale, v_scale, max_seq_len, out):
+        return None
 
 
 def _register_fakes() -> None:
@@ -94,6 +129,8 @@ def _register_fakes() -> None:
     reg("sonar_amd::per_token_quant_fp8")(quant_fake(torch.float8_e4m3fn))
     if not _LAYER_MISSING:
         _register_layer_fakes(reg, quant_fake)
+    if not _ATTENTION_MISSING:
+        _register_attention_fakes(reg)
 
     @reg("sonar_amd::gptq_marlin_moe_repack")
     def _(b_q_weight, perm, size_k, size_n):
@@ -227,13 +264,13 @@ def per_token_quant_fp8(x: torch.Tensor):
     return torch.ops.sonar_amd.per_token_quant_fp8(x)
 
 
-def _layer_op(name: str):
+def _layer_op(name: str, missing: list[str] = _LAYER_MISSING):
     """An op of the layer library itself, not the name that looks for an overload at every call."""
-    if not _LAYER_MISSING:
+    if not missing:
         return getattr(torch.ops.sonar_amd, name).default
 
     def absent(*args):
-        raise ImportError(f"{' and '.join(_LAYER_MISSING)} missing: build with `python -m sonar_amd.build`; there is no "
+        raise ImportError(f"{' and '.join(missing)} missing: build with `python -m sonar_amd.build`; there is no "
                           f"other implementation of {name}")
     return absent
 
@@ -241,6 +278,10 @@ def _layer_op(name: str):
 _rms_norm_per_token_quant = _layer_op("rms_norm_per_token_quant")
 _scaled_mm_int8 = _layer_op("scaled_mm_int8")
 _topk_routing = _layer_op("topk_routing")
+_qk_norm_rope = _layer_op("qk_norm_rope", _ATTENTION_MISSING)
+_qk_norm_rope_append = _layer_op("qk_norm_rope_append", _ATTENTION_MISSING)
+_paged_attention = _layer_op("paged_attention", _ATTENTION_MISSING)
+_paged_attention_out = _layer_op("paged_attention_out", _ATTENTION_MISSING)
 
 
 def rms_norm_per_token_quant(x: torch.Tensor, weight: torch.Tensor, epsilon: float,
@@ -288,6 +329,75 @@ def topk_routing(gating_output: torch.Tensor, topk: int, scoring_func: str = "so
     At most 1024 experts, 64 groups, 64 choices."""
     return _topk_routing(gating_output, topk, scoring_func, renormalize, bias, num_expert_group, topk_group,
                          routed_scaling_factor)
+
+
+def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor | None = None,
+                 cos_sin_cache: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                 epsilon: float = 1e-6, is_neox: bool = True):
+    """Norm of each query and key head and rotation by the token's position, in one launch (the reference's rotary_embedding and
+    fused_qk_norm_rope): (query, key), new tensors of the inputs' shapes.
+
+      y = x / sqrt(mean(x^2) + epsilon) * weight over head_dim, where a weight is given;
+      the first rotary_dim numbers in pairs (a, b) -> (a cos - b sin, b cos + a sin), where a table is given
+
+    all in float32, rounded once.  query: (tokens, heads, head_dim), key: (tokens, kv_heads, head_dim), float16, bfloat16 or float32,
+    of any strides: views of the qkv projection's output are read as they lie.  positions: (tokens,), int64 or int32.
+    cos_sin_cache: float32 (positions, rotary_dim), a position's cosines, then its sines (`rotary.rotary_cos_sin` makes one; a scaling
+    for long contexts is in it).  is_neox: pairs are (i, i + rotary_dim / 2), else neighbours.  Weights: (head_dim,) of query's type.
+    A position outside the table turns the token's rotated numbers into NaN.  head_dim at most 1024, epsilon at least 2^-126."""
+    return _qk_norm_rope(query, key, positions, cos_sin_cache, q_weight, k_weight, epsilon, is_neox)
+
+
+def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                        slot_mapping: torch.Tensor, positions: torch.Tensor | None = None, cos_sin_cache: torch.Tensor | None = None,
+                        q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, epsilon: float = 1e-6,
+                        is_neox: bool = True, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """`qk_norm_rope` whose keys go, with the values, to the pages of a cache (the reference's reshape_and_cache_flash on the way):
+    returns the queries.
+
+    key_cache, value_cache: (pages, page_size, kv_heads, head_dim) of any strides but the last (a layout with the heads before the
+    slots is a transposed view), of query's type or float8_e4m3fn.  An 8-bit cache holds codes that stand for code * scale: the nearest
+    to y / scale, at most 448; k_scale and v_scale: float32, one number or one a kv head.  slot_mapping: (tokens,), int64 or int32:
+    token t goes to slot s % page_size of page s // page_size, s = slot_mapping[t]; nowhere where s is negative or past the last page.
+    Which of two tokens with the same slot stays is not defined.  Without a table and weights this is the plain append."""
+    return _qk_norm_rope_append(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin_cache, q_weight, k_weight,
+                                epsilon, is_neox, k_scale, v_scale)
+
+
+def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, query_start_loc: torch.Tensor, scale: float | None = None, causal: bool = True,
+                    window: int = 0, softcap: float = 0.0, alibi_slopes: torch.Tensor | None = None,
+                    tree_mask: torch.Tensor | None = None, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                    max_seq_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a ragged batch over a paged cache, which holds the batch's own keys and values already (`qk_norm_rope_append`):
+    prompts, pieces of prompts, single tokens and trees of drafted tokens, in any mixture.
+
+    query: (tokens, heads, head_dim), float16 or bfloat16; sequence i's queries are the tokens query_start_loc[i] up to
+    query_start_loc[i + 1] (int32, (sequences + 1,), from 0 on), the last ones of its seq_lens[i] tokens (int32, (sequences,)).
+    Caches as `qk_norm_rope_append` fills them, 16-byte aligned; block_table: int32 (sequences, pages), key p of sequence i is in page
+    block_table[i, p // page_size].  heads is a multiple of the cache's kv heads, neighbours share one.  scale: head_dim ** -0.5.
+
+      s = scale * (q . k);  softcap > 0: softcap * tanh(s / softcap);  alibi_slopes (float32, (heads,)): s - slope * |distance|
+      out = softmax(s over the keys that the query sees) v
+
+    causal: a query sees its own and earlier keys, with window > 0 the last `window` of them; not causal: every key of its sequence.
+    tree_mask (int64, (tokens, words)): a query sees the keys before its sequence's queries, and of those the ones whose bits are set:
+    bit c % 64 of word c // 64 is query c of the sequence (a draft's own bit among them); it takes the place of `causal` and goes with
+    neither window nor slopes.  A query that sees no key gives zeros, as do tokens behind the last sequence; with `out`, those are left as
+    they are.  NaNs and infinities in what a query does not see do not reach it.  Pages that no query sees are not read; a
+    page number outside the cache among the others makes the results NaN.
+
+    max_seq_len: the longest sequence, if the caller knows: how far the keys are split over workgroups is chosen for it, and for
+    all of the block table without it; results are right, if not the same bits, for any number.
+    head_dim a multiple of 16, at most 256."""
+    if scale is None:
+        scale = query.shape[-1] ** -0.5
+    if out is None:
+        return _paged_attention(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, scale, causal, window, softcap,
+                                alibi_slopes, tree_mask, k_scale, v_scale, max_seq_len)
+    _paged_attention_out(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, scale, causal, window, softcap,
+                         alibi_slopes, tree_mask, k_scale, v_scale, max_seq_len, out)
+    return out
 
 
 def marlin_gemm(a: torch.Tensor, c: torch.Tensor | None, b_q_weight: torch.Tensor,

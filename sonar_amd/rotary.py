@@ -1,0 +1,49 @@
+"""Tables of cosines and sines that `ops.qk_norm_rope` and `ops.qk_norm_rope_append` read: made once, at load."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+
+def rotary_rates(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> torch.Tensor:
+    """The angle of each pair per position, float64 (rotary_dim / 2,): base ** (-2 i / rotary_dim), and with `scaling`, as a model's
+    configuration holds it ("rope_type" and its numbers):
+
+      linear   every rate divided by `factor`
+      llama3   by wavelength: those longer than original_max_position_embeddings / low_freq_factor are divided by `factor`, those
+               shorter than it / high_freq_factor stay, a straight line of the inverse wavelength between
+      yarn     by turns within original_max_position_embeddings: pairs of `beta_fast` (32) turns or more stay, of `beta_slow` (1) or
+               fewer are divided by `factor`, a straight line of the pair's number between"""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim = {rotary_dim} must be even and positive")
+    rates = float(base) ** -(torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    if scaling is None:
+        return rates
+    kind, factor = scaling["rope_type"], float(scaling["factor"])
+    if kind == "linear":
+        return rates / factor
+    original = scaling["original_max_position_embeddings"]
+    if kind == "llama3":
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        stay = ((rates * original / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+    elif kind == "yarn":
+        # the pair that turns n times within the original context
+        pair = lambda n: rotary_dim * math.log(original / (2 * math.pi * n)) / (2 * math.log(base))  # noqa: E731
+        first = max(math.floor(pair(scaling.get("beta_fast", 32))), 0)
+        last = min(math.ceil(pair(scaling.get("beta_slow", 1))), rotary_dim - 1)
+        stay = 1 - ((torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0, 1)
+    else:
+        raise ValueError(f"rope_type = {kind!r} is not linear, llama3 or yarn")
+    return rates * stay + rates / factor * (1 - stay)
+
+
+def rotary_cos_sin(rotary_dim: int, max_position: int, base: float = 10000.0, scaling: dict | None = None,
+                   device: torch.device | str | None = None) -> torch.Tensor:
+    """float32 (max_position, rotary_dim): a position's cosines, then its sines.  The angles are formed in 64 bits, as those of far
+    positions need; for yarn both are multiplied by `attention_factor`, 0.1 ln(factor) + 1 if the configuration does not say."""
+    angles = torch.arange(max_position, dtype=torch.float64)[:, None] * rotary_rates(rotary_dim, base, scaling)
+    size = 1.0
+    if scaling is not None and scaling["rope_type"] == "yarn":
+        size = scaling.get("attention_factor") or (0.1 * math.log(scaling["factor"]) + 1 if scaling["factor"] > 1 else 1.0)
+    return (torch.cat([angles.cos(), angles.sin()], dim=1) * size).float().to(device)
