@@ -72,13 +72,13 @@ int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  * table_pages * page_size.  Tokens from starts[seqs] on get zeros where clear_rest, else are left as they are.
  *   q, out      dtype (SONAR_DTYPE_F16 / _BF16) (token, head, d) with strides; q 16-byte aligned, its strides multiples of 8; out 8-byte
  *               aligned, its strides multiples of 4; out does not overlap the inputs
- *   caches      of dtype or SONAR_CACHE_FP8; 16-byte aligned, strides multiples of 16 bytes; page_size slots a page; below 2^40 bytes
+ *   caches      of dtype or SONAR_CACHE_FP8; 16-byte aligned, strides multiples of 16 bytes; page_size slots a page; 64 GiB at most
  *   block_table int32[seqs][table_stride], table_pages of a row in use;  seq_lens int32[seqs];  starts int32[seqs + 1], rising, from 0
  *   slopes      float[heads] or NULL;  tree_mask int64[tokens][tree_words] or NULL
  *   max_seq_len what the split of the keys is chosen for; longer sequences are right too
  *   scratch     device memory, 16-byte aligned, of sonar_paged_attention_scratch_bytes(...) bytes (may be 0); calls that overlap in
  *               time need scratches of their own
- * head_dim a multiple of 16, at most 256; scale > 0; tokens * heads and table_pages * page_size below 2^31. */
+ * head_dim a multiple of 16, at most 256; scale > 0; tokens * heads below 2^31, table_pages * page_size below 2^31 - 1024. */
 size_t sonar_paged_attention_scratch_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                            int64_t max_seq_len, int64_t window);
 int sonar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const sonar_kv_cache* key_cache,

@@ -235,7 +235,7 @@ void paged_attention_out(const Tensor& query, const Tensor& key_cache, const Ten
   TORCH_CHECK(out.device() == query.device() && out.scalar_type() == query.scalar_type() && out.sizes() == query.sizes() &&
                   (out.size(2) <= 1 || out.stride(2) == 1), "out must have query's shape, type and device, the numbers of a head behind each other");
   at::assert_no_internal_overlap(out);
-  at::assert_no_overlap(out, query);
+  for (const Tensor* t : {&query, &key_cache, &value_cache}) at::assert_no_overlap(out, *t);
   attend(query, key_cache, value_cache, block_table, seq_lens, query_start_loc, scale, causal, window, softcap, alibi_slopes, tree_mask, k_scale,
          v_scale, max_seq_len, out, false);
 }

@@ -64,9 +64,9 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
       if (tile * kTile >= full_low && tile * kTile + kTile <= full_high) continue;
       for (int key = tile * kTile; key < min(tile * kTile + kTile, r.len); ++key) {
         const int at = page_of(p, key);
-        const long page = p.table[(long)r.seq * p.table_stride + at];
-        if (page < 0 || page >= p.pages) continue;
-        const char* from = p.v.data + page * p.v.page + (key - at * p.page_size) * p.v.slot + kv_head * p.v.head;
+        bool bad = false;
+        const uint32_t place = place_of(p, p.v, key, at, p.table[(long)r.seq * p.table_stride + at], bad);
+        const char* from = row_at(p.v.data + kv_head * p.v.head, place);
         float v;
         if (FP8) v = __builtin_amdgcn_cvt_f32_fp8((int)(uint8_t)from[d], 0);
         else v = (float)((const T*)from)[d];
@@ -89,34 +89,51 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
 }
 
 // ---------------------------------------------------------------- many rows
-// A workgroup takes 128 rows of a kv head, 32 a wavefront, and walks the keys in tiles of 64 that its wavefronts share through
-// LDS, two tiles there: while one is worked on, the next one's numbers are on their way in registers.
-constexpr int kWaves = 4, kRows = 32 * kWaves;
+// A workgroup takes 32 rows of a kv head for each of its WAVES wavefronts, and walks the keys in tiles of 64 that they share through
+// LDS, two tiles there: while one is worked on, the next one is on its way.  Bound by the matrix pipes and the vector units together:
+// 8192 tokens of 32 heads of 128 (8 kv heads) in bf16 take 567 us, 970 TFLOP/s, with 43 % of the pipes' cycles; the same without its
+// copies to LDS 489, without its reads of LDS too 442.  Each step of the way there, at that size: copies through registers and
+// products, weights, products one after the other 769; addresses found once a key 656; scores a half tile ahead 612; instructions
+// in turn 586 (heads of 256: 466 to 365 for 4096 tokens); copies straight into LDS 574.
 
+// A row of a tile in LDS has no gap, as the copies straight into LDS leave none: its pieces of 16 bytes are swapped instead, by
+// the row's number, so that the lanes which read at once find different banks: 16 lanes a piece of a row each of the keys, 32 lanes
+// four pieces of four rows of the values.
 template <int DP>
-constexpr int pitch() { return DP * 2 + 32; }   // bytes of a row of a tile in LDS: 8 neighbouring rows start at banks of their own
+__device__ __forceinline__ int key_swap(int row) { return DP == 64 ? row >> 1 & 7 : DP == 128 ? row & 15 : row & 7; }
 template <int DP>
-constexpr int tile_bytes() { return kTile * pitch<DP>(); }
+__device__ __forceinline__ int value_swap(int row) { return DP == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4; }
 template <int DP>
-constexpr int rows_lds() { return 4 * tile_bytes<DP>() + 16; }
+constexpr int rows_lds() { return 4 * kTile * DP * 2; }
 
-template <typename T, int DP, bool FP8, bool EXTRA>
-__global__ __launch_bounds__(kWaves * 64, DP <= 128 ? 2 : 1) void attention_rows_kernel(const AttentionParams p) {
+// Asynchronous copy of 16 bytes a lane to LDS, lane after lane from byte `lds` on.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 is a reserved register: that it changes is what the clobber says
+__device__ __forceinline__ void copy_16_to_lds(uint32_t lds, const char* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+template <typename T, int DP, bool FP8, bool EXTRA, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 1) void attention_rows_kernel(const AttentionParams p) {
   typedef Element<T> E;
   typedef typename E::eight eight;
-  constexpr int kSteps = DP / 16, kColumns = DP / 32, kPitch = pitch<DP>(), kTileBytes = tile_bytes<DP>();
+  constexpr int kRows = 32 * WAVES;
+  constexpr int kSteps = DP / 16, kColumns = DP / 32, kPitch = DP * 2, kTileBytes = kTile * kPitch;
   constexpr int kLanes = FP8 ? DP / 16 : DP / 8;             // of a row, 16 bytes each
   constexpr int kGroup = 64 / kLanes;                        // rows that a wavefront copies at once
-  constexpr int kPasses = kTile / (kWaves * kGroup);
+  constexpr int kPasses = kTile / (WAVES * kGroup);
   extern __shared__ __attribute__((aligned(16))) char lds[];
   char* const k_tiles = lds;
   char* const v_tiles = lds + 2 * kTileBytes;
-  int* const flags = (int*)(lds + 4 * kTileBytes);
+  int* const flags = (int*)lds;   // behind the last tile
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kv_head = blockIdx.x % p.kv_heads, split = blockIdx.x / p.kv_heads / p.blocks;
+  int item, kv_head;
+  item_of(p, p.blocks * p.splits, blockIdx.x, item, kv_head);
+  const int split = item / p.blocks;
   // the blocks of the last tokens, which see the most keys, first
-  const RowBlock r = row_block<kRows>(p, p.blocks - 1 - blockIdx.x / p.kv_heads % p.blocks);
+  const RowBlock r = row_block<kRows>(p, p.blocks - 1 - item % p.blocks);
   if (r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;
 
   const int row = r.first + wave * 32 + (lane & 31), half = lane >> 5;
@@ -152,136 +169,225 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 128 ? 2 : 1) void attention_rows
     }
   }
 
-  // ---- copies of the tiles
-  u32x4_t k_next[kPasses], v_next[kPasses];
+  // ---- copies of the tiles: lane l finds the places of key l, and the lanes that copy the key get them from it.  Tiles past the last
+  // one find the last keys again, which nothing uses.  16-bit numbers go straight into LDS, 8-bit codes through registers.
   bool bad = false;
-  const int chunk = lane % kLanes, of_group = lane / kLanes;
-  const bool has_chunk = chunk * (FP8 ? 16 : 8) < p.dim, whole_groups = p.page_size % kGroup == 0;
-  const char* const k_base = p.k.data + kv_head * p.k.head;
-  const char* const v_base = p.v.data + kv_head * p.v.head;
+  int page_ahead = 0;        // the number of the page of this lane's key, a tile ahead of the places
+  uint32_t places = 0;       // of its values
+  uint32_t k_rows[kPasses], v_rows[kPasses];   // the places of the rows that this lane copies
+  u32x4_t k_next[FP8 ? kPasses : 1], v_next[FP8 ? kPasses : 1];
+  const int of_group = lane / kLanes, my_row_of_16 = wave * kGroup + of_group;   // (passes are multiples of 16 rows apart, of 8 in the widest form)
+  const int k_chunk = FP8 ? lane % kLanes : lane % kLanes ^ key_swap<DP>(my_row_of_16);
+  const int v_chunk = FP8 ? lane % kLanes : lane % kLanes ^ value_swap<DP>(my_row_of_16);
+  const bool has_k = k_chunk * (FP8 ? 16 : 8) < p.dim, has_v = v_chunk * (FP8 ? 16 : 8) < p.dim;
+  const bool alike = p.k.page == p.v.page && p.k.slot == p.v.slot;
+  const char* const k_base = p.k.data + kv_head * p.k.head + k_chunk * 16;
+  const char* const v_base = p.v.data + kv_head * p.v.head + v_chunk * 16;
+  const uint32_t k_lds = (uint32_t)(uintptr_t)(lds_void_t*)k_tiles + wave * 1024, v_lds = (uint32_t)(uintptr_t)(lds_void_t*)v_tiles + wave * 1024;
   const int32_t* const pages = p.table + (long)min(r.seq, p.seqs - 1) * p.table_stride;
-  auto fetch = [&](int of_tile) {
+  auto key_of = [&](int of_tile) { return min(max(of_tile * kTile + lane, low), high - 1); };
+  auto look_up = [&](int of_tile) { page_ahead = pages[page_of(p, key_of(of_tile))]; };
+  auto spread = [&](uint32_t (&rows)[kPasses], uint32_t place) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) rows[i] = __builtin_amdgcn_ds_bpermute(4 * ((i * WAVES + wave) * kGroup + of_group), (int)place);
+  };
+  auto find = [&](int of_tile) {   // the values' rows of the tile before, whose places are known, and the keys' of this one
+    spread(v_rows, places);
+    const int key = key_of(of_tile), at = page_of(p, key);
+    const uint32_t of_keys = place_of(p, p.k, key, at, page_ahead, bad);
+    places = alike ? of_keys : place_of(p, p.v, key, at, page_ahead, bad);
+    spread(k_rows, of_keys);
+  };
+  auto fetch = [&](u32x4_t* to, const char* base, const uint32_t (&rows)[kPasses], bool has, uint32_t at) {
+    if (!has) return;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int first = of_tile * kTile + (i * kWaves + wave) * kGroup;
-      k_next[i] = v_next[i] = u32x4_t{};
-      if (whole_groups) {   // the rows of a group lie in one page: its address is the wavefront's
-        const int key = min(max(first, low & -kGroup), (high - 1) & -kGroup), at = page_of(p, key);
-        const long page = page_number(p, pages[at], bad);
-        const int slot = key - at * p.page_size;
-        const uint32_t k_lane = of_group * (uint32_t)p.k.slot + chunk * 16, v_lane = of_group * (uint32_t)p.v.slot + chunk * 16;
-        const char* k_from = k_base + page * p.k.page + slot * p.k.slot;
-        const char* v_from = v_base + page * p.v.page + slot * p.v.slot;
-        if (has_chunk) {
-          k_next[i] = *reinterpret_cast<const u32x4_t*>(k_from + k_lane);
-          v_next[i] = *reinterpret_cast<const u32x4_t*>(v_from + v_lane);
-        }
-      } else {
-        const int key = min(max(first + of_group, low), high - 1), at = page_of(p, key);
-        const long page = page_number(p, pages[at], bad), slot = key - at * p.page_size;
-        if (has_chunk) {
-          k_next[i] = *reinterpret_cast<const u32x4_t*>(k_base + page * p.k.page + slot * p.k.slot + chunk * 16);
-          v_next[i] = *reinterpret_cast<const u32x4_t*>(v_base + page * p.v.page + slot * p.v.slot + chunk * 16);
-        }
-      }
+      if constexpr (FP8) to[i] = *reinterpret_cast<const u32x4_t*>(row_at(base, rows[i]));
+      else copy_16_to_lds(__builtin_amdgcn_readfirstlane(at + i * (WAVES * 1024)), row_at(base, rows[i]));
     }
   };
-  bool specials = false;   // infinities and NaNs of v were left out of a tile that is masked for some query
-  auto keep = [&](int of_tile, int buffer) {
-    const bool masked = of_tile * kTile < block_full_low || of_tile * kTile + kTile > block_full_high;
+  uint32_t specials = 0;   // infinities and NaNs of v were left out of a tile that is masked for some query
+  // What was fetched is in LDS when this ends, as far as this wavefront fetched it.
+  auto keep = [&](char* to_k, char* to_v, bool sift) {
+    if constexpr (FP8) {
+      auto widened = [&](u32x4_t x, char* tiles, int swap, int i, bool sift) {
+        char* row = tiles + my_row_of_16 * kPitch + i * (WAVES * kGroup * kPitch);
+        u32x4_t y = widen<T>(x[2], x[3]);
+        x = widen<T>(x[0], x[1]);
+        if (sift) x = finite_part<T>(x, specials), y = finite_part<T>(y, specials);
+        *reinterpret_cast<u32x4_t*>(row + 16 * (2 * k_chunk ^ swap)) = x;
+        *reinterpret_cast<u32x4_t*>(row + 16 * (2 * k_chunk + 1 ^ swap)) = y;
+      };
+      if (has_k) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int at = buffer * kTileBytes + ((i * kWaves + wave) * kGroup + of_group) * kPitch + chunk * (FP8 ? 32 : 16);
-      u32x4_t k0 = k_next[i], v0 = v_next[i];
-      if constexpr (FP8) {
-        const u32x4_t k1 = widen<T>(k0[2], k0[3]);
-        u32x4_t v1 = widen<T>(v0[2], v0[3]);
-        k0 = widen<T>(k0[0], k0[1]), v0 = widen<T>(v0[0], v0[1]);
-        if (masked) v1 = finite_part<T>(v1, specials);
-        *reinterpret_cast<u32x4_t*>(k_tiles + at + 16) = k1;
-        *reinterpret_cast<u32x4_t*>(v_tiles + at + 16) = v1;
+        for (int i = 0; i < kPasses; ++i) {
+          widened(k_next[i], to_k, key_swap<DP>(my_row_of_16), i, false);
+          widened(v_next[i], to_v, value_swap<DP>(my_row_of_16), i, sift);
+        }
       }
-      if (masked) v0 = finite_part<T>(v0, specials);
-      *reinterpret_cast<u32x4_t*>(k_tiles + at) = k0;
-      *reinterpret_cast<u32x4_t*>(v_tiles + at) = v0;
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (sift && has_v) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          u32x4_t* at = reinterpret_cast<u32x4_t*>(to_v + (i * WAVES + wave) * 1024 + lane * 16);
+          *at = finite_part<T>(*at, specials);
+        }
+      }
     }
   };
 
+  // ---- 32 keys at a time: the scores of the next ones, the weights of these, the output of those before, which do not wait for
+  // one another
   floatx16_t out[kColumns];
 #pragma unroll
   for (int c = 0; c < kColumns; ++c) out[c] = floatx16_t{};
   float most = -kInfinity, sum = 0.0f;
-
-  if (tile < last) {
-    fetch(tile);
-    keep(tile, 0);
-  }
-  __syncthreads();
-  for (int buffer = 0; tile < last; ++tile, buffer ^= 1) {
-    if (tile + 1 < last) fetch(tile + 1);
-    const int base = tile * kTile;
-    if (base < wave_high && base + kTile > wave_low) {
-      const bool masked = base < wave_full_low || base + kTile > wave_full_high;
-      // scores of 64 keys: lane l has those of query l % 32 with the keys 32 u + 8 (i / 4) + 4 (l / 32) + i % 4
-      floatx16_t s[2];
+  floatx16_t s[2];          // lane l has those of query l % 32 with the keys 8 (i / 4) + 4 (l / 32) + i % 4 of 32
+  eight weights[2][2];      // of 32 keys
+  // Half h of the tile `of_tile`: its scores become weights.  Meanwhile the scores of the half behind it are formed from k_from, and the
+  // half before it, h ^ 1 of v_from, goes to the output with its weights.  The matrix pipes take 32 cycles for a product, and a
+  // wavefront's instructions start in their order: so that pipes and vector units both have work, each product is followed by a
+  // share of the other instructions, and its operands are read from LDS two products of its kind ahead.
+  constexpr int kSlots = kSteps + 2 * kColumns, kTops = kSlots / 4;
+  eight k_piece[kSteps], v_piece[2 * kColumns];
+  const int k_place = (lane & 31) * kPitch + 16 * (half ^ key_swap<DP>(lane & 31)), v_row = 4 * half + (lane & 15) / 4;
+  const int v_place = v_row * kPitch + (32 * (lane >> 4 & 1) + (lane & 3) * 8 ^ 16 * value_swap<DP>(v_row));
+  // lane l reads key l % 32 of the half, numbers 16 d + 8 (l / 32)
+  auto read_keys = [&](const char* tiles, int h, int d) {
+    k_piece[d] = *reinterpret_cast<const eight*>(tiles + 32 * h * kPitch + (k_place ^ 32 * d));
+  };
+  // lane l reads column l % 16 of v for four keys at a time: keys 16 t + 8 u + 4 (l / 32), columns 32 c + 16 (l / 16 % 2)
+  auto read_values = [&](const char* tiles, int h, int n) {
+    const int t = n / kColumns, c = n % kColumns;
+    const char* from = tiles + (32 * h + 16 * t) * kPitch + (v_place ^ 64 * c);
+    const short4_t a = turned(from), b = turned(from + 8 * kPitch);
+    v_piece[n] = __builtin_bit_cast(eight, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto step = [&](int of_tile, auto half_of_tile, const char* k_from, const char* v_from) {
+    constexpr int h = decltype(half_of_tile)::value;
+    const int base = of_tile * kTile + 32 * h;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = floatx16_t{};
-        const char* from = k_tiles + buffer * kTileBytes + (32 * u + (lane & 31)) * kPitch + 16 * half;
+    for (int n = 0; n < 2; ++n) read_values(v_from, h ^ 1, n), read_keys(k_from, h ^ 1, n);
+    if (EXTRA) {
+      const float distance = (float)(sight.position - base - 4 * half);
 #pragma unroll
-        for (int d = 0; d < kSteps; ++d) s[u] = E::mfma32(*reinterpret_cast<const eight*>(from + 32 * d), q[d], s[u]);
-      }
-      if (EXTRA) {
-        const float distance = (float)(sight.position - base - 4 * half);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[u][i] = score.of(s[u][i], distance - (float)(32 * u + 8 * (i / 4) + i % 4));
-      }
-      if (masked) {
-        const uint64_t bits = sight.of(base) >> 4 * half;
-        const uint32_t seen[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[u][i] = seen[u] & (1u << (8 * (i / 4) + i % 4)) ? s[u][i] : -kInfinity;
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-      top = joined<true>(top, [](float a, float b) { return fmaxf(a, b); });
-      if (!EXTRA) top *= score.by;
-      if (__any(top > most + 8.0f)) {
-        const float now = fmaxf(most, top), by = now == -kInfinity ? 1.0f : __builtin_amdgcn_exp2f(most - now);
-        most = now, sum *= by;
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) out[c] *= by;
-      }
-      const float less = most == -kInfinity ? 0.0f : most;
-      eight weights[4];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float x = s[i / 16][i % 16];
-        const float w = __builtin_amdgcn_exp2f(EXTRA ? x - less : __builtin_fmaf(x, score.by, -less));
-        sum += w;
-        weights[i / 8][i % 8] = (T)w;
-      }
-      // lane l reads column l % 16 of v for four keys at a time: keys 16 t + 8 u + 4 (l / 32), columns 32 c + 16 (l / 16 % 2)
-      const char* from = v_tiles + buffer * kTileBytes + (4 * half + (lane & 15) / 4) * kPitch + 32 * (lane >> 4 & 1) + (lane & 3) * 8;
-      auto column = [&](int c, int t) {
-        const short4_t a = turned(from + 16 * t * kPitch + 64 * c), b = turned(from + (16 * t + 8) * kPitch + 64 * c);
-        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-      };
-#pragma unroll
-      for (int c = 0; c < kColumns; ++c)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) out[c] = E::mfma32(__builtin_bit_cast(eight, column(c, t)), weights[t], out[c]);
+      for (int i = 0; i < 16; ++i) s[h][i] = score.of(s[h][i], distance - (float)(8 * (i / 4) + i % 4));
     }
-    if (tile + 1 < last) keep(tile + 1, buffer ^ 1);
+    if (base < wave_full_low || base + 32 > wave_full_high) {
+      const uint32_t seen = (uint32_t)(sight.of(base) >> 4 * half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[h][i] = shown(s[h][i], seen, 8 * (i / 4) + i % 4);
+    }
+    s[h ^ 1] = floatx16_t{};
+    float top = -kInfinity, less = 0.0f, by = 1.0f;
+    bool rises = false;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int n = i / 2;
+      if (i % 2 == 0) {
+        if (n + 2 < 2 * kColumns) read_values(v_from, h ^ 1, n + 2);
+        out[n % kColumns] = E::mfma32(v_piece[n], weights[h ^ 1][n / kColumns], out[n % kColumns]);
+      } else {
+        if (n + 2 < kSteps) read_keys(k_from, h ^ 1, n + 2);
+        s[h ^ 1] = E::mfma32(k_piece[n], q[n], s[h ^ 1]);
+      }
+      if (i < kTops) {
+#pragma unroll
+        for (int e = 16 * i / kTops; e < 16 * (i + 1) / kTops; ++e) top = fmaxf(top, s[h][e]);
+      } else if (i == kTops) {
+        if (!EXTRA) top *= score.by;
+        rises = __any(top > most + 8.0f);
+        const float old = most, higher = fmaxf(old, joined<true>(top, [](float a, float b) { return fmaxf(a, b); }));
+        most = rises ? higher : old;
+        less = most == -kInfinity ? 0.0f : most, by = __builtin_amdgcn_exp2f(old - less);
+        sum *= by;
+      } else {
+        constexpr int kLeft = kSlots - kTops - 1;
+        const int j = i - kTops - 1;
+#pragma unroll
+        for (int pair = 8 * j / kLeft; pair < 8 * (j + 1) / kLeft; ++pair) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = s[h][2 * pair + e];
+            w[e] = __builtin_amdgcn_exp2f(EXTRA ? x - less : __builtin_fmaf(x, score.by, -less));
+          }
+          auto both = E::pair(w[0], w[1]);
+          asm volatile("" : "+v"(both));   // (or the weights would be formed where they are used, behind the products)
+          weights[h][pair / 4][pair % 4 * 2] = both[0], weights[h][pair / 4][pair % 4 * 2 + 1] = both[1];
+          sum = E::add(both, sum);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (rises) {
+      float shrink = by;
+      asm volatile("" : "+v"(shrink));   // (or the products would be formed every time, ahead of the branch)
+#pragma unroll
+      for (int c = 0; c < kColumns; ++c) out[c] *= shrink;
+    }
+  };
+  if (p.dim < DP) {   // what no copy reaches
+    for (int i = threadIdx.x * 16; i < 4 * kTileBytes; i += WAVES * 64 * 16) *reinterpret_cast<u32x4_t*>(lds + i) = u32x4_t{};
     __syncthreads();
+  }
+  if (tile < last) {
+    look_up(tile);
+    find(tile);
+    look_up(tile + 1);
+    fetch(k_next, k_base, k_rows, has_k, k_lds);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) weights[1][i] = eight{};
+    for (int i = threadIdx.x * 16; i < kTileBytes; i += WAVES * 64 * 16) *reinterpret_cast<u32x4_t*>(v_tiles + kTileBytes + i) = u32x4_t{};
+    if constexpr (FP8) {
+      if (has_k) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+          char* row = k_tiles + my_row_of_16 * kPitch + i * (WAVES * kGroup * kPitch);
+          const int swap = key_swap<DP>(my_row_of_16);
+          *reinterpret_cast<u32x4_t*>(row + 16 * (2 * k_chunk ^ swap)) = widen<T>(k_next[i][0], k_next[i][1]);
+          *reinterpret_cast<u32x4_t*>(row + 16 * (2 * k_chunk + 1 ^ swap)) = widen<T>(k_next[i][2], k_next[i][3]);
+        }
+      }
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    find(tile + 1);
+    fetch(v_next, v_base, v_rows, has_v, v_lds);
+    fetch(k_next, k_base, k_rows, has_k, k_lds + kTileBytes);
+    look_up(tile + 2);
+    s[0] = floatx16_t{};
+#pragma unroll
+    for (int d = 0; d < kSteps; ++d) {
+      read_keys(k_tiles, 0, d);
+      s[0] = E::mfma32(k_piece[d], q[d], s[0]);
+    }
+    int buffer = 0;
+    for (; tile < last; ++tile, buffer ^= kTileBytes) {
+      char *const k_here = k_tiles + buffer, *const v_here = v_tiles + buffer;
+      char *const k_there = k_tiles + (buffer ^ kTileBytes), *const v_there = v_tiles + (buffer ^ kTileBytes);
+      step(tile, std::integral_constant<int, 0>{}, k_here, v_there);
+      find(tile + 2);
+      keep(k_there, v_here, tile * kTile < block_full_low || tile * kTile + kTile > block_full_high);
+      __syncthreads();
+      fetch(v_next, v_base, v_rows, has_v, v_lds + (buffer ^ kTileBytes));
+      fetch(k_next, k_base, k_rows, has_k, k_lds + buffer);
+      look_up(tile + 3);
+      step(tile, std::integral_constant<int, 1>{}, k_there, v_here);
+    }
+#pragma unroll
+    for (int n = 0; n < 2 * kColumns; ++n) {
+      read_values(v_tiles + (buffer ^ kTileBytes), 1, n);
+      out[n % kColumns] = E::mfma32(v_piece[n], weights[1][n / kColumns], out[n % kColumns]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (copies that nothing uses would land in LDS of another workgroup)
   }
 
   // ---- results
+  __syncthreads();
   if (threadIdx.x == 0) flags[0] = 0;
   __syncthreads();
   if (bad) atomicOr(flags, 1);
@@ -316,65 +422,359 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 128 ? 2 : 1) void attention_rows
     add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last, min(r.rows, r.first + kRows), block_full_low, block_full_high);
 }
 
-// ---------------------------------------------------------------- the parts of a split joined
-// A wavefront a row: out = sum over the parts of 2^(m_i - m) o_i, divided by that of their sums.
-template <typename T, int ROWS>
-__global__ __launch_bounds__(256) void attention_join_kernel(const AttentionParams p) {
-  const int lane = threadIdx.x & 63;
-  const int kv_head = blockIdx.x % p.kv_heads, rest = blockIdx.x / p.kv_heads;
-  constexpr int kQuarters = ROWS >= 16 ? ROWS / 16 : 1;   // workgroups of a block of rows, 16 rows each
-  const RowBlock r = row_block<ROWS>(p, rest / kQuarters);
-  if (r.first >= r.rows || r.seq == p.seqs) return;
-  int low, high, first, last, parts;
-  keys_seen(p, r, r.first / p.group, min(r.first + ROWS - 1, r.rows - 1) / p.group, low, high);
-  first = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile;
-  split_of(p, 0, first, last, parts);
-  if (parts <= 1) return;
-  const float v_scale = value_scale(p, kv_head);
-  for (int i = threadIdx.x >> 6; i < min(ROWS, 16); i += 4) {
-    const int row = r.first + rest % kQuarters * 16 + i;
-    if (row >= r.rows) return;
-    const long token = r.token + row / p.group, head = kv_head * p.group + row % p.group;
-    const long at = token * p.heads + head, step = (long)p.tokens * p.heads;
-    float most = -kInfinity;
-    for (int s = 0; s < parts; ++s) most = fmaxf(most, p.part_ml[at + s * step].x);
-    const float less = most == -kInfinity ? 0.0f : most;
-    float sum = 0.0f, out[4] = {};
-    for (int s = 0; s < parts; ++s) {
-      const float2 ml = p.part_ml[at + s * step];
-      const float by = __builtin_amdgcn_exp2f(ml.x - less);
-      sum = __builtin_fmaf(by, ml.y, sum);
-      if (4 * lane < p.dim) {
-        const floatx4_t o = *reinterpret_cast<const floatx4_t*>(p.part_o + (at + s * step) * p.dim + 4 * lane);
+// ---------------------------------------------------------------- few rows
+// A workgroup takes 16 * TILES rows of a kv head, and its wavefronts take 32 keys in turn, each with a maximum, a sum and an output
+// of its own, which are joined at the end.  Keys go from memory straight into the registers of the product, values through a piece
+// of LDS that is the wavefront's own, to be turned there: no wavefront waits for another until the end.
+constexpr int kWaves = 4;    // of a workgroup
+constexpr int kUnit = 32;    // keys that a wavefront takes at once
+
+template <int DP>
+constexpr int pitch() { return DP * 2 + 32; }   // bytes of a row there: 8 neighbouring rows start at banks of their own
+template <int DP>
+constexpr int few_lds() { return kWaves * kUnit * pitch<DP>() + kWaves * 16 * 8 + 16; }
+
+constexpr int few_waves(int dp, int tiles) { return dp == 64 ? 5 - tiles : dp == 128 ? 4 - tiles : 3 - tiles; }   // a SIMD
+
+template <typename T, int DP, bool FP8, bool EXTRA, int TILES>
+__global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_few_kernel(const AttentionParams p) {
+  typedef Element<T> E;
+  typedef typename E::eight eight;
+  constexpr int kSteps = DP / 32, kColumns = DP / 16, kPitch = pitch<DP>(), kLoads = FP8 ? DP / 64 : DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int column = lane & 15, quarter = lane >> 4;
+  char* const mine = lds + wave * kUnit * kPitch;
+  float2* const sums = (float2*)(lds + kWaves * kUnit * kPitch);   // [kWaves][16]
+  int* const flags = (int*)(sums + kWaves * 16);
+
+  int item, kv_head;
+  item_of(p, p.blocks * p.splits, blockIdx.x, item, kv_head);
+  const int split = item / p.blocks;
+  const RowBlock r = row_block<16 * TILES>(p, item % p.blocks);
+  if (r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;
+  const int block_t0 = r.first / p.group, block_t1 = min(r.first + 16 * TILES - 1, r.rows - 1) / p.group;
+  int low, high;
+  keys_seen(p, r, block_t0, block_t1, low, high);
+  int first_tile = low / kTile, last_tile = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
+  if (!split_of(p, split, first_tile, last_tile, parts)) return;
+  const bool bounded = p.causal && p.tree == nullptr;
+  const int full_low = bounded && p.window > 0 ? max(r.past + block_t1 - p.window + 1, 0) : 0;
+  const int full_high = p.tree != nullptr ? min(r.len, r.past) : bounded ? min(r.len, r.past + block_t0 + 1) : r.len;
+
+  Sight sight[TILES];
+  Score score[TILES];
+  eight q[TILES][kSteps];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(by, o[e], out[e]);
-      }
-    }
-    const float by = sum == 0.0f ? 0.0f : v_scale / sum;
-    if (4 * lane < p.dim) {
-      *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + 4 * lane) =
-          four<T>(out[0] * by, out[1] * by, out[2] * by, out[3] * by);
+  for (int n = 0; n < TILES; ++n) {
+    const int row = min(r.first + 16 * n + column, r.rows - 1), t = row / p.group, head = kv_head * p.group + row % p.group;
+    const long token = r.token + t;
+    sight[n] = Sight{r.past + t, r.len, r.past, bounded && p.window > 0 ? r.past + t - p.window + 1 : 0,
+                     p.tree == nullptr ? nullptr : p.tree + token * p.tree_words, p.tree_words, p.causal};
+    score[n] = score_of(p, kv_head, head);
+    const T* from = (const T*)p.q + token * p.q_token + head * p.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {   // of an 8-bit cache a lane holds 16 neighbouring numbers of a key, for two steps
+      const int d = FP8 ? 64 * (s / 2) + 16 * quarter + 8 * (s % 2) : 32 * s + 8 * quarter;
+      q[n][s] = eight{};
+      if (d < p.dim) q[n][s] = *reinterpret_cast<const eight*>(from + d);
     }
   }
+
+  const char* const k_base = p.k.data + kv_head * p.k.head + 16 * quarter;
+  const char* const v_base = p.v.data + kv_head * p.v.head + 16 * quarter;
+  const int32_t* const pages = p.table + (long)min(r.seq, p.seqs - 1) * p.table_stride;
+  bool bad = false;
+  uint32_t specials = 0;
+  u32x4_t k[2][kLoads], v[2][kLoads];   // keys 16 a + lane % 16
+  int numbers[2];                       // of their pages, a unit ahead
+  auto key_of = [&](int unit, int a) { return min(max(unit * kUnit + 16 * a + column, low), high - 1); };
+  auto look_up = [&](int unit) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) numbers[a] = pages[page_of(p, key_of(unit, a))];
+  };
+  auto fetch = [&](int unit) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int key = key_of(unit, a), at = page_of(p, key);
+      const char* k_from = row_at(k_base, place_of(p, p.k, key, at, numbers[a], bad));
+      const char* v_from = row_at(v_base, place_of(p, p.v, key, at, numbers[a], bad));
+#pragma unroll
+      for (int s = 0; s < kLoads; ++s) {
+        k[a][s] = v[a][s] = u32x4_t{};
+        if ((FP8 ? 64 * s + 16 * quarter : 32 * s + 8 * quarter) < p.dim) {
+          k[a][s] = *reinterpret_cast<const u32x4_t*>(k_from + 64 * s);
+          v[a][s] = *reinterpret_cast<const u32x4_t*>(v_from + 64 * s);
+        }
+      }
+    }
+  };
+
+  floatx4_t out[kColumns][TILES];
+  float most[TILES], sum[TILES];
+#pragma unroll
+  for (int n = 0; n < TILES; ++n) {
+    most[n] = -kInfinity, sum[n] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) out[c][n] = floatx4_t{};
+  }
+  int unit = 2 * first_tile + wave;
+  const int last = min(2 * last_tile, (high + kUnit - 1) / kUnit);
+  if (unit < last) {
+    look_up(unit);
+    fetch(unit);
+    if (unit + kWaves < last) look_up(unit + kWaves);
+  }
+  for (; unit < last; unit += kWaves) {
+    const int base = unit * kUnit;
+    const bool masked = base < full_low || base + kUnit > full_high;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int s = 0; s < kLoads; ++s) {
+        char* to = mine + (16 * a + column) * kPitch + (FP8 ? 128 * s + 32 * quarter : 64 * s + 16 * quarter);
+        u32x4_t v0 = v[a][s];
+        if constexpr (FP8) {
+          u32x4_t v1 = widen<T>(v0[2], v0[3]);
+          v0 = widen<T>(v0[0], v0[1]);
+          if (masked) v1 = finite_part<T>(v1, specials);
+          *reinterpret_cast<u32x4_t*>(to + 16) = v1;
+        }
+        if (masked) v0 = finite_part<T>(v0, specials);
+        *reinterpret_cast<u32x4_t*>(to) = v0;
+      }
+    // scores of 32 keys: lane l has those of query l % 16 with the keys 16 a + 4 (l / 16) + i
+    floatx4_t s[2][TILES];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int n = 0; n < TILES; ++n) {
+        s[a][n] = floatx4_t{};
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          u32x4_t piece;
+          if constexpr (FP8) piece = d % 2 == 0 ? widen<T>(k[a][d / 2][0], k[a][d / 2][1]) : widen<T>(k[a][d / 2][2], k[a][d / 2][3]);
+          else piece = k[a][d];
+          s[a][n] = E::mfma16(__builtin_bit_cast(eight, piece), q[n][d], s[a][n]);
+        }
+      }
+    if (unit + kWaves < last) {
+      fetch(unit + kWaves);
+      if (unit + 2 * kWaves < last) look_up(unit + 2 * kWaves);
+    }
+    eight weights[TILES];
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) {
+      if (EXTRA) {
+        const float distance = (float)(sight[n].position - base - 4 * quarter);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i / 4][n][i % 4] = score[n].of(s[i / 4][n][i % 4], distance - (float)(16 * (i / 4) + i % 4));
+      }
+      if (masked) {
+        const uint32_t seen = (uint32_t)(sight[n].of(base) >> 4 * quarter);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i / 4][n][i % 4] = shown(s[i / 4][n][i % 4], seen, 16 * (i / 4) + i % 4);
+      }
+      float top = s[0][n][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][n][i % 4]);
+      if (!EXTRA) top *= score[n].by;
+      if (__any(top > most[n] + 8.0f)) {
+        auto larger = [](float a, float b) { return fmaxf(a, b); };
+        const float now = fmaxf(most[n], joined<true>(joined<false>(top, larger), larger));
+        const float by = now == -kInfinity ? 1.0f : __builtin_amdgcn_exp2f(most[n] - now);
+        most[n] = now, sum[n] *= by;
+#pragma unroll
+        for (int c = 0; c < kColumns; ++c) out[c][n] *= by;
+      }
+      const float less = most[n] == -kInfinity ? 0.0f : most[n];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = s[i / 4][n][i % 4];
+        const float w = __builtin_amdgcn_exp2f(EXTRA ? x - less : __builtin_fmaf(x, score[n].by, -less));
+        sum[n] += w;
+        weights[n][i] = (T)w;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (what other lanes wrote is read)
+    __builtin_amdgcn_wave_barrier();
+    // lane l reads column l % 16 of v for four keys at a time: keys 16 a + 4 (l / 16)
+    const char* from = mine + (4 * quarter + column / 4) * kPitch + (column & 3) * 8;
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) {
+      const short4_t a = turned(from + 32 * c), b = turned(from + 16 * kPitch + 32 * c);
+      const eight piece = __builtin_bit_cast(eight, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int n = 0; n < TILES; ++n) out[c][n] = E::mfma16(piece, weights[n], out[c][n]);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // ---- the wavefronts' results joined, 16 rows at a time: a row's numbers 4 (DP + 4) bytes apart
+  if (threadIdx.x == 0) flags[0] = 0;
+  __syncthreads();
+  if (bad) atomicOr(flags, 1);
+  if (specials) atomicOr(flags, 2);
+  constexpr int kOut = 4 * DP + 16;
+  const float v_scale = value_scale(p, kv_head);
+#pragma unroll
+  for (int n = 0; n < TILES; ++n) {
+    auto add = [](float a, float b) { return a + b; };
+    sum[n] = joined<true>(joined<false>(sum[n], add), add);
+    if (quarter == 0) sums[wave * 16 + column] = make_float2(most[n], sum[n]);
+#pragma unroll
+    for (int c = 0; c < kColumns; ++c) *reinterpret_cast<floatx4_t*>(mine + column * kOut + 64 * c + 16 * quarter) = out[c][n];
+    __syncthreads();
+    const int in_tile = threadIdx.x / 16, row = r.first + 16 * n + in_tile;
+    if (row < r.rows) {
+      const long token = r.token + row / p.group;
+      const int head = kv_head * p.group + row % p.group;
+      float all = -kInfinity, total = 0.0f, by[kWaves];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) all = fmaxf(all, sums[w * 16 + in_tile].x);
+      const float less = all == -kInfinity ? 0.0f : all;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        by[w] = __builtin_amdgcn_exp2f(sums[w * 16 + in_tile].x - less);
+        total = __builtin_fmaf(by[w], sums[w * 16 + in_tile].y, total);
+      }
+      if (flags[0] & 1) total = __builtin_nanf("");
+      const long at = ((long)split * p.tokens + token) * p.heads + head;
+      if (parts > 1 && threadIdx.x % 16 == 0) p.part_ml[at] = make_float2(all, total);
+      const float scale = total == 0.0f ? 0.0f : v_scale / total;
+#pragma unroll
+      for (int j = 0; j < DP / 64; ++j) {
+        const int d = 64 * j + 4 * (threadIdx.x % 16);
+        if (d >= p.dim) continue;
+        floatx4_t o{};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const floatx4_t x = *reinterpret_cast<const floatx4_t*>(lds + w * kUnit * kPitch + in_tile * kOut + 4 * d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by[w], x[e], o[e]);
+        }
+        if (parts > 1) *reinterpret_cast<floatx4_t*>(p.part_o + at * p.dim + d) = o;
+        else *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + d) =
+            four<T>(o[0] * scale, o[1] * scale, o[2] * scale, o[3] * scale);
+      }
+    }
+    __syncthreads();
+  }
+  if (flags[0] & 2)
+    add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last_tile, min(r.rows, r.first + 16 * TILES), full_low, full_high);
+}
+
+// ---------------------------------------------------------------- the parts of a split joined
+// out = sum over the parts of 2^(m_i - m) o_i, divided by that of their sums.  A wavefront (WIDE: a workgroup) a row; 4 numbers of it
+// a lane, LANES = dim / 4 rounded up, so that 64 / LANES parts are read at once by a wavefront.
+template <typename T, int LANES, bool WIDE>
+__global__ __launch_bounds__(256) void attention_join_kernel(const AttentionParams p) {
+  constexpr int kAtOnce = 64 / LANES, kStep = WIDE ? 4 * kAtOnce : kAtOnce;
+  __shared__ float4 numbers[WIDE ? 4 : 1][64];
+  __shared__ float totals[WIDE ? 4 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long at = (long)blockIdx.x * (WIDE ? 1 : 4) + (WIDE ? 0 : wave);
+  if (at >= (long)p.tokens * p.heads) return;
+  const int token = at / p.heads, head = at % p.heads, kv_head = head / p.group;
+  RowBlock r = sequence_of(p, token, [](int, int start) { return start; });
+  if (r.seq == p.seqs || token < r.token) return;
+  r.first = ((token - r.token) * p.group + head % p.group) / p.rows * p.rows;
+  int low, high;
+  keys_seen(p, r, r.first / p.group, min(r.first + p.rows - 1, r.rows - 1) / p.group, low, high);
+  int first = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
+  split_of(p, 0, first, last, parts);
+  if (parts <= 1) return;
+  const long step = (long)p.tokens * p.heads;
+  auto larger = [](float a, float b) { return fmaxf(a, b); };
+  float most = -kInfinity;
+  for (int s = lane; s < parts; s += 64) most = fmaxf(most, p.part_ml[at + s * step].x);
+  most = over_wave(most, -kInfinity, larger);
+  const float less = most == -kInfinity ? 0.0f : most;
+  float sum = 0.0f, out[4] = {};
+  const int d = lane % LANES * 4;
+#pragma unroll 4
+  for (int s = (WIDE ? wave * kAtOnce : 0) + lane / LANES; s < parts; s += kStep) {
+    const float2 ml = p.part_ml[at + s * step];
+    const float by = __builtin_amdgcn_exp2f(ml.x - less);
+    sum = __builtin_fmaf(by, ml.y, sum);
+    if (d < p.dim) {
+      const floatx4_t o = *reinterpret_cast<const floatx4_t*>(p.part_o + (at + s * step) * p.dim + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(by, o[e], out[e]);
+    }
+  }
+  auto add = [](float a, float b) { return a + b; };
+  if (LANES <= 16) {
+    sum = joined<false>(sum, add);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = joined<false>(out[e], add);
+  }
+  if (LANES <= 32) {
+    sum = joined<true>(sum, add);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = joined<true>(out[e], add);
+  }
+  if (WIDE) {
+    numbers[wave][lane] = make_float4(out[0], out[1], out[2], out[3]);
+    if (lane == 0) totals[wave] = sum;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 x = numbers[w][lane];
+      out[0] += x.x, out[1] += x.y, out[2] += x.z, out[3] += x.w, sum += totals[w];
+    }
+  }
+  if (lane >= LANES || d >= p.dim) return;
+  const float by = sum == 0.0f ? 0.0f : value_scale(p, kv_head) / sum;
+  *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + d) =
+      four<T>(out[0] * by, out[1] * by, out[2] * by, out[3] * by);
 }
 
 // ---------------------------------------------------------------- the choice
+// Whether there is a form of eight wavefronts and 256 rows: the widest heads have no registers for it, and the narrow ones gain nothing
+// (8192 tokens of 32 heads of 64: 353 us, with 128 rows 344; of 128: 574 and 590).
+constexpr bool eight_waves(int dp) { return dp == 128; }
+
 struct Plan {
+  int rows;   // of a block: 16 and 32 in the form for few rows, 128 and 256 in that for many
   long blocks, splits, split_tiles;
   size_t ml_bytes, o_bytes;
 };
 
 Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_seq_len, int64_t window) {
   Plan plan{};
-  const int64_t group = heads / kv_heads;
-  plan.blocks = tokens * group / kRows + seqs + 1;
-  // parts of the keys so that there are some 512 workgroups, of 256 keys at least
-  const int64_t rows = std::max<int64_t>((tokens * group + kRows - 1) / kRows, std::min(seqs, tokens));
-  const int64_t keys = window > 0 ? std::min(max_seq_len, window + (tokens + seqs - 1) / std::max<int64_t>(seqs, 1)) : max_seq_len;
-  const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
-  const int64_t wanted = std::max<int64_t>(512 / std::max<int64_t>(rows * kv_heads, 1), 1);
-  plan.split_tiles = std::max<int64_t>((tiles + wanted - 1) / wanted, 4);
-  plan.splits = (tiles + plan.split_tiles - 1) / plan.split_tiles;
+  const int64_t group = heads / kv_heads, queries = (tokens + seqs - 1) / std::max<int64_t>(seqs, 1), of_sequence = queries * group;
+  const int dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  // 256 rows from two rounds of workgroups on: two pieces of 2048 tokens behind 6144 others 488 us, with 128 rows 510; 33 sequences of
+  // up to 500 tokens, one round, 212 and 177
+  plan.rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : eight_waves(dp) && tokens * heads / 256 >= 512 ? 256 : 128;
+  plan.blocks = tokens * group / plan.rows + seqs + 1;
+  const int64_t groups = std::max<int64_t>((tokens * group + plan.rows - 1) / plan.rows, std::min(seqs, tokens)) * kv_heads;
+  const int64_t keys = std::max<int64_t>(window > 0 ? std::min(max_seq_len, window + queries) : max_seq_len, 1);
+  if (plan.rows <= 32) {
+    // Tiles of a part: with t of them a workgroup takes some 0.6 t us, and joining the others 0.1 us a part, so that the square root
+    // of 0.15 times the sequence's tiles is about the best for one sequence (8000 keys: 4 tiles 18.3 us, 2 23.5); with more of them
+    // about 2048 workgroups, which even out (64 sequences of 800 to 4096 keys: 162 us, with 512 workgroups 196).
+    const int64_t tiles = (keys + kTile - 1) / kTile;
+    const int64_t for_one = (int64_t)__builtin_sqrt(0.15 * (double)tiles + 0.25), for_many = std::min<int64_t>(groups * tiles / 2048, 32);
+    plan.split_tiles = std::min(std::max<int64_t>(std::max(for_one, for_many), 2), tiles);
+    plan.splits = (tiles + plan.split_tiles - 1) / plan.split_tiles;
+  } else {
+    // Parts, by what a round of workgroups takes (us a tile, measured) and what writing and reading the parts takes.
+    const int64_t tiles = (keys - std::min(queries, keys) / 2 + kTile - 1) / kTile, longest = (keys + kTile - 1) / kTile;
+    const double of_tile = dp == 64 ? 1.3 : dp == 128 ? 2.1 : 2.6;
+    const int64_t at_once = dp == 256 || plan.rows == 256 ? 256 : 512;
+    double best = 0.0;
+    plan.splits = 1;
+    for (int64_t parts = 1; parts <= 32 && parts <= tiles; ++parts) {
+      const double rounds = (double)((groups * parts + at_once - 1) / at_once), bytes = 8.0 * (double)(parts * tokens * heads * head_dim);
+      const double time = rounds * ((double)((tiles + parts - 1) / parts) * of_tile + 4.0) + (parts > 1 ? 5.0 + 0.3 * (double)parts + bytes / 4e6 : 0.0);
+      if (parts == 1 || time < 0.97 * best) best = time, plan.splits = parts;
+    }
+    plan.split_tiles = (longest + plan.splits - 1) / plan.splits;
+    plan.splits = (longest + plan.split_tiles - 1) / plan.split_tiles;
+  }
   if (plan.splits > 1) {
     plan.ml_bytes = (size_t)(plan.splits * tokens * heads) * sizeof(float2);
     plan.ml_bytes = (plan.ml_bytes + 15) / 16 * 16;
@@ -383,24 +783,39 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
   return plan;
 }
 
+template <typename T, int DP>
+int launch_join(const AttentionParams& p, hipStream_t st) {
+  if (p.splits == 1) return SONAR_OK;
+  const long rows = (long)p.tokens * p.heads;
+  // (a workgroup a row where parts are many and rows few: one sequence of 8000 keys 18 us, a wavefront a row 24)
+  if (p.splits > 8 && rows <= 1024) attention_join_kernel<T, DP / 4, true><<<(uint32_t)rows, 256, 0, st>>>(p);
+  else attention_join_kernel<T, DP / 4, false><<<(uint32_t)((rows + 3) / 4), 256, 0, st>>>(p);
+  return launch_status("attention_join_kernel");
+}
+
+template <typename K>
+int launch_one(K kernel, const AttentionParams& p, int waves, int lds, const char* name, hipStream_t st) {
+  if (lds > 65536) SONAR_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  kernel<<<(uint32_t)(p.blocks * p.kv_heads * p.splits), waves * 64, lds, st>>>(p);
+  return launch_status(name);
+}
+
 template <typename T, int DP, bool FP8, bool EXTRA>
-int launch_rows(const AttentionParams& p, hipStream_t st) {
-  const void* kernel = (const void*)attention_rows_kernel<T, DP, FP8, EXTRA>;
-  if (rows_lds<DP>() > 65536) SONAR_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, rows_lds<DP>()));
-  attention_rows_kernel<T, DP, FP8, EXTRA><<<(uint32_t)(p.blocks * p.kv_heads * p.splits), kWaves * 64, rows_lds<DP>(), st>>>(p);
-  if (int rc = launch_status("attention_rows_kernel")) return rc;
-  if (p.splits > 1) {
-    attention_join_kernel<T, kRows><<<(uint32_t)(p.blocks * (kRows / 16) * p.kv_heads), 256, 0, st>>>(p);
-    return launch_status("attention_join_kernel");
-  }
-  return SONAR_OK;
+int launch_form(const AttentionParams& p, hipStream_t st) {
+  int rc;
+  if (p.rows == 16) rc = launch_one(attention_few_kernel<T, DP, FP8, EXTRA, 1>, p, kWaves, few_lds<DP>(), "attention_few_kernel", st);
+  else if (p.rows == 32) rc = launch_one(attention_few_kernel<T, DP, FP8, EXTRA, 2>, p, kWaves, few_lds<DP>(), "attention_few_kernel", st);
+  else if (p.rows == 128) rc = launch_one(attention_rows_kernel<T, DP, FP8, EXTRA, 4>, p, 4, rows_lds<DP>(), "attention_rows_kernel", st);
+  else if constexpr (eight_waves(DP)) rc = launch_one(attention_rows_kernel<T, DP, FP8, EXTRA, 8>, p, 8, rows_lds<DP>(), "attention_rows_kernel", st);
+  else return fail(SONAR_E_INVALID, "no form of %d rows", p.rows);
+  return rc != SONAR_OK ? rc : launch_join<T, DP>(p, st);
 }
 
 template <typename T, int DP>
 int launch_width(const AttentionParams& p, bool fp8, hipStream_t st) {
   const bool extra = p.cap > 0.0f || p.slopes != nullptr;
-  if (fp8) return extra ? launch_rows<T, DP, true, true>(p, st) : launch_rows<T, DP, true, false>(p, st);
-  return extra ? launch_rows<T, DP, false, true>(p, st) : launch_rows<T, DP, false, false>(p, st);
+  if (fp8) return extra ? launch_form<T, DP, true, true>(p, st) : launch_form<T, DP, true, false>(p, st);
+  return extra ? launch_form<T, DP, false, true>(p, st) : launch_form<T, DP, false, false>(p, st);
 }
 
 template <typename T>
@@ -446,7 +861,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   SONAR_REQUIRE(cache_dtype == dtype || cache_dtype == SONAR_CACHE_FP8, "cache_dtype = %d does not go with dtype = %d", cache_dtype, dtype);
   SONAR_REQUIRE(key_cache && value_cache, "key_cache and value_cache must not be NULL");
   SONAR_REQUIRE(page_size >= 1 && pages >= 0 && pages < (1LL << 31) && table_pages >= 0 && page_size < (1LL << 31) &&
-                    table_pages < (1LL << 31) && table_pages * page_size < (1LL << 31),
+                    table_pages < (1LL << 31) && table_pages * page_size < (1LL << 31) - 1024,
                 "pages = %ld of %ld slots, %ld a sequence", (long)pages, (long)page_size, (long)table_pages);
   SONAR_REQUIRE(scale > 0.0 && scale <= 3e38, "scale = %g must be positive", scale);
   SONAR_REQUIRE(cap >= 0.0 && cap <= 1e30, "cap = %g must be 0 (none) or positive", cap);
@@ -458,7 +873,9 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
     SONAR_REQUIRE(c->page_stride % unit == 0 && c->slot_stride % unit == 0 && c->head_stride % unit == 0 && (uintptr_t)c->data % 16 == 0,
                   "a cache must be 16-byte aligned, with strides of multiples of 16 bytes; got %ld, %ld, %ld elements", (long)c->page_stride,
                   (long)c->slot_stride, (long)c->head_stride);
-    SONAR_REQUIRE(c->slot_stride >= 0 && c->slot_stride * cache_size * 64 < (1LL << 31), "a cache's slots are %ld elements apart", (long)c->slot_stride);
+    SONAR_REQUIRE(c->slot_stride >= 0 && c->page_stride >= 0 && c->slot_stride < (1LL << 36) / page_size && c->page_stride < (1LL << 37) / (pages + 1) &&
+                      ((pages - 1) * c->page_stride + (page_size - 1) * c->slot_stride) * cache_size < (1LL << 36),
+                  "a cache of %ld pages %ld elements apart: more than 64 GiB", (long)pages, (long)c->page_stride);
     SONAR_REQUIRE(cache_dtype != SONAR_CACHE_FP8 || (c->scale != nullptr && (c->scale_len == 1 || c->scale_len == kv_heads)),
                   "an 8-bit cache needs 1 or %ld scales; got %ld", (long)kv_heads, c->scale == nullptr ? 0L : (long)c->scale_len);
   }
@@ -472,12 +889,12 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, max_seq_len, window);
   if (scratch_bytes < plan.ml_bytes + plan.o_bytes || scratch == nullptr) plan.splits = 1;
   SONAR_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
-  SONAR_REQUIRE(plan.blocks * kv_heads * plan.splits < (1LL << 24) && plan.blocks * (kRows / 16) * kv_heads < (1LL << 24),
+  SONAR_REQUIRE(plan.blocks * kv_heads * plan.splits < (1LL << 24) && (plan.splits == 1 || tokens * heads < (1LL << 24)),
                 "%ld tokens of %ld sequences and %ld heads take too many workgroups", (long)tokens, (long)seqs, (long)heads);
   auto pages_of = [&](const sonar_kv_cache* c) {
     const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
-    return CachePages{(const char*)c->data, c->page_stride * cache_size, c->slot_stride * cache_size, c->head_stride * cache_size,
-                      fp8 ? c->scale : nullptr, c->scale_len > 1};
+    return CachePages{(const char*)c->data, (uint32_t)(c->page_stride * cache_size / 16), (uint32_t)(c->slot_stride * cache_size / 16),
+                      c->head_stride * cache_size, fp8 ? c->scale : nullptr, c->scale_len > 1};
   };
   AttentionParams p{};
   p.q = (const char*)q, p.q_token = q_token_stride, p.q_head = q_head_stride;
@@ -486,13 +903,14 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   p.out = (char*)out, p.out_token = out_token_stride, p.out_head = out_head_stride;
   p.slopes = slopes, p.tree = (const uint64_t*)tree_mask, p.tree_words = (int)tree_words;
   p.part_ml = (float2*)scratch, p.part_o = (float*)((char*)scratch + plan.ml_bytes);
-  p.scale = (float)scale, p.cap = (float)cap, p.window = (int)window, p.causal = causal != 0, p.clear_rest = clear_rest != 0;
+  p.scale = (float)scale, p.cap = (float)cap, p.window = window < table_pages * page_size ? (int)window : 0, p.causal = causal != 0, p.clear_rest = clear_rest != 0;
   int log = 0;
   while ((1LL << log) < page_size) ++log;
   p.page_shift = 31 + log, p.page_magic = (uint32_t)((1ULL << p.page_shift) / (uint64_t)page_size + 1);
   p.page_size = (int)page_size, p.pages = (int)pages, p.table_pages = (int)table_pages;
   p.tokens = (int)tokens, p.seqs = (int)seqs, p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads);
-  p.dim = (int)head_dim, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles;
+  p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles;
+  p.by_dies = plan.rows <= 32;
   const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
   hipStream_t st = (hipStream_t)stream;
   return dtype == SONAR_DTYPE_F16 ? launch<_Float16>(p, fp8, st) : launch<__bf16>(p, fp8, st);

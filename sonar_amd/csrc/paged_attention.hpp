@@ -17,7 +17,8 @@ constexpr float kInfinity = __builtin_inff();
 
 struct CachePages {
   const char* data;
-  long page, slot, head;   // strides in bytes
+  uint32_t page, slot;     // strides in units of 16 bytes; no cache has 2^32 of them
+  long head;               // in bytes
   const float* scale;      // NULL: 1
   int scale_heads;         // scale holds a number for each kv head
 };
@@ -39,8 +40,8 @@ struct AttentionParams {
   uint32_t page_magic;   // key / page_size = key * page_magic >> page_shift for keys below 2^31
   int page_shift, page_size, pages, table_pages;
   int window, tree_words, tokens, seqs, heads, kv_heads, group, dim;
-  int blocks, splits, split_tiles;   // blocks of rows; at most `splits` parts of the keys, of `split_tiles` tiles at least
-  bool causal, clear_rest;
+  int rows, blocks, splits, split_tiles;   // rows of a block, blocks of rows; at most `splits` parts of the keys, of `split_tiles` tiles at least
+  bool causal, clear_rest, by_dies;
 };
 
 // Rows are pairs (token, query head of the kv head), the head fastest.  A sequence's rows start a new block.
@@ -52,28 +53,54 @@ struct RowBlock {
   int len, past;  // keys of the sequence; position of its first query
 };
 
-// The sequence of block `b`: sequence i owns the numbers from starts[i] * group / ROWS + i on, which are as many as its blocks
-// or one more.  A wavefront searches 64 places at a time.
-template <int ROWS>
-__device__ __forceinline__ RowBlock row_block(const AttentionParams& p, int b) {
+// What workgroup `b` takes: a kv head and one of `items`.  Neighbouring workgroups run on different dies (8, in turn): each die gets
+// items of its own with all their heads, one after the other.
+__device__ __forceinline__ void item_of(const AttentionParams& p, int items, int b, int& item, int& kv_head) {
+  const int whole = p.by_dies ? items / 8 * 8 : 0;
+  if (b < whole * p.kv_heads) {
+    kv_head = b / 8 % p.kv_heads, item = b / 8 / p.kv_heads * 8 + b % 8;
+  } else {
+    const int rest = b - whole * p.kv_heads;
+    kv_head = rest % p.kv_heads, item = whole + rest / p.kv_heads;
+  }
+}
+
+// The first token of sequence i, as far as there are tokens.
+__device__ __forceinline__ int start_of(const AttentionParams& p, int i) { return min(max(p.starts[i], 0), p.tokens); }
+
+// The last sequence i of [0, seqs] with number(i, its start) <= b, for numbers that rise from 0, and its sizes; its first row is left
+// to the caller.  A wavefront looks at 64 places at a time; in the last round the lanes have the sizes too, so that a batch of up
+// to 62 sequences takes one trip to memory.
+template <typename F>
+__device__ __forceinline__ RowBlock sequence_of(const AttentionParams& p, int b, F number) {
   const int lane = threadIdx.x & 63;
-  auto start = [&](int i) { return (int)min(max(p.starts[i], 0), p.tokens); };
-  auto number = [&](int i) { return (int)((long)start(i) * p.group / ROWS) + i; };
   int low = 0, count = p.seqs + 1;
-  while (count > 1) {
-    const int step = (count + 63) / 64, i = lane * step;
-    const uint64_t below = __ballot(i < count && number(low + min(i, count - 1)) <= b);
+  while (count > 63) {
+    const int step = (count + 63) / 64, i = low + min(lane * step, count - 1);
+    const uint64_t below = __ballot(lane * step < count && number(i, start_of(p, i)) <= b);
     const int last = max(__builtin_popcountll(below) - 1, 0) * step;
     low += last, count = min(step, count - last);
   }
+  const int i = low + lane;
+  const int start = i <= p.seqs ? start_of(p, i) : p.tokens, len = i < p.seqs ? p.lens[i] : 0;
+  const uint64_t below = __ballot(lane < count && number(i, start) <= b);
+  const int found = max(__builtin_popcountll(below) - 1, 0);
   RowBlock r;
-  r.seq = __builtin_amdgcn_readfirstlane(low);
-  r.token = __builtin_amdgcn_readfirstlane(start(r.seq));
-  const int end = r.seq < p.seqs ? __builtin_amdgcn_readfirstlane(start(r.seq + 1)) : p.tokens;
-  r.first = (b - __builtin_amdgcn_readfirstlane(number(r.seq))) * ROWS;
+  r.seq = low + found;
+  r.token = of_lane(start, found);
+  const int end = r.seq < p.seqs ? of_lane(start, found + 1) : p.tokens;
   r.rows = max(end - r.token, 0) * p.group;
-  r.len = r.seq < p.seqs ? (int)min((long)max(p.lens[r.seq], 0), (long)p.table_pages * p.page_size) : 0;
+  r.len = (int)min((long)max(of_lane(len, found), 0), (long)p.table_pages * p.page_size);
   r.past = r.len - (end - r.token);
+  return r;
+}
+
+// Block `b` of rows: sequence i owns the numbers from starts[i] * group / ROWS + i on, which are as many as its blocks or one more.
+template <int ROWS>
+__device__ __forceinline__ RowBlock row_block(const AttentionParams& p, int b) {
+  auto number = [&](int i, int start) { return (int)((long)start * p.group / ROWS) + i; };
+  RowBlock r = sequence_of(p, b, number);
+  r.first = (b - number(r.seq, r.token)) * ROWS;
   return r;
 }
 
@@ -111,16 +138,23 @@ struct Sight {
   }
 };
 
+// A score where bit `i` of `seen` is set, else -infinity.
+__device__ __forceinline__ float shown(float score, uint32_t seen, int i) {
+  const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, i, 1);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, score) & keep) | (__builtin_bit_cast(uint32_t, -kInfinity) & ~keep));
+}
+
 __device__ __forceinline__ int page_of(const AttentionParams& p, int key) {
   return (int)((uint64_t)(uint32_t)key * p.page_magic >> p.page_shift);
 }
 
-// The number of a page as it may be used; `bad` where the table's is none.
-__device__ __forceinline__ int page_number(const AttentionParams& p, int number, bool& bad) {
-  if ((uint32_t)number < (uint32_t)p.pages) return number;
-  bad = true;
-  return 0;
+// Where a key's row lies in a cache, in units of 16 bytes from a head's first page; `number`: its page's number, `bad` where that is none.
+__device__ __forceinline__ uint32_t place_of(const AttentionParams& p, const CachePages& c, int key, int at, int number, bool& bad) {
+  const bool known = (uint32_t)number < (uint32_t)p.pages;
+  bad |= !known;
+  return (known ? number : 0) * c.page + (key - at * p.page_size) * c.slot;
 }
+__device__ __forceinline__ const char* row_at(const char* base, uint32_t place) { return base + ((uint64_t)place << 4); }
 
 template <typename T>
 struct Element;
@@ -133,6 +167,12 @@ struct Element<__bf16> {
   }
   __device__ __forceinline__ static floatx4_t mfma16(eight a, eight b, floatx4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  typedef bf16x2_t two;
+  __device__ __forceinline__ static two pair(float a, float b) { return two{(__bf16)a, (__bf16)b}; }
+  // `to` and two numbers, added in fp32 by one instruction
+  __device__ __forceinline__ static float add(two v, float to) {
+    return __builtin_amdgcn_fdot2_f32_bf16(v, two{(__bf16)1.0f, (__bf16)1.0f}, to, false);
   }
   template <bool HIGH>
   __device__ __forceinline__ static uint32_t from_fp8(uint32_t v) {
@@ -149,6 +189,11 @@ struct Element<_Float16> {
   __device__ __forceinline__ static floatx4_t mfma16(eight a, eight b, floatx4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
+  typedef half2_t two;
+  __device__ __forceinline__ static two pair(float a, float b) { return two{(_Float16)a, (_Float16)b}; }
+  __device__ __forceinline__ static float add(two v, float to) {
+    return __builtin_amdgcn_fdot2(v, two{(_Float16)1.0f, (_Float16)1.0f}, to, false);
+  }
   template <bool HIGH>
   __device__ __forceinline__ static uint32_t from_fp8(uint32_t v) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, HIGH));
@@ -163,16 +208,17 @@ __device__ __forceinline__ u32x4_t widen(uint32_t a, uint32_t b) {
                  E::template from_fp8<true>(b)};
 }
 
-// Eight 16-bit numbers with 0 in the place of infinities and NaNs; `found` where there are some.
+// Eight 16-bit numbers with 0 in the place of infinities and NaNs; `found` is not 0 where there are some.  (An exponent of ones and
+// one more carry into the sign's place, in both halves of a word at once.)
 template <typename T>
-__device__ __forceinline__ u32x4_t finite_part(u32x4_t v, bool& found) {
-  constexpr uint32_t kLow = Element<T>::kExponent, kHigh = kLow << 16;
+__device__ __forceinline__ u32x4_t finite_part(u32x4_t v, uint32_t& found) {
+  constexpr uint32_t kOnes = Element<T>::kExponent * 0x10001u, kOne = kOnes & ~(kOnes << 1) & 0x7fff7fffu;
   u32x4_t out;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t keep = ((v[i] & kLow) == kLow ? 0 : 0xffffu) | ((v[i] & kHigh) == kHigh ? 0 : 0xffff0000u);
-    found |= keep != ~0u;
-    out[i] = v[i] & keep;
+    const uint32_t special = ((v[i] & kOnes) + kOne) & 0x80008000u;
+    found |= special;
+    out[i] = v[i] & ~((special >> 15) * 0xffffu);
   }
   return out;
 }

@@ -93,8 +93,8 @@ def test_attention_refuses(change, message):
 
 def test_caches_are_refused():
     _lib, lib = library()
-    for bad in (cache(_lib, page=2052), cache(_lib, slot=132), cache(_lib, head=68), cache(_lib, data=FAKE + 8), cache(_lib, slot=1 << 25),
-                cache(_lib, slot=-128)):
+    for bad in (cache(_lib, page=2052), cache(_lib, slot=132), cache(_lib, head=68), cache(_lib, data=FAKE + 8), cache(_lib, slot=1 << 36),
+                cache(_lib, page=1 << 36), cache(_lib, page=1 << 32), cache(_lib, slot=-128), cache(_lib, page=-2048)):
         for name in ("keys", "values"):
             assert attention_call(lib, _lib, **{name: bad}) == _lib.E_INVALID
     for bad in (cache(_lib), cache(_lib, FAKE, 3), cache(_lib, FAKE, 0), cache(_lib, FAKE, 1, slot=136)):

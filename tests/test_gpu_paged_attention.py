@@ -67,12 +67,15 @@ class Batch:
                                   self.dim ** -0.5 if scale is None else scale, causal, window, softcap,
                                   None if alibi_slopes is None else numbers(alibi_slopes), None if self.tree is None else self.tree.numpy())
 
-    def check(self, got, **more):
+    def limits(self, **more):
         want, size, most = self.want(**more)
         h, u = HALF_STEP[self.dtype], 2.0 ** -24
         e = (self.dim + 8) * u * most + 2.0 ** -22 + more.get("softcap", 0.0) * 2.0 ** -20
         keys = max([n for n, _ in self.lengths] + [1])
-        limit = size * (h + 2 * e[:, :, None] + keys * u) + np.abs(want) * h + 2.0 ** -24
+        return want, size * (h + 2 * e[:, :, None] + keys * u) + np.abs(want) * h + 2.0 ** -24
+
+    def check(self, got, **more):
+        want, limit = self.limits(**more)
         off = np.abs(numbers(got) - want)
         assert got.dtype == DTYPES[self.dtype] and (off <= limit).all(), (off.max(), (off / limit).max(), np.argwhere(~(off <= limit))[:5])
 
