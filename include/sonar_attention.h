@@ -80,7 +80,7 @@ int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  *               time need scratches of their own
  * head_dim a multiple of 16, at most 256; scale > 0; tokens * heads below 2^31, table_pages * page_size below 2^31 - 1024. */
 size_t sonar_paged_attention_scratch_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                           int64_t max_seq_len, int64_t window);
+                                           int cache_dtype, int64_t max_seq_len, int64_t window);
 int sonar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const sonar_kv_cache* key_cache,
                           const sonar_kv_cache* value_cache, int cache_dtype, int64_t pages, int64_t page_size,
                           const int32_t* block_table, int64_t table_stride, int64_t table_pages, const int32_t* seq_lens,

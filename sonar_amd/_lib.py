@@ -150,7 +150,7 @@ ATTENTION_PROTOTYPES = {
     "sonar_qk_norm_rope": (c_int, [c_void_p, c_int64, c_int64] * 3 + [c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_void_p,
                                    c_void_p, c_double, c_void_p, c_void_p, POINTER(KvCache), POINTER(KvCache), c_int, c_void_p, c_int,
                                    c_int64, c_int64, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p]),
-    "sonar_paged_attention_scratch_bytes": (c_size_t, [c_int64] * 7),
+    "sonar_paged_attention_scratch_bytes": (c_size_t, [c_int64] * 5 + [c_int] + [c_int64] * 2),
     "sonar_paged_attention": (c_int, [c_void_p, c_int64, c_int64, POINTER(KvCache), POINTER(KvCache), c_int, c_int64, c_int64, c_void_p,
                                       c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_double, c_double,
                                       c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_int, c_int64, c_int64, c_int64,

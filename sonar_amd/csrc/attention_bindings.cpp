@@ -203,7 +203,7 @@ void attend(const Tensor& query, const Tensor& key_cache, const Tensor& value_ca
   const Tensor tree = tree_mask.has_value() ? tree_mask->contiguous() : Tensor();
   const int64_t table_pages = table.size(1), table_stride = seqs > 1 ? table.stride(0) : table_pages;
   const int64_t longest = max_seq_len.has_value() ? *max_seq_len : table_pages * page_size;
-  const size_t scratch_bytes = sonar_paged_attention_scratch_bytes(tokens, seqs, heads, kv_heads, dim, longest, window);
+  const size_t scratch_bytes = sonar_paged_attention_scratch_bytes(tokens, seqs, heads, kv_heads, dim, cache_code(key_cache, dtype), longest, window);
   Tensor scratch;
   if (scratch_bytes > 0) scratch = new_tensor(query, {(int64_t)scratch_bytes}, at::kByte);
   raise_if_failed(sonar_paged_attention(

@@ -18,22 +18,22 @@ namespace {
 
 constexpr int kTile = 64;   // keys
 
-// What turns a score q . k into a power of two, for the forms with a cap or slopes.
+// What turns a score q . k into a power of two: s * by, or capped cap * tanh of it as cap - 2 cap / (1 + e^2x); less the slope's part.
+enum Scores { kPlain, kCapped, kSloped };   // (sloped ones may be capped too)
 struct Score {
-  float by, cap, slope;   // plain: s * by; capped: cap * tanh of it
-  bool capped;
-  __device__ __forceinline__ float of(float s, float distance) const {
-    if (capped) s = cap - 2.0f * cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * by));
-    else s *= by;
-    return __builtin_fmaf(-slope, fabsf(distance), s);
+  float by, cap, slope;
+  bool is_capped;
+  __device__ __forceinline__ float capped(float s) const {
+    return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * by)), cap);
   }
+  __device__ __forceinline__ float sloped(float s, float distance) const { return __builtin_fmaf(-slope, fabsf(distance), s); }
 };
 
 __device__ __forceinline__ Score score_of(const AttentionParams& p, int kv_head, int head) {
   const float k_scale = p.k.scale == nullptr ? 1.0f : p.k.scale[p.k.scale_heads ? kv_head : 0];
   Score s;
-  s.capped = p.cap > 0.0f;
-  s.by = s.capped ? 2.0f * kLog2E * p.scale * k_scale / p.cap : p.scale * k_scale * kLog2E;
+  s.is_capped = p.cap > 0.0f;
+  s.by = s.is_capped ? 2.0f * kLog2E * p.scale * k_scale / p.cap : p.scale * k_scale * kLog2E;
   s.cap = p.cap * kLog2E;
   s.slope = p.slopes == nullptr ? 0.0f : p.slopes[head] * kLog2E;
   return s;
@@ -100,7 +100,7 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
 // the row's number, so that the lanes which read at once find different banks: 16 lanes a piece of a row each of the keys, 32 lanes
 // four pieces of four rows of the values.
 template <int DP>
-__device__ __forceinline__ int key_swap(int row) { return DP == 64 ? row >> 1 & 7 : DP == 128 ? row & 15 : row & 7; }
+__device__ __forceinline__ int key_swap(int row) { return DP == 64 ? row >> 1 & 7 : row & 15; }
 template <int DP>
 __device__ __forceinline__ int value_swap(int row) { return DP == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4; }
 template <int DP>
@@ -114,7 +114,7 @@ __device__ __forceinline__ void copy_16_to_lds(uint32_t lds, const char* from) {
 }
 #pragma clang diagnostic pop
 
-template <typename T, int DP, bool FP8, bool EXTRA, int WAVES>
+template <typename T, int DP, bool FP8, int SCORES, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 1) void attention_rows_kernel(const AttentionParams p) {
   typedef Element<T> E;
   typedef typename E::eight eight;
@@ -141,9 +141,9 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   const long token = r.token + t;
   const int wave_t0 = min(r.first + wave * 32, r.rows - 1) / p.group, wave_t1 = min(r.first + wave * 32 + 31, r.rows - 1) / p.group;
   const int block_t0 = r.first / p.group, block_t1 = min(r.first + kRows - 1, r.rows - 1) / p.group;
-  int low, high, wave_low, wave_high;
+  const bool busy = r.first + wave * 32 < r.rows;   // (else the wavefront only copies)
+  int low, high;
   keys_seen(p, r, block_t0, block_t1, low, high);
-  keys_seen(p, r, wave_t0, wave_t1, wave_low, wave_high);
   int tile = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
   if (!split_of(p, split, tile, last, parts)) return;
   const int first_tile = tile;
@@ -176,13 +176,15 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   uint32_t places = 0;       // of its values
   uint32_t k_rows[kPasses], v_rows[kPasses];   // the places of the rows that this lane copies
   u32x4_t k_next[FP8 ? kPasses : 1], v_next[FP8 ? kPasses : 1];
-  const int of_group = lane / kLanes, my_row_of_16 = wave * kGroup + of_group;   // (passes are multiples of 16 rows apart, of 8 in the widest form)
+  const int of_group = lane / kLanes, my_row_of_16 = wave * kGroup + of_group;   // (passes are 16 rows apart or more, but 8 in the widest form)
   const int k_chunk = FP8 ? lane % kLanes : lane % kLanes ^ key_swap<DP>(my_row_of_16);
   const int v_chunk = FP8 ? lane % kLanes : lane % kLanes ^ value_swap<DP>(my_row_of_16);
-  const bool has_k = k_chunk * (FP8 ? 16 : 8) < p.dim, has_v = v_chunk * (FP8 ? 16 : 8) < p.dim;
+  constexpr bool kOdd = WAVES * kGroup == 8;   // every other pass is swapped by 8 pieces more
+  const bool has_k = k_chunk * (FP8 ? 16 : 8) < p.dim, has_odd = (k_chunk ^ 8) * 8 < p.dim, has_v = v_chunk * (FP8 ? 16 : 8) < p.dim;
   const bool alike = p.k.page == p.v.page && p.k.slot == p.v.slot;
   const char* const k_base = p.k.data + kv_head * p.k.head + k_chunk * 16;
   const char* const v_base = p.v.data + kv_head * p.v.head + v_chunk * 16;
+  const char* const k_odd = p.k.data + kv_head * p.k.head + (k_chunk ^ 8) * 16;
   const uint32_t k_lds = (uint32_t)(uintptr_t)(lds_void_t*)k_tiles + wave * 1024, v_lds = (uint32_t)(uintptr_t)(lds_void_t*)v_tiles + wave * 1024;
   const int32_t* const pages = p.table + (long)min(r.seq, p.seqs - 1) * p.table_stride;
   auto key_of = [&](int of_tile) { return min(max(of_tile * kTile + lane, low), high - 1); };
@@ -198,14 +200,19 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     places = alike ? of_keys : place_of(p, p.v, key, at, page_ahead, bad);
     spread(k_rows, of_keys);
   };
-  auto fetch = [&](u32x4_t* to, const char* base, const uint32_t (&rows)[kPasses], bool has, uint32_t at) {
+  auto fetch = [&](u32x4_t* to, const char* base, const uint32_t (&rows)[kPasses], bool has, uint32_t at, int first, int step) {
     if (!has) return;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
+    for (int i = first; i < kPasses; i += step) {
       if constexpr (FP8) to[i] = *reinterpret_cast<const u32x4_t*>(row_at(base, rows[i]));
       else copy_16_to_lds(__builtin_amdgcn_readfirstlane(at + i * (WAVES * 1024)), row_at(base, rows[i]));
     }
   };
+  auto fetch_keys = [&](uint32_t at) {
+    fetch(k_next, k_base, k_rows, has_k, at, 0, kOdd ? 2 : 1);
+    if constexpr (kOdd) fetch(k_next, k_odd, k_rows, has_odd, at, 1, 2);
+  };
+  auto fetch_values = [&](uint32_t at) { fetch(v_next, v_base, v_rows, has_v, at, 0, 1); };
   uint32_t specials = 0;   // infinities and NaNs of v were left out of a tile that is masked for some query
   // What was fetched is in LDS when this ends, as far as this wavefront fetched it.
   auto keep = [&](char* to_k, char* to_v, bool sift) {
@@ -269,13 +276,21 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     const int base = of_tile * kTile + 32 * h;
 #pragma unroll
     for (int n = 0; n < 2; ++n) read_values(v_from, h ^ 1, n), read_keys(k_from, h ^ 1, n);
-    if (EXTRA) {
+    const bool masked = base < wave_full_low || base + 32 > wave_full_high;
+    uint32_t seen = ~0u;
+    if (masked) seen = (uint32_t)(sight.of(base) >> 4 * half);
+    if (SCORES == kSloped) {
       const float distance = (float)(sight.position - base - 4 * half);
+      if (score.is_capped) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[h][i] = score.of(s[h][i], distance - (float)(8 * (i / 4) + i % 4));
+        for (int i = 0; i < 16; ++i) s[h][i] = score.capped(s[h][i]);
+      } else {
+        s[h] *= score.by;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[h][i] = score.sloped(s[h][i], distance - (float)(8 * (i / 4) + i % 4));
     }
-    if (base < wave_full_low || base + 32 > wave_full_high) {
-      const uint32_t seen = (uint32_t)(sight.of(base) >> 4 * half);
+    if (SCORES != kCapped && masked) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[h][i] = shown(s[h][i], seen, 8 * (i / 4) + i % 4);
     }
@@ -295,9 +310,12 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
       }
       if (i < kTops) {
 #pragma unroll
-        for (int e = 16 * i / kTops; e < 16 * (i + 1) / kTops; ++e) top = fmaxf(top, s[h][e]);
+        for (int e = 16 * i / kTops; e < 16 * (i + 1) / kTops; ++e) {
+          if (SCORES == kCapped) s[h][e] = shown(score.capped(s[h][e]), seen, 8 * (e / 4) + e % 4);
+          top = fmaxf(top, s[h][e]);
+        }
       } else if (i == kTops) {
-        if (!EXTRA) top *= score.by;
+        if (SCORES == kPlain) top *= score.by;
         rises = __any(top > most + 8.0f);
         const float old = most, higher = fmaxf(old, joined<true>(top, [](float a, float b) { return fmaxf(a, b); }));
         most = rises ? higher : old;
@@ -312,7 +330,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float x = s[h][2 * pair + e];
-            w[e] = __builtin_amdgcn_exp2f(EXTRA ? x - less : __builtin_fmaf(x, score.by, -less));
+            w[e] = __builtin_amdgcn_exp2f(SCORES == kPlain ? __builtin_fmaf(x, score.by, -less) : x - less);
           }
           auto both = E::pair(w[0], w[1]);
           asm volatile("" : "+v"(both));   // (or the weights would be formed where they are used, behind the products)
@@ -337,7 +355,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     look_up(tile);
     find(tile);
     look_up(tile + 1);
-    fetch(k_next, k_base, k_rows, has_k, k_lds);
+    fetch_keys(k_lds);
 #pragma unroll
     for (int i = 0; i < 2; ++i) weights[1][i] = eight{};
     for (int i = threadIdx.x * 16; i < kTileBytes; i += WAVES * 64 * 16) *reinterpret_cast<u32x4_t*>(v_tiles + kTileBytes + i) = u32x4_t{};
@@ -356,8 +374,8 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     }
     __syncthreads();
     find(tile + 1);
-    fetch(v_next, v_base, v_rows, has_v, v_lds);
-    fetch(k_next, k_base, k_rows, has_k, k_lds + kTileBytes);
+    fetch_values(v_lds);
+    fetch_keys(k_lds + kTileBytes);
     look_up(tile + 2);
     s[0] = floatx16_t{};
 #pragma unroll
@@ -369,14 +387,14 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     for (; tile < last; ++tile, buffer ^= kTileBytes) {
       char *const k_here = k_tiles + buffer, *const v_here = v_tiles + buffer;
       char *const k_there = k_tiles + (buffer ^ kTileBytes), *const v_there = v_tiles + (buffer ^ kTileBytes);
-      step(tile, std::integral_constant<int, 0>{}, k_here, v_there);
+      if (busy) step(tile, std::integral_constant<int, 0>{}, k_here, v_there);
       find(tile + 2);
       keep(k_there, v_here, tile * kTile < block_full_low || tile * kTile + kTile > block_full_high);
       __syncthreads();
-      fetch(v_next, v_base, v_rows, has_v, v_lds + (buffer ^ kTileBytes));
-      fetch(k_next, k_base, k_rows, has_k, k_lds + buffer);
+      fetch_values(v_lds + (buffer ^ kTileBytes));
+      fetch_keys(k_lds + buffer);
       look_up(tile + 3);
-      step(tile, std::integral_constant<int, 1>{}, k_there, v_here);
+      if (busy) step(tile, std::integral_constant<int, 1>{}, k_there, v_here);
     }
 #pragma unroll
     for (int n = 0; n < 2 * kColumns; ++n) {
@@ -423,21 +441,21 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
 }
 
 // ---------------------------------------------------------------- few rows
-// A workgroup takes 16 * TILES rows of a kv head, and its wavefronts take 32 keys in turn, each with a maximum, a sum and an output
+// A workgroup takes 16 rows of a kv head, and its wavefronts take 32 keys in turn, each with a maximum, a sum and an output
 // of its own, which are joined at the end.  Keys go from memory straight into the registers of the product, values through a piece
 // of LDS that is the wavefront's own, to be turned there: no wavefront waits for another until the end.
-constexpr int kWaves = 4;    // of a workgroup
+constexpr int kFew = 4;      // wavefronts of a workgroup
 constexpr int kUnit = 32;    // keys that a wavefront takes at once
 
 template <int DP>
 constexpr int pitch() { return DP * 2 + 32; }   // bytes of a row there: 8 neighbouring rows start at banks of their own
 template <int DP>
-constexpr int few_lds() { return kWaves * kUnit * pitch<DP>() + kWaves * 16 * 8 + 16; }
+constexpr int few_lds() { return kFew * kUnit * pitch<DP>() + kFew * 16 * 8 + 16; }
 
-constexpr int few_waves(int dp, int tiles) { return dp == 64 ? 5 - tiles : dp == 128 ? 4 - tiles : 3 - tiles; }   // a SIMD
+constexpr int few_waves(int dp, bool fp8) { return dp == 64 ? 4 : dp == 128 ? 3 : fp8 ? 2 : 1; }   // a SIMD
 
-template <typename T, int DP, bool FP8, bool EXTRA, int TILES>
-__global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_few_kernel(const AttentionParams p) {
+template <typename T, int DP, bool FP8, int SCORES>
+__global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_kernel(const AttentionParams p) {
   typedef Element<T> E;
   typedef typename E::eight eight;
   constexpr int kSteps = DP / 32, kColumns = DP / 16, kPitch = pitch<DP>(), kLoads = FP8 ? DP / 64 : DP / 32;
@@ -445,15 +463,15 @@ __global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_f
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int column = lane & 15, quarter = lane >> 4;
   char* const mine = lds + wave * kUnit * kPitch;
-  float2* const sums = (float2*)(lds + kWaves * kUnit * kPitch);   // [kWaves][16]
-  int* const flags = (int*)(sums + kWaves * 16);
+  float2* const sums = (float2*)(lds + kFew * kUnit * kPitch);   // [kFew][16]
+  int* const flags = (int*)(sums + kFew * 16);
 
   int item, kv_head;
   item_of(p, p.blocks * p.splits, blockIdx.x, item, kv_head);
   const int split = item / p.blocks;
-  const RowBlock r = row_block<16 * TILES>(p, item % p.blocks);
+  const RowBlock r = row_block<16>(p, item % p.blocks);
   if (r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;
-  const int block_t0 = r.first / p.group, block_t1 = min(r.first + 16 * TILES - 1, r.rows - 1) / p.group;
+  const int block_t0 = r.first / p.group, block_t1 = min(r.first + 16 - 1, r.rows - 1) / p.group;
   int low, high;
   keys_seen(p, r, block_t0, block_t1, low, high);
   int first_tile = low / kTile, last_tile = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
@@ -462,22 +480,19 @@ __global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_f
   const int full_low = bounded && p.window > 0 ? max(r.past + block_t1 - p.window + 1, 0) : 0;
   const int full_high = p.tree != nullptr ? min(r.len, r.past) : bounded ? min(r.len, r.past + block_t0 + 1) : r.len;
 
-  Sight sight[TILES];
-  Score score[TILES];
-  eight q[TILES][kSteps];
-#pragma unroll
-  for (int n = 0; n < TILES; ++n) {
-    const int row = min(r.first + 16 * n + column, r.rows - 1), t = row / p.group, head = kv_head * p.group + row % p.group;
-    const long token = r.token + t;
-    sight[n] = Sight{r.past + t, r.len, r.past, bounded && p.window > 0 ? r.past + t - p.window + 1 : 0,
-                     p.tree == nullptr ? nullptr : p.tree + token * p.tree_words, p.tree_words, p.causal};
-    score[n] = score_of(p, kv_head, head);
-    const T* from = (const T*)p.q + token * p.q_token + head * p.q_head;
+  const int my_row = min(r.first + column, r.rows - 1), t = my_row / p.group, head = kv_head * p.group + my_row % p.group;
+  const long my_token = r.token + t;
+  const Sight sight{r.past + t, r.len, r.past, bounded && p.window > 0 ? r.past + t - p.window + 1 : 0,
+                    p.tree == nullptr ? nullptr : p.tree + my_token * p.tree_words, p.tree_words, p.causal};
+  const Score score = score_of(p, kv_head, head);
+  eight q[kSteps];
+  {
+    const T* from = (const T*)p.q + my_token * p.q_token + head * p.q_head;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {   // of an 8-bit cache a lane holds 16 neighbouring numbers of a key, for two steps
       const int d = FP8 ? 64 * (s / 2) + 16 * quarter + 8 * (s % 2) : 32 * s + 8 * quarter;
-      q[n][s] = eight{};
-      if (d < p.dim) q[n][s] = *reinterpret_cast<const eight*>(from + d);
+      q[s] = eight{};
+      if (d < p.dim) q[s] = *reinterpret_cast<const eight*>(from + d);
     }
   }
 
@@ -510,22 +525,18 @@ __global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_f
     }
   };
 
-  floatx4_t out[kColumns][TILES];
-  float most[TILES], sum[TILES];
+  floatx4_t out[kColumns];
 #pragma unroll
-  for (int n = 0; n < TILES; ++n) {
-    most[n] = -kInfinity, sum[n] = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kColumns; ++c) out[c][n] = floatx4_t{};
-  }
+  for (int c = 0; c < kColumns; ++c) out[c] = floatx4_t{};
+  float most = -kInfinity, sum = 0.0f;
   int unit = 2 * first_tile + wave;
   const int last = min(2 * last_tile, (high + kUnit - 1) / kUnit);
   if (unit < last) {
     look_up(unit);
     fetch(unit);
-    if (unit + kWaves < last) look_up(unit + kWaves);
+    if (unit + kFew < last) look_up(unit + kFew);
   }
-  for (; unit < last; unit += kWaves) {
+  for (; unit < last; unit += kFew) {
     const int base = unit * kUnit;
     const bool masked = base < full_low || base + kUnit > full_high;
 #pragma unroll
@@ -544,57 +555,59 @@ __global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_f
         *reinterpret_cast<u32x4_t*>(to) = v0;
       }
     // scores of 32 keys: lane l has those of query l % 16 with the keys 16 a + 4 (l / 16) + i
-    floatx4_t s[2][TILES];
+    floatx4_t s[2];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < 2; ++a) {
+      s[a] = floatx4_t{};
 #pragma unroll
-      for (int n = 0; n < TILES; ++n) {
-        s[a][n] = floatx4_t{};
-#pragma unroll
-        for (int d = 0; d < kSteps; ++d) {
-          u32x4_t piece;
-          if constexpr (FP8) piece = d % 2 == 0 ? widen<T>(k[a][d / 2][0], k[a][d / 2][1]) : widen<T>(k[a][d / 2][2], k[a][d / 2][3]);
-          else piece = k[a][d];
-          s[a][n] = E::mfma16(__builtin_bit_cast(eight, piece), q[n][d], s[a][n]);
-        }
+      for (int d = 0; d < kSteps; ++d) {
+        u32x4_t piece;
+        if constexpr (FP8) piece = d % 2 == 0 ? widen<T>(k[a][d / 2][0], k[a][d / 2][1]) : widen<T>(k[a][d / 2][2], k[a][d / 2][3]);
+        else piece = k[a][d];
+        s[a] = E::mfma16(__builtin_bit_cast(eight, piece), q[d], s[a]);
       }
-    if (unit + kWaves < last) {
-      fetch(unit + kWaves);
-      if (unit + 2 * kWaves < last) look_up(unit + 2 * kWaves);
     }
-    eight weights[TILES];
+    if (unit + kFew < last) {
+      fetch(unit + kFew);
+      if (unit + 2 * kFew < last) look_up(unit + 2 * kFew);
+    }
+    eight weights;
+    if (SCORES == kCapped || (SCORES == kSloped && score.is_capped)) {
 #pragma unroll
-    for (int n = 0; n < TILES; ++n) {
-      if (EXTRA) {
-        const float distance = (float)(sight[n].position - base - 4 * quarter);
+      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = score.capped(s[i / 4][i % 4]);
+    } else if (SCORES == kSloped) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i / 4][n][i % 4] = score[n].of(s[i / 4][n][i % 4], distance - (float)(16 * (i / 4) + i % 4));
-      }
-      if (masked) {
-        const uint32_t seen = (uint32_t)(sight[n].of(base) >> 4 * quarter);
+      for (int a = 0; a < 2; ++a) s[a] *= score.by;
+    }
+    if (SCORES == kSloped) {
+      const float distance = (float)(sight.position - base - 4 * quarter);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[i / 4][n][i % 4] = shown(s[i / 4][n][i % 4], seen, 16 * (i / 4) + i % 4);
-      }
-      float top = s[0][n][0];
+      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = score.sloped(s[i / 4][i % 4], distance - (float)(16 * (i / 4) + i % 4));
+    }
+    if (masked) {
+      const uint32_t seen = (uint32_t)(sight.of(base) >> 4 * quarter);
 #pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][n][i % 4]);
-      if (!EXTRA) top *= score[n].by;
-      if (__any(top > most[n] + 8.0f)) {
-        auto larger = [](float a, float b) { return fmaxf(a, b); };
-        const float now = fmaxf(most[n], joined<true>(joined<false>(top, larger), larger));
-        const float by = now == -kInfinity ? 1.0f : __builtin_amdgcn_exp2f(most[n] - now);
-        most[n] = now, sum[n] *= by;
+      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = shown(s[i / 4][i % 4], seen, 16 * (i / 4) + i % 4);
+    }
+    float top = s[0][0];
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) out[c][n] *= by;
-      }
-      const float less = most[n] == -kInfinity ? 0.0f : most[n];
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i / 4][i % 4]);
+    if (SCORES == kPlain) top *= score.by;
+    if (__any(top > most + 8.0f)) {
+      auto larger = [](float a, float b) { return fmaxf(a, b); };
+      const float now = fmaxf(most, joined<true>(joined<false>(top, larger), larger));
+      const float by = now == -kInfinity ? 1.0f : __builtin_amdgcn_exp2f(most - now);
+      most = now, sum *= by;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = s[i / 4][n][i % 4];
-        const float w = __builtin_amdgcn_exp2f(EXTRA ? x - less : __builtin_fmaf(x, score[n].by, -less));
-        sum[n] += w;
-        weights[n][i] = (T)w;
-      }
+      for (int c = 0; c < kColumns; ++c) out[c] *= by;
+    }
+    const float less = most == -kInfinity ? 0.0f : most;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = s[i / 4][i % 4];
+      const float w = __builtin_amdgcn_exp2f(SCORES == kPlain ? __builtin_fmaf(x, score.by, -less) : x - less);
+      sum += w;
+      weights[i] = (T)w;
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");   // (what other lanes wrote is read)
     __builtin_amdgcn_wave_barrier();
@@ -603,79 +616,85 @@ __global__ __launch_bounds__(kWaves * 64, few_waves(DP, TILES)) void attention_f
 #pragma unroll
     for (int c = 0; c < kColumns; ++c) {
       const short4_t a = turned(from + 32 * c), b = turned(from + 16 * kPitch + 32 * c);
-      const eight piece = __builtin_bit_cast(eight, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int n = 0; n < TILES; ++n) out[c][n] = E::mfma16(piece, weights[n], out[c][n]);
+      out[c] = E::mfma16(__builtin_bit_cast(eight, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)), weights, out[c]);
     }
     __builtin_amdgcn_wave_barrier();
   }
 
-  // ---- the wavefronts' results joined, 16 rows at a time: a row's numbers 4 (DP + 4) bytes apart
+  // ---- the wavefronts' results joined: a row's numbers 4 (DP + 4) bytes apart
   if (threadIdx.x == 0) flags[0] = 0;
   __syncthreads();
   if (bad) atomicOr(flags, 1);
   if (specials) atomicOr(flags, 2);
   constexpr int kOut = 4 * DP + 16;
-  const float v_scale = value_scale(p, kv_head);
+  auto add = [](float a, float b) { return a + b; };
+  sum = joined<true>(joined<false>(sum, add), add);
+  if (quarter == 0) sums[wave * 16 + column] = make_float2(most, sum);
 #pragma unroll
-  for (int n = 0; n < TILES; ++n) {
-    auto add = [](float a, float b) { return a + b; };
-    sum[n] = joined<true>(joined<false>(sum[n], add), add);
-    if (quarter == 0) sums[wave * 16 + column] = make_float2(most[n], sum[n]);
+  for (int c = 0; c < kColumns; ++c) *reinterpret_cast<floatx4_t*>(mine + column * kOut + 64 * c + 16 * quarter) = out[c];
+  __syncthreads();
+  const int in_tile = threadIdx.x / 16, row = r.first + in_tile;
+  if (row < r.rows) {
+    const long token = r.token + row / p.group;
+    const int head = kv_head * p.group + row % p.group;
+    float all = -kInfinity, total = 0.0f, by[kFew];
 #pragma unroll
-    for (int c = 0; c < kColumns; ++c) *reinterpret_cast<floatx4_t*>(mine + column * kOut + 64 * c + 16 * quarter) = out[c][n];
-    __syncthreads();
-    const int in_tile = threadIdx.x / 16, row = r.first + 16 * n + in_tile;
-    if (row < r.rows) {
-      const long token = r.token + row / p.group;
-      const int head = kv_head * p.group + row % p.group;
-      float all = -kInfinity, total = 0.0f, by[kWaves];
+    for (int w = 0; w < kFew; ++w) all = fmaxf(all, sums[w * 16 + in_tile].x);
+    const float less = all == -kInfinity ? 0.0f : all;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) all = fmaxf(all, sums[w * 16 + in_tile].x);
-      const float less = all == -kInfinity ? 0.0f : all;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        by[w] = __builtin_amdgcn_exp2f(sums[w * 16 + in_tile].x - less);
-        total = __builtin_fmaf(by[w], sums[w * 16 + in_tile].y, total);
-      }
-      if (flags[0] & 1) total = __builtin_nanf("");
-      const long at = ((long)split * p.tokens + token) * p.heads + head;
-      if (parts > 1 && threadIdx.x % 16 == 0) p.part_ml[at] = make_float2(all, total);
-      const float scale = total == 0.0f ? 0.0f : v_scale / total;
-#pragma unroll
-      for (int j = 0; j < DP / 64; ++j) {
-        const int d = 64 * j + 4 * (threadIdx.x % 16);
-        if (d >= p.dim) continue;
-        floatx4_t o{};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const floatx4_t x = *reinterpret_cast<const floatx4_t*>(lds + w * kUnit * kPitch + in_tile * kOut + 4 * d);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by[w], x[e], o[e]);
-        }
-        if (parts > 1) *reinterpret_cast<floatx4_t*>(p.part_o + at * p.dim + d) = o;
-        else *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + d) =
-            four<T>(o[0] * scale, o[1] * scale, o[2] * scale, o[3] * scale);
-      }
+    for (int w = 0; w < kFew; ++w) {
+      by[w] = __builtin_amdgcn_exp2f(sums[w * 16 + in_tile].x - less);
+      total = __builtin_fmaf(by[w], sums[w * 16 + in_tile].y, total);
     }
-    __syncthreads();
+    if (flags[0] & 1) total = __builtin_nanf("");
+    const long at = ((long)split * p.tokens + token) * p.heads + head;
+    if (parts > 1 && threadIdx.x % 16 == 0) p.part_ml[at] = make_float2(all, total);
+    const float scale = total == 0.0f ? 0.0f : value_scale(p, kv_head) / total;
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+      const int d = 64 * j + 4 * (threadIdx.x % 16);
+      if (d >= p.dim) continue;
+      floatx4_t o{};
+#pragma unroll
+      for (int w = 0; w < kFew; ++w) {
+        const floatx4_t x = *reinterpret_cast<const floatx4_t*>(lds + w * kUnit * kPitch + in_tile * kOut + 4 * d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by[w], x[e], o[e]);
+      }
+      if (parts > 1) *reinterpret_cast<floatx4_t*>(p.part_o + at * p.dim + d) = o;
+      else *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + d) =
+          four<T>(o[0] * scale, o[1] * scale, o[2] * scale, o[3] * scale);
+    }
   }
   if (flags[0] & 2)
-    add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last_tile, min(r.rows, r.first + 16 * TILES), full_low, full_high);
+    add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last_tile, min(r.rows, r.first + 16), full_low, full_high);
 }
 
 // ---------------------------------------------------------------- the parts of a split joined
-// out = sum over the parts of 2^(m_i - m) o_i, divided by that of their sums.  A wavefront (WIDE: a workgroup) a row; 4 numbers of it
-// a lane, LANES = dim / 4 rounded up, so that 64 / LANES parts are read at once by a wavefront.
-template <typename T, int LANES, bool WIDE>
-__global__ __launch_bounds__(256) void attention_join_kernel(const AttentionParams p) {
-  constexpr int kAtOnce = 64 / LANES, kStep = WIDE ? 4 * kAtOnce : kAtOnce;
-  __shared__ float4 numbers[WIDE ? 4 : 1][64];
-  __shared__ float totals[WIDE ? 4 : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long at = (long)blockIdx.x * (WIDE ? 1 : 4) + (WIDE ? 0 : wave);
-  if (at >= (long)p.tokens * p.heads) return;
-  const int token = at / p.heads, head = at % p.heads, kv_head = head / p.group;
+// out = sum over the parts of 2^(m_i - m) o_i, divided by that of their sums, with a running maximum m for each group of lanes.  WAVES
+// wavefronts a row (1: four rows a workgroup); LANES lanes hold a row's numbers, four each, so that a wavefront reads 64 / LANES
+// parts at once.  The first parts are read before it is known how many there are: one trip to memory less.
+template <typename T, int LANES, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_kernel(const AttentionParams p) {
+  constexpr int kAtOnce = 64 / LANES, kStep = WAVES * kAtOnce, kBatch = 4;
+  __shared__ float4 numbers[WAVES][LANES];
+  __shared__ float2 sums[WAVES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = lane % LANES * 4;
+  const long row = WAVES == 1 ? (long)blockIdx.x * 4 + wave : (long)blockIdx.x, step = (long)p.tokens * p.heads;
+  if (row >= step) return;
+  float2 ml[kBatch];
+  floatx4_t o[kBatch];
+  auto load = [&](int first, int end) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int s = min(first + i * kStep, end - 1);
+      ml[i] = p.part_ml[row + s * step];
+      if (d < p.dim) o[i] = *reinterpret_cast<const floatx4_t*>(p.part_o + (row + s * step) * p.dim + d);
+    }
+  };
+  int s = (WAVES == 1 ? 0 : wave * kAtOnce) + lane / LANES;
+  load(s, p.splits);
+  const int token = row / p.heads, head = row % p.heads, kv_head = head / p.group;
   RowBlock r = sequence_of(p, token, [](int, int start) { return start; });
   if (r.seq == p.seqs || token < r.token) return;
   r.first = ((token - r.token) * p.group + head % p.group) / p.rows * p.rows;
@@ -684,26 +703,40 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
   int first = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
   split_of(p, 0, first, last, parts);
   if (parts <= 1) return;
-  const long step = (long)p.tokens * p.heads;
-  auto larger = [](float a, float b) { return fmaxf(a, b); };
-  float most = -kInfinity;
-  for (int s = lane; s < parts; s += 64) most = fmaxf(most, p.part_ml[at + s * step].x);
-  most = over_wave(most, -kInfinity, larger);
-  const float less = most == -kInfinity ? 0.0f : most;
-  float sum = 0.0f, out[4] = {};
-  const int d = lane % LANES * 4;
-#pragma unroll 4
-  for (int s = (WIDE ? wave * kAtOnce : 0) + lane / LANES; s < parts; s += kStep) {
-    const float2 ml = p.part_ml[at + s * step];
-    const float by = __builtin_amdgcn_exp2f(ml.x - less);
-    sum = __builtin_fmaf(by, ml.y, sum);
-    if (d < p.dim) {
-      const floatx4_t o = *reinterpret_cast<const floatx4_t*>(p.part_o + (at + s * step) * p.dim + d);
+  float most = -kInfinity, sum = 0.0f;
+  floatx4_t out{};
+  // (to the powers of two of another maximum; both -infinity where there is nothing yet)
+  auto shrink = [](float from, float to) { return to == -kInfinity ? 1.0f : __builtin_amdgcn_exp2f(from - to); };
+  for (;;) {
+    float top = most;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(by, o[e], out[e]);
-    }
+    for (int i = 0; i < kBatch; ++i) top = s + i * kStep < parts ? fmaxf(top, ml[i].x) : top;
+    const float by = shrink(most, top);
+    most = top, sum *= by;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] *= by;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (s + i * kStep < parts) {
+        const float w = shrink(ml[i].x, top);
+        sum = __builtin_fmaf(w, ml[i].y, sum);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = __builtin_fmaf(w, o[i][e], out[e]);
+      }
+    s += kBatch * kStep;
+    if (__all(s >= parts)) break;
+    load(s, parts);
   }
+  // the groups of lanes, then the wavefronts
+  auto larger = [](float a, float b) { return fmaxf(a, b); };
   auto add = [](float a, float b) { return a + b; };
+  float top = most;
+  if (LANES <= 16) top = joined<false>(top, larger);
+  if (LANES <= 32) top = joined<true>(top, larger);
+  const float by = shrink(most, top);
+  sum *= by;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] *= by;
   if (LANES <= 16) {
     sum = joined<false>(sum, add);
 #pragma unroll
@@ -714,21 +747,28 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
 #pragma unroll
     for (int e = 0; e < 4; ++e) out[e] = joined<true>(out[e], add);
   }
-  if (WIDE) {
-    numbers[wave][lane] = make_float4(out[0], out[1], out[2], out[3]);
-    if (lane == 0) totals[wave] = sum;
+  if (WAVES > 1) {
+    if (lane < LANES) numbers[wave][lane] = make_float4(out[0], out[1], out[2], out[3]);
+    if (lane == 0) sums[wave] = make_float2(top, sum);
     __syncthreads();
     if (wave != 0) return;
+    most = -kInfinity;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const float4 x = numbers[w][lane];
-      out[0] += x.x, out[1] += x.y, out[2] += x.z, out[3] += x.w, sum += totals[w];
+    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, sums[w].x);
+    out = floatx4_t{}, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float4 x = numbers[w][lane % LANES];
+      const float by = shrink(sums[w].x, most);
+      sum = __builtin_fmaf(by, sums[w].y, sum);
+      out[0] = __builtin_fmaf(by, x.x, out[0]), out[1] = __builtin_fmaf(by, x.y, out[1]);
+      out[2] = __builtin_fmaf(by, x.z, out[2]), out[3] = __builtin_fmaf(by, x.w, out[3]);
     }
   }
   if (lane >= LANES || d >= p.dim) return;
-  const float by = sum == 0.0f ? 0.0f : value_scale(p, kv_head) / sum;
+  const float scale = sum == 0.0f ? 0.0f : value_scale(p, kv_head) / sum;
   *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + d) =
-      four<T>(out[0] * by, out[1] * by, out[2] * by, out[3] * by);
+      four<T>(out[0] * scale, out[1] * scale, out[2] * scale, out[3] * scale);
 }
 
 // ---------------------------------------------------------------- the choice
@@ -737,44 +777,53 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionPara
 constexpr bool eight_waves(int dp) { return dp == 128; }
 
 struct Plan {
-  int rows;   // of a block: 16 and 32 in the form for few rows, 128 and 256 in that for many
+  int rows;   // of a block: 16 in the form for few rows, 128 and 256 in that for many
   long blocks, splits, split_tiles;
   size_t ml_bytes, o_bytes;
 };
 
-Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t max_seq_len, int64_t window) {
+Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim, bool fp8, int64_t max_seq_len, int64_t window) {
   Plan plan{};
-  const int64_t group = heads / kv_heads, queries = (tokens + seqs - 1) / std::max<int64_t>(seqs, 1), of_sequence = queries * group;
+  const int64_t group = heads / kv_heads, queries = (tokens + seqs - 1) / std::max<int64_t>(seqs, 1);
+  const int64_t keys = std::max<int64_t>(window > 0 ? std::min(max_seq_len, window + queries) : max_seq_len, 1), longest = (keys + kTile - 1) / kTile;
   const int dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-  // 256 rows from two rounds of workgroups on: two pieces of 2048 tokens behind 6144 others 488 us, with 128 rows 510; 33 sequences of
-  // up to 500 tokens, one round, 212 and 177
-  plan.rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : eight_waves(dp) && tokens * heads / 256 >= 512 ? 256 : 128;
+  auto groups_of = [&](int rows) {
+    return std::max<int64_t>((tokens * group + rows - 1) / rows, std::min(seqs, tokens)) * kv_heads;
+  };
+  // Few rows a sequence: the form for many, whose copies are further ahead, once there is much to read, and of 16-bit numbers in
+  // heads of more than 64 (64 sequences of 800 to 4096 keys, 4 rows each: 142 us, the form for few 154; of 8-bit codes 104 and 89, in
+  // heads of 64 50 and 52; one sequence of 700 keys 10.4 and 9.3, of 8000 18.5 and 17.1).  From two rounds of workgroups on blocks of
+  // 256 rows: two pieces of 2048 tokens behind 6144 others 488 us, with 128 rows 510; 33 sequences of up to 500 tokens, one round, 212
+  // and 177.
+  const bool few = queries * group <= 16 && (fp8 || dp == 64 || groups_of(16) * longest < 2048);
+  plan.rows = few ? 16 : eight_waves(dp) && tokens * heads / 256 >= 512 ? 256 : 128;
   plan.blocks = tokens * group / plan.rows + seqs + 1;
-  const int64_t groups = std::max<int64_t>((tokens * group + plan.rows - 1) / plan.rows, std::min(seqs, tokens)) * kv_heads;
-  const int64_t keys = std::max<int64_t>(window > 0 ? std::min(max_seq_len, window + queries) : max_seq_len, 1);
-  if (plan.rows <= 32) {
+  const int64_t groups = groups_of(plan.rows);
+  if (few) {
     // Tiles of a part: with t of them a workgroup takes some 0.6 t us, and joining the others 0.1 us a part, so that the square root
-    // of 0.15 times the sequence's tiles is about the best for one sequence (8000 keys: 4 tiles 18.3 us, 2 23.5); with more of them
-    // about 2048 workgroups, which even out (64 sequences of 800 to 4096 keys: 162 us, with 512 workgroups 196).
-    const int64_t tiles = (keys + kTile - 1) / kTile;
-    const int64_t for_one = (int64_t)__builtin_sqrt(0.15 * (double)tiles + 0.25), for_many = std::min<int64_t>(groups * tiles / 2048, 32);
-    plan.split_tiles = std::min(std::max<int64_t>(std::max(for_one, for_many), 2), tiles);
-    plan.splits = (tiles + plan.split_tiles - 1) / plan.split_tiles;
+    // of 0.15 times the sequence's tiles is about the best for one sequence (8000 keys: 4 tiles 17.2 us, 2 19.1); with more of them
+    // about 4096 workgroups, which even out (64 sequences of 800 to 4096 keys: 155 us with 8 tiles, 4 158, 16 164).
+    const int64_t for_one = (int64_t)__builtin_sqrt(0.15 * (double)longest + 0.25), for_many = groups * longest / 4096;
+    plan.split_tiles = std::min(std::min<int64_t>(std::max<int64_t>(std::max(for_one, for_many), 2), 8), longest);
   } else {
-    // Parts, by what a round of workgroups takes (us a tile, measured) and what writing and reading the parts takes.
-    const int64_t tiles = (keys - std::min(queries, keys) / 2 + kTile - 1) / kTile, longest = (keys + kTile - 1) / kTile;
-    const double of_tile = dp == 64 ? 1.3 : dp == 128 ? 2.1 : 2.6;
-    const int64_t at_once = dp == 256 || plan.rows == 256 ? 256 : 512;
+    // Parts, by what a compute unit's workgroups take for a tile (us, measured: alone, and as many as it holds together) and what
+    // writing and reading the parts takes.
+    const int64_t tiles = (keys - std::min(queries, keys) / 2 + kTile - 1) / kTile;
+    auto of_tile = [&](int64_t workgroups) {   // of one compute unit
+      if (dp == 256 || plan.rows == 256) return (double)workgroups * (dp == 256 ? 2.6 : 2.2);
+      if (dp == 64) return (double)(workgroups / 3) * 1.3 + (workgroups % 3 == 0 ? 0.0 : workgroups % 3 == 1 ? 0.9 : 1.1);
+      return (double)(workgroups / 2) * 2.1 + (workgroups % 2 == 0 ? 0.0 : queries * group > 64 ? 1.9 : 1.35);
+    };
     double best = 0.0;
-    plan.splits = 1;
-    for (int64_t parts = 1; parts <= 32 && parts <= tiles; ++parts) {
-      const double rounds = (double)((groups * parts + at_once - 1) / at_once), bytes = 8.0 * (double)(parts * tokens * heads * head_dim);
-      const double time = rounds * ((double)((tiles + parts - 1) / parts) * of_tile + 4.0) + (parts > 1 ? 5.0 + 0.3 * (double)parts + bytes / 4e6 : 0.0);
-      if (parts == 1 || time < 0.97 * best) best = time, plan.splits = parts;
+    int64_t parts = 1;
+    for (int64_t n = 1; n <= 64 && n <= tiles; ++n) {
+      const double bytes = 8.0 * (double)(n * tokens * heads * head_dim);
+      const double time = (double)((tiles + n - 1) / n) * of_tile((groups * n + 255) / 256) + (n > 1 ? 5.0 + 0.3 * (double)n + bytes / 4e6 : 0.0);
+      if (n == 1 || time < 0.97 * best) best = time, parts = n;
     }
-    plan.split_tiles = (longest + plan.splits - 1) / plan.splits;
-    plan.splits = (longest + plan.split_tiles - 1) / plan.split_tiles;
+    plan.split_tiles = (longest + parts - 1) / parts;
   }
+  plan.splits = (longest + plan.split_tiles - 1) / plan.split_tiles;
   if (plan.splits > 1) {
     plan.ml_bytes = (size_t)(plan.splits * tokens * heads) * sizeof(float2);
     plan.ml_bytes = (plan.ml_bytes + 15) / 16 * 16;
@@ -788,8 +837,8 @@ int launch_join(const AttentionParams& p, hipStream_t st) {
   if (p.splits == 1) return SONAR_OK;
   const long rows = (long)p.tokens * p.heads;
   // (a workgroup a row where parts are many and rows few: one sequence of 8000 keys 18 us, a wavefront a row 24)
-  if (p.splits > 8 && rows <= 1024) attention_join_kernel<T, DP / 4, true><<<(uint32_t)rows, 256, 0, st>>>(p);
-  else attention_join_kernel<T, DP / 4, false><<<(uint32_t)((rows + 3) / 4), 256, 0, st>>>(p);
+  if (p.splits > 8 && rows <= 256) attention_join_kernel<T, DP / 4, 8><<<(uint32_t)rows, 512, 0, st>>>(p);
+  else attention_join_kernel<T, DP / 4, 1><<<(uint32_t)((rows + 3) / 4), 256, 0, st>>>(p);
   return launch_status("attention_join_kernel");
 }
 
@@ -800,22 +849,25 @@ int launch_one(K kernel, const AttentionParams& p, int waves, int lds, const cha
   return launch_status(name);
 }
 
-template <typename T, int DP, bool FP8, bool EXTRA>
+template <typename T, int DP, bool FP8, int SCORES>
 int launch_form(const AttentionParams& p, hipStream_t st) {
   int rc;
-  if (p.rows == 16) rc = launch_one(attention_few_kernel<T, DP, FP8, EXTRA, 1>, p, kWaves, few_lds<DP>(), "attention_few_kernel", st);
-  else if (p.rows == 32) rc = launch_one(attention_few_kernel<T, DP, FP8, EXTRA, 2>, p, kWaves, few_lds<DP>(), "attention_few_kernel", st);
-  else if (p.rows == 128) rc = launch_one(attention_rows_kernel<T, DP, FP8, EXTRA, 4>, p, 4, rows_lds<DP>(), "attention_rows_kernel", st);
-  else if constexpr (eight_waves(DP)) rc = launch_one(attention_rows_kernel<T, DP, FP8, EXTRA, 8>, p, 8, rows_lds<DP>(), "attention_rows_kernel", st);
+  if (p.rows == 16) rc = launch_one(attention_few_kernel<T, DP, FP8, SCORES>, p, kFew, few_lds<DP>(), "attention_few_kernel", st);
+  else if (p.rows == 128) rc = launch_one(attention_rows_kernel<T, DP, FP8, SCORES, 4>, p, 4, rows_lds<DP>(), "attention_rows_kernel", st);
+  else if constexpr (eight_waves(DP)) rc = launch_one(attention_rows_kernel<T, DP, FP8, SCORES, 8>, p, 8, rows_lds<DP>(), "attention_rows_kernel", st);
   else return fail(SONAR_E_INVALID, "no form of %d rows", p.rows);
   return rc != SONAR_OK ? rc : launch_join<T, DP>(p, st);
 }
 
+template <typename T, int DP, bool FP8>
+int launch_scores(const AttentionParams& p, hipStream_t st) {
+  if (p.slopes != nullptr) return launch_form<T, DP, FP8, kSloped>(p, st);
+  return p.cap > 0.0f ? launch_form<T, DP, FP8, kCapped>(p, st) : launch_form<T, DP, FP8, kPlain>(p, st);
+}
+
 template <typename T, int DP>
 int launch_width(const AttentionParams& p, bool fp8, hipStream_t st) {
-  const bool extra = p.cap > 0.0f || p.slopes != nullptr;
-  if (fp8) return extra ? launch_form<T, DP, true, true>(p, st) : launch_form<T, DP, true, false>(p, st);
-  return extra ? launch_form<T, DP, false, true>(p, st) : launch_form<T, DP, false, false>(p, st);
+  return fp8 ? launch_scores<T, DP, true>(p, st) : launch_scores<T, DP, false>(p, st);
 }
 
 template <typename T>
@@ -842,9 +894,9 @@ int check_sizes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, i
 using namespace sonar;
 
 extern "C" size_t sonar_paged_attention_scratch_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads,
-                                                      int64_t head_dim, int64_t max_seq_len, int64_t window) {
+                                                      int64_t head_dim, int cache_dtype, int64_t max_seq_len, int64_t window) {
   if (check_sizes(tokens, seqs, heads, kv_heads, head_dim, max_seq_len, window) != SONAR_OK || tokens == 0 || seqs == 0) return 0;
-  const Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, max_seq_len, window);
+  const Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, cache_dtype == SONAR_CACHE_FP8, max_seq_len, window);
   return plan.ml_bytes + plan.o_bytes;
 }
 
@@ -886,7 +938,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   SONAR_REQUIRE(seqs >= 1, "tokens without sequences: seqs = 0");
   SONAR_REQUIRE(seq_lens && (table_pages == 0 || (block_table && table_stride >= table_pages && pages >= 1 && key_cache->data && value_cache->data)),
                 "seq_lens, a block_table of %ld pages a row and caches with pages are needed", (long)table_pages);
-  Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, max_seq_len, window);
+  Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, cache_dtype == SONAR_CACHE_FP8, max_seq_len, window);
   if (scratch_bytes < plan.ml_bytes + plan.o_bytes || scratch == nullptr) plan.splits = 1;
   SONAR_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
   SONAR_REQUIRE(plan.blocks * kv_heads * plan.splits < (1LL << 24) && (plan.splits == 1 || tokens * heads < (1LL << 24)),
@@ -910,7 +962,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   p.page_size = (int)page_size, p.pages = (int)pages, p.table_pages = (int)table_pages;
   p.tokens = (int)tokens, p.seqs = (int)seqs, p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads);
   p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles;
-  p.by_dies = plan.rows <= 32;
+  p.by_dies = plan.rows == 16;
   const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
   hipStream_t st = (hipStream_t)stream;
   return dtype == SONAR_DTYPE_F16 ? launch<_Float16>(p, fp8, st) : launch<__bf16>(p, fp8, st);

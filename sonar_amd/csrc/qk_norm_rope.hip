@@ -112,8 +112,9 @@ __device__ __forceinline__ void store_fp8(char* to, const float (&y)[VEC], float
 // `lanes` lanes a head, two runs of VEC numbers a lane: of the rotated numbers those of VEC whole pairs (run i of either half,
 // or runs 2i and 2i + 1), behind them two neighbouring runs.  A thread keeps its part of the cosines, sines and weights for all
 // heads of its token that it takes.
+// (128 registers for four wavefronts a SIMD: 73 us for the 77 with 132; eight numbers of 32 bits would spill there)
 template <typename T, int VEC>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const RopeParams p) {
+__global__ __launch_bounds__(kThreads, VEC * sizeof(T) > 16 ? 3 : 4) void qk_norm_rope_kernel(const RopeParams p) {
 #pragma clang fp contract(off)
   const int slot = threadIdx.x / p.lanes, j = threadIdx.x % p.lanes;
   const int tokens_here = kThreads / p.lanes / p.of_token;
@@ -298,6 +299,9 @@ int launch_runs(RopeParams p, hipStream_t st) {
   const int slots = kThreads / p.lanes, all = p.heads + (p.cached ? 2 : 1) * p.kv_heads;
   p.of_token = slots;
   while (p.of_token > 1 && p.of_token / 2 >= all) p.of_token /= 2;
+  // Four heads or more a thread, which then reads that many at once and its cosines, sines and weights once for them, while there are
+  // threads enough: 16384 tokens of 40 heads of 128 with norms 77 us, a head or two a thread 111; 4096 20.4 and 24.3.
+  while (p.of_token > 1 && all / p.of_token < kAhead && p.tokens * (p.of_token / 2) * p.lanes >= 262144) p.of_token /= 2;
   const int tokens_here = slots / p.of_token;
   qk_norm_rope_kernel<T, VEC><<<(uint32_t)((p.tokens + tokens_here - 1) / tokens_here), kThreads, 0, st>>>(p);
   return launch_status("qk_norm_rope_kernel");

@@ -107,7 +107,7 @@ def test_calls_without_tokens_launch_nothing():
     _lib, lib = library()
     assert rope_call(lib, _lib, tokens=0, q=None, k=None, positions=None) == 0
     assert attention_call(lib, _lib, tokens=0, q=None, seqs=0, lens=None) == 0
-    assert lib.sonar_paged_attention_scratch_bytes(0, 4, 8, 8, 64, 10000, 0) == 0
+    assert lib.sonar_paged_attention_scratch_bytes(0, 4, 8, 8, 64, 1, 10000, 0) == 0
 
 
 # ---------------------------------------------------------------- ops
