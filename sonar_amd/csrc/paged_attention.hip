@@ -294,57 +294,53 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[h][i] = shown(s[h][i], seen, 8 * (i / 4) + i % 4);
     }
-    s[h ^ 1] = floatx16_t{};
-    float top = -kInfinity, less = 0.0f, by = 1.0f;
-    bool rises = false;
+    // The weights are formed with the maximum so far, as if the scores had not risen past it, and anew in the rare case that they have:
+    // so nothing waits for the comparison.
+    const float before = sum;
+    float top = -kInfinity;
+    auto weight = [&](int e, float less) {
+      return __builtin_amdgcn_exp2f(SCORES == kPlain ? __builtin_fmaf(s[h][e], score.by, -less) : s[h][e] - less);
+    };
+    auto put = [&](int e, float one, float two) {
+      auto both = E::pair(one, two);
+      asm volatile("" : "+v"(both));   // (or the weights would be formed where they are used, behind the products)
+      weights[h][e / 8][e % 8] = both[0], weights[h][e / 8][e % 8 + 1] = both[1];
+      sum = E::add(both, sum);
+    };
+    const float less = most == -kInfinity ? 0.0f : most;
+    float last_weight = 0.0f;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
       const int n = i / 2;
       if (i % 2 == 0) {
+        if (n + 2 < kSteps) read_keys(k_from, h ^ 1, n + 2);
+        s[h ^ 1] = E::mfma32(k_piece[n], q[n], n == 0 ? floatx16_t{} : s[h ^ 1]);
+      } else {
         if (n + 2 < 2 * kColumns) read_values(v_from, h ^ 1, n + 2);
         out[n % kColumns] = E::mfma32(v_piece[n], weights[h ^ 1][n / kColumns], out[n % kColumns]);
-      } else {
-        if (n + 2 < kSteps) read_keys(k_from, h ^ 1, n + 2);
-        s[h ^ 1] = E::mfma32(k_piece[n], q[n], s[h ^ 1]);
       }
-      if (i < kTops) {
 #pragma unroll
-        for (int e = 16 * i / kTops; e < 16 * (i + 1) / kTops; ++e) {
-          if (SCORES == kCapped) s[h][e] = shown(score.capped(s[h][e]), seen, 8 * (e / 4) + e % 4);
-          top = fmaxf(top, s[h][e]);
+      for (int e = 16 * i / kSlots; e < 16 * (i + 1) / kSlots; ++e) {
+        if (SCORES == kCapped) s[h][e] = shown(score.capped(s[h][e]), seen, 8 * (e / 4) + e % 4);
+        const float w = weight(e, less);
+        if (e % 2 == 1) {
+          put(e - 1, last_weight, w);
+          top = fmaxf(fmaxf(top, s[h][e - 1]), s[h][e]);
         }
-      } else if (i == kTops) {
-        if (SCORES == kPlain) top *= score.by;
-        rises = __any(top > most + 8.0f);
-        const float old = most, higher = fmaxf(old, joined<true>(top, [](float a, float b) { return fmaxf(a, b); }));
-        most = rises ? higher : old;
-        less = most == -kInfinity ? 0.0f : most, by = __builtin_amdgcn_exp2f(old - less);
-        sum *= by;
-      } else {
-        constexpr int kLeft = kSlots - kTops - 1;
-        const int j = i - kTops - 1;
-#pragma unroll
-        for (int pair = 8 * j / kLeft; pair < 8 * (j + 1) / kLeft; ++pair) {
-          float w[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = s[h][2 * pair + e];
-            w[e] = __builtin_amdgcn_exp2f(SCORES == kPlain ? __builtin_fmaf(x, score.by, -less) : x - less);
-          }
-          auto both = E::pair(w[0], w[1]);
-          asm volatile("" : "+v"(both));   // (or the weights would be formed where they are used, behind the products)
-          weights[h][pair / 4][pair % 4 * 2] = both[0], weights[h][pair / 4][pair % 4 * 2 + 1] = both[1];
-          sum = E::add(both, sum);
-        }
+        last_weight = w;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (rises) {
-      float shrink = by;
-      asm volatile("" : "+v"(shrink));   // (or the products would be formed every time, ahead of the branch)
+    if (SCORES == kPlain) top *= score.by;
+    if (__any(top > most + 8.0f)) {
+      const float now = fmaxf(most, joined<true>(top, [](float a, float b) { return fmaxf(a, b); }));
+      const float less = now == -kInfinity ? 0.0f : now, by = __builtin_amdgcn_exp2f(most - less);
+      most = now, sum = before * by;
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) out[c] *= shrink;
+      for (int c = 0; c < kColumns; ++c) out[c] *= by;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) put(e, weight(e, less), weight(e + 1, less));
     }
   };
   if (p.dim < DP) {   // what no copy reaches
@@ -352,14 +348,22 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     __syncthreads();
   }
   if (tile < last) {
+    // the first tile's keys and values and the next one's keys, all on their way at once
     look_up(tile);
-    find(tile);
+    const int first_page = page_ahead;
     look_up(tile + 1);
+    const int second_page = page_ahead;
+    look_up(tile + 2);
+    const int third_page = page_ahead;
+    page_ahead = first_page;
+    find(tile);
     fetch_keys(k_lds);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) weights[1][i] = eight{};
-    for (int i = threadIdx.x * 16; i < kTileBytes; i += WAVES * 64 * 16) *reinterpret_cast<u32x4_t*>(v_tiles + kTileBytes + i) = u32x4_t{};
+    page_ahead = second_page;
     if constexpr (FP8) {
+      spread(v_rows, places);
+      fetch_values(v_lds);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) weights[1][i] = eight{};
       if (has_k) {
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
@@ -369,14 +373,19 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
           *reinterpret_cast<u32x4_t*>(row + 16 * (2 * k_chunk + 1 ^ swap)) = widen<T>(k_next[i][2], k_next[i][3]);
         }
       }
+      find(tile + 1);
+      fetch_keys(k_lds + kTileBytes);
     } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      find(tile + 1);
+      fetch_values(v_lds);
+      fetch_keys(k_lds + kTileBytes);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) weights[1][i] = eight{};
     }
+    page_ahead = third_page;
+    for (int i = threadIdx.x * 16; i < kTileBytes; i += WAVES * 64 * 16) *reinterpret_cast<u32x4_t*>(v_tiles + kTileBytes + i) = u32x4_t{};
+    if constexpr (!FP8) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    find(tile + 1);
-    fetch_values(v_lds);
-    fetch_keys(k_lds + kTileBytes);
-    look_up(tile + 2);
     s[0] = floatx16_t{};
 #pragma unroll
     for (int d = 0; d < kSteps; ++d) {
@@ -426,15 +435,30 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
           if (32 * c + 2 * i < p.dim)
             *reinterpret_cast<floatx4_t*>(to + 32 * c + 2 * i) = floatx4_t{out[c][i], out[c][i + 1], out[c][i + 2], out[c][i + 3]};
     }
-  } else if (row < r.rows) {
+  } else {
+    // through LDS, to leave as whole lines: a row's pieces of 16 bytes swapped by its number, as the tiles' are
+    __syncthreads();
+    char* const mine = lds + wave * 32 * kPitch;
+    constexpr int kPieces = kPitch / 16, kSwap = kPieces < 16 ? kPieces - 1 : 15;
     const float by = sum == 0.0f ? 0.0f : value_scale(p, kv_head) / sum;
-    T* to = (T*)p.out + token * p.out_token + head * p.out_head + 4 * half;
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
-        if (32 * c + 2 * i < p.dim)
-          *reinterpret_cast<Four<T>*>(to + 32 * c + 2 * i) = four<T>(out[c][i] * by, out[c][i + 1] * by, out[c][i + 2] * by, out[c][i + 3] * by);
+        *reinterpret_cast<Four<T>*>(mine + (lane & 31) * kPitch + ((4 * c + i / 4) ^ (lane & kSwap & 31)) * 16 + 8 * half) =
+            four<T>(out[c][i] * by, out[c][i + 1] * by, out[c][i + 2] * by, out[c][i + 3] * by);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const long place = token * p.out_token + head * p.out_head;
+    typedef uint32_t lines __attribute__((ext_vector_type(4), aligned(8)));
+#pragma unroll
+    for (int i = 0; i < 32 * kPieces / 64; ++i) {
+      const int from = (i * 64 + lane) / kPieces, piece = (i * 64 + lane) % kPieces;
+      const uint32_t low = __builtin_amdgcn_ds_bpermute(4 * from, (int)place), high = __builtin_amdgcn_ds_bpermute(4 * from, (int)(place >> 32));
+      const lines x = *reinterpret_cast<const lines*>(mine + from * kPitch + (piece ^ (from & kSwap)) * 16);
+      if (r.first + wave * 32 + from < r.rows && piece * 8 < p.dim)
+        *reinterpret_cast<lines*>((T*)p.out + (long)((uint64_t)high << 32 | low) + piece * 8) = x;
+    }
   }
   if (found & 2)
     add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last, min(r.rows, r.first + kRows), block_full_low, block_full_high);

@@ -159,3 +159,14 @@ def test_random_batches():
         if len(b.q):
             print(seed, lengths, more, flush=True)
             b.check(b.call(), **{}) if not more else b.check(b.call(**more), **more)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("extra", [{}, dict(softcap=30.0), dict(alibi_slopes=torch.tensor([0.5, 0.1, 0.01, 0.7]))], ids=["plain", "capped", "sloped"])
+def test_every_form(dtype, dim, fp8, extra):
+    """Few rows and many, whole and in parts that a wavefront or eight of them join, of every type, width, cache and score."""
+    for lengths in (ONES, PIECES, [(3000, 1)], [(1500, 130)]):
+        b = Batch(dim, lengths, kv_heads=1, dim=dim, dtype=dtype, fp8=fp8)
+        b.check(b.call(**extra), **extra)

@@ -212,21 +212,26 @@ def test_blocks_of_256_rows(dtype, dim, lengths):
     assert ((got.double() - want).abs() <= limit).all()
 
 
-def test_256_rows_of_codes_and_caps():
-    """The forms of 256 rows for 8-bit codes and capped scores, against those of 128 rows and of few rows on the same numbers."""
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("extra", [{}, dict(softcap=20.0), dict(alibi_slopes=True)], ids=["plain", "capped", "sloped"])
+def test_256_rows_of_codes_and_scores(dtype, fp8, extra):
+    """Every form of 256 rows, against those of 128 rows and of few rows on the same numbers."""
     from sonar_amd import ops
-    for fp8, cap in ((True, 0.0), (False, 20.0), (True, 20.0)):
-        b = Batch(11, [(4200, 4100)], heads=32, kv_heads=4, dim=128, fp8=fp8)
-        got = b.call(softcap=cap)
-        d = lambda t: None if t is None else t.to(DEV)  # noqa: E731
-        for at in (0, 777, 2000, 4000):   # pieces of the same prompt: the queries up to there as a prompt of their own
-            for queries in (1, 100):
-                n = 100 + at + queries
-                part = ops.paged_attention(d(b.q)[at:at + queries], d(b.k), d(b.v), d(b.table), d(torch.tensor([n], dtype=torch.int32)),
-                                           d(torch.tensor([0, queries], dtype=torch.int32)), softcap=cap, k_scale=d(b.k_scale), v_scale=d(b.v_scale))
-                # both are within the tolerance of the exact numbers; a mean of |v| is about 0.8 of v's scale, at most 4 of it here
-                most = 4 * (float(b.v_scale) * 4 if fp8 else 1)
-                assert (part.double() - got[at:at + queries].double()).abs().max() <= 4 * 2.0 ** -8 * most
+    b = Batch(11, [(4200, 4100)], heads=32, kv_heads=4, dim=128, fp8=fp8, dtype=dtype)
+    more = dict(extra)
+    if "alibi_slopes" in more:
+        more["alibi_slopes"] = torch.linspace(0.001, 0.5, 32, device=DEV)
+    got = b.call(**more)
+    d = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+    for at in (0, 777, 2000, 4000):   # pieces of the same prompt: the queries up to there as a prompt of their own
+        for queries in (1, 100):
+            n = 100 + at + queries
+            part = ops.paged_attention(d(b.q)[at:at + queries], d(b.k), d(b.v), d(b.table), d(torch.tensor([n], dtype=torch.int32)),
+                                       d(torch.tensor([0, queries], dtype=torch.int32)), k_scale=d(b.k_scale), v_scale=d(b.v_scale), **more)
+            # each is off by less than 2 h of the mean of |v| (see the head of the file) and h of itself: both by 6 h of the largest |v|
+            most = b.v.float().abs().max() * (float(b.v_scale) if fp8 else 1.0)
+            assert (part.double() - got[at:at + queries].double()).abs().max() <= 6 * HALF_STEP[dtype] * most
 
 
 def test_a_cache_past_32_bits():
