@@ -24,7 +24,8 @@ const char* sonar_attention_last_error(void);
 
 /* A paged cache of keys or values: element (page, slot, head, d) lies at data + page * page_stride + slot * slot_stride +
  * head * head_stride + d.  `dtype` is the element type, or SONAR_CACHE_FP8 for float8_e4m3fn codes, which stand for
- * code * scale; `scale` holds 1 or kv_heads float32 numbers on the device (scale_len; NULL for 16- and 32-bit caches). */
+ * code * scale; `scale` holds 1 or kv_heads float32 numbers on the device (scale_len; NULL for 16- and 32-bit caches), which must be
+ * positive: a negative or NaN scale of the keys makes attention's results NaN. */
 #define SONAR_CACHE_FP8 3
 typedef struct sonar_kv_cache {
   void* data;
@@ -47,7 +48,8 @@ typedef struct sonar_kv_cache {
  *   q_out          dtype[tokens][heads][head_dim];  k_out dtype[tokens][kv_heads][head_dim], NULL with a cache
  *   key_cache, value_cache  both or neither; cache_dtype: dtype or SONAR_CACHE_FP8 (not with F32)
  *   slots          int64 (slots_64) or int32 [tokens]: token t goes to slot slots[t] % page_size of page slots[t] / page_size;
- *                  numbers outside [0, pages * page_size) go nowhere.  Which of two tokens with one slot stays is not defined.
+ *                  numbers outside [0, pages * page_size) go nowhere.  Which of two tokens with one slot
+ *                  stays is not defined, for each head anew.
  * tokens * (heads + 2 kv_heads) below 2^31, head_dim at most 1024. */
 int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
                        int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride, const void* positions,
@@ -75,10 +77,10 @@ int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  *   caches      of dtype or SONAR_CACHE_FP8; 16-byte aligned, strides multiples of 16 bytes; page_size slots a page; 64 GiB at most
  *   block_table int32[seqs][table_stride], table_pages of a row in use;  seq_lens int32[seqs];  starts int32[seqs + 1], rising, from 0
  *   slopes      float[heads] or NULL;  tree_mask int64[tokens][tree_words] or NULL
- *   max_seq_len what the split of the keys is chosen for; longer sequences are right too
+ *   max_seq_len what the split of the keys is chosen for; longer sequences are right too, and much shorter ones about as fast
  *   scratch     device memory, 16-byte aligned, of sonar_paged_attention_scratch_bytes(...) bytes (may be 0); calls that overlap in
  *               time need scratches of their own
- * head_dim a multiple of 16, at most 256; scale > 0; tokens * heads below 2^31, table_pages * page_size below 2^31 - 1024. */
+ * head_dim a multiple of 16, at most 256; scale, and cap if not 0, from 1e-30 to 1e30; tokens * heads below 2^31, table_pages * page_size below 2^31 - 1024. */
 size_t sonar_paged_attention_scratch_bytes(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                            int cache_dtype, int64_t max_seq_len, int64_t window);
 int sonar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const sonar_kv_cache* key_cache,

@@ -154,6 +154,7 @@ Tensor qk_norm_rope_append(const Tensor& query, const Tensor& key, const Tensor&
               "key_cache and value_cache must have one shape and type");
   at::assert_no_internal_overlap(key_cache);
   at::assert_no_internal_overlap(value_cache);
+  at::assert_no_overlap(key_cache, value_cache);
   TORCH_CHECK(slot_mapping.device() == query.device() && is_index(slot_mapping) && slot_mapping.dim() == 1 && slot_mapping.size(0) == tokens,
               "slot_mapping must hold ", tokens, " int64 or int32 numbers on query's device");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(query.device());
@@ -198,7 +199,8 @@ void attend(const Tensor& query, const Tensor& key_cache, const Tensor& value_ca
   c10::hip::HIPGuardMasqueradingAsCUDA guard(query.device());
   const Heads q(query, true);
   const Tensor lens = seq_lens.contiguous(), starts = query_start_loc.contiguous();
-  const Tensor table = block_table.size(1) > 1 && block_table.stride(1) != 1 ? block_table.contiguous() : block_table;
+  const bool rows = (block_table.size(1) <= 1 || block_table.stride(1) == 1) && (seqs <= 1 || block_table.stride(0) >= block_table.size(1));
+  const Tensor table = rows ? block_table : block_table.clone(at::MemoryFormat::Contiguous);
   const Tensor slopes = alibi_slopes.has_value() ? alibi_slopes->contiguous() : Tensor();
   const Tensor tree = tree_mask.has_value() ? tree_mask->contiguous() : Tensor();
   const int64_t table_pages = table.size(1), table_stride = seqs > 1 ? table.stride(0) : table_pages;

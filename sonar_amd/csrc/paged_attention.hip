@@ -16,15 +16,20 @@ namespace sonar {
 char* last_error_buffer();
 namespace {
 
-constexpr int kTile = 64;   // keys
-
 // What turns a score q . k into a power of two: s * by, or capped cap * tanh of it as cap - 2 cap / (1 + e^2x); less the slope's part.
-enum Scores { kPlain, kCapped, kSloped };   // (sloped ones may be capped too)
+enum Scores { kPlain, kCapped, kSloped };   // (sloped ones may be capped too, and have slopes of 0 where the cap is large)
 struct Score {
   float by, cap, slope;
   bool is_capped;
   __device__ __forceinline__ float capped(float s) const {
     return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s * by)), cap);
+  }
+  // The same for any cap: what is much smaller than it would be the difference of two large numbers above, off by 2^-22 of the cap.
+  // Below an eighth of it four terms of tanh's series are off by 2^-29 of themselves.
+  __device__ __forceinline__ float any_capped(float s) const {
+    const float x = s * by * (0.5f / kLog2E), xx = x * x;
+    const float series = __builtin_fmaf(xx, __builtin_fmaf(xx, __builtin_fmaf(xx, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    return fabsf(x) < 0.125f ? cap * (x * series) : capped(s);
   }
   __device__ __forceinline__ float sloped(float s, float distance) const { return __builtin_fmaf(-slope, fabsf(distance), s); }
 };
@@ -34,6 +39,8 @@ __device__ __forceinline__ Score score_of(const AttentionParams& p, int kv_head,
   Score s;
   s.is_capped = p.cap > 0.0f;
   s.by = s.is_capped ? 2.0f * kLog2E * p.scale * k_scale / p.cap : p.scale * k_scale * kLog2E;
+  // positive and finite, so that what is masked stays at -infinity and the largest product is the largest score
+  s.by = k_scale >= 0.0f ? fminf(fmaxf(s.by, 0x1p-126f), 0x1p127f) : __builtin_nanf("");
   s.cap = p.cap * kLog2E;
   s.slope = p.slopes == nullptr ? 0.0f : p.slopes[head] * kLog2E;
   return s;
@@ -134,7 +141,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   const int split = item / p.blocks;
   // the blocks of the last tokens, which see the most keys, first
   const RowBlock r = row_block<kRows>(p, p.blocks - 1 - item % p.blocks);
-  if (r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;
+  if (r.first < 0 || r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;   // (negative where starts do not rise)
 
   const int row = r.first + wave * 32 + (lane & 31), half = lane >> 5;
   const int my_row = min(row, r.rows - 1), t = my_row / p.group, head = kv_head * p.group + my_row % p.group;
@@ -145,7 +152,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   int low, high;
   keys_seen(p, r, block_t0, block_t1, low, high);
   int tile = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
-  if (!split_of(p, split, tile, last, parts)) return;
+  if (!split_of(p, r, split, tile, last, parts)) return;
   const int first_tile = tile;
   // tiles that every query of the wavefront (of the block) sees whole: from `full_low` up to `full_high`
   const bool bounded = p.causal && p.tree == nullptr;
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
       const float distance = (float)(sight.position - base - 4 * half);
       if (score.is_capped) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[h][i] = score.capped(s[h][i]);
+        for (int i = 0; i < 16; ++i) s[h][i] = score.any_capped(s[h][i]);
       } else {
         s[h] *= score.by;
       }
@@ -494,12 +501,12 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
   item_of(p, p.blocks * p.splits, blockIdx.x, item, kv_head);
   const int split = item / p.blocks;
   const RowBlock r = row_block<16>(p, item % p.blocks);
-  if (r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;
+  if (r.first < 0 || r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;   // (negative where starts do not rise)
   const int block_t0 = r.first / p.group, block_t1 = min(r.first + 16 - 1, r.rows - 1) / p.group;
   int low, high;
   keys_seen(p, r, block_t0, block_t1, low, high);
   int first_tile = low / kTile, last_tile = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
-  if (!split_of(p, split, first_tile, last_tile, parts)) return;
+  if (!split_of(p, r, split, first_tile, last_tile, parts)) return;
   const bool bounded = p.causal && p.tree == nullptr;
   const int full_low = bounded && p.window > 0 ? max(r.past + block_t1 - p.window + 1, 0) : 0;
   const int full_high = p.tree != nullptr ? min(r.len, r.past) : bounded ? min(r.len, r.past + block_t0 + 1) : r.len;
@@ -596,9 +603,12 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
       if (unit + 2 * kFew < last) look_up(unit + 2 * kFew);
     }
     eight weights;
-    if (SCORES == kCapped || (SCORES == kSloped && score.is_capped)) {
+    if (SCORES == kCapped) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = score.capped(s[i / 4][i % 4]);
+    } else if (SCORES == kSloped && score.is_capped) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i / 4][i % 4] = score.any_capped(s[i / 4][i % 4]);
     } else if (SCORES == kSloped) {
 #pragma unroll
       for (int a = 0; a < 2; ++a) s[a] *= score.by;
@@ -725,7 +735,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_
   int low, high;
   keys_seen(p, r, r.first / p.group, min(r.first + p.rows - 1, r.rows - 1) / p.group, low, high);
   int first = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
-  split_of(p, 0, first, last, parts);
+  split_of(p, r, 0, first, last, parts);
   if (parts <= 1) return;
   float most = -kInfinity, sum = 0.0f;
   floatx4_t out{};
@@ -803,6 +813,8 @@ constexpr bool eight_waves(int dp) { return dp == 128; }
 struct Plan {
   int rows;   // of a block: 16 in the form for few rows, 128 and 256 in that for many
   long blocks, splits, split_tiles;
+  int longest;
+  float few_share;
   size_t ml_bytes, o_bytes;
 };
 
@@ -811,6 +823,7 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
   const int64_t group = heads / kv_heads, queries = (tokens + seqs - 1) / std::max<int64_t>(seqs, 1);
   const int64_t keys = std::max<int64_t>(window > 0 ? std::min(max_seq_len, window + queries) : max_seq_len, 1), longest = (keys + kTile - 1) / kTile;
   const int dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  plan.longest = (int)keys;
   auto groups_of = [&](int rows) {
     return std::max<int64_t>((tokens * group + rows - 1) / rows, std::min(seqs, tokens)) * kv_heads;
   };
@@ -824,11 +837,12 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
   plan.blocks = tokens * group / plan.rows + seqs + 1;
   const int64_t groups = groups_of(plan.rows);
   if (few) {
-    // Tiles of a part: with t of them a workgroup takes some 0.6 t us, and joining the others 0.1 us a part, so that the square root
-    // of 0.15 times the sequence's tiles is about the best for one sequence (8000 keys: 4 tiles 17.2 us, 2 19.1); with more of them
-    // about 4096 workgroups, which even out (64 sequences of 800 to 4096 keys: 155 us with 8 tiles, 4 158, 16 164).
-    const int64_t for_one = (int64_t)__builtin_sqrt(0.15 * (double)longest + 0.25), for_many = groups * longest / 4096;
-    plan.split_tiles = std::min(std::min<int64_t>(std::max<int64_t>(std::max(for_one, for_many), 2), 8), longest);
+    // Workgroups that find no part for them cost a trip to memory each, and the lengths may be far below what they might be: no more
+    // than 256 parts, and of more than 4 no more than make 4096 workgroups.
+    plan.few_share = (float)groups / 4096.0f;
+    plan.split_tiles = 2;
+    plan.splits = std::min<int64_t>(std::max<int64_t>(4096 / groups, 4), 256);
+    plan.splits = std::min<int64_t>(plan.splits, (longest + few_tiles((int)longest, plan.few_share) - 1) / few_tiles((int)longest, plan.few_share));
   } else {
     // Parts, by what a compute unit's workgroups take for a tile (us, measured: alone, and as many as it holds together) and what
     // writing and reading the parts takes.
@@ -845,9 +859,9 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
       const double time = (double)((tiles + n - 1) / n) * of_tile((groups * n + 255) / 256) + (n > 1 ? 5.0 + 0.3 * (double)n + bytes / 4e6 : 0.0);
       if (n == 1 || time < 0.97 * best) best = time, parts = n;
     }
-    plan.split_tiles = (longest + parts - 1) / parts;
+    plan.splits = parts, plan.split_tiles = std::min<int64_t>((longest + parts - 1) / parts, 4);
   }
-  plan.splits = (longest + plan.split_tiles - 1) / plan.split_tiles;
+  if (tokens * heads >= 1LL << 24 || plan.blocks * kv_heads * plan.splits >= 1LL << 24) plan.splits = 1;   // (2^32 threads are a launch's most)
   if (plan.splits > 1) {
     plan.ml_bytes = (size_t)(plan.splits * tokens * heads) * sizeof(float2);
     plan.ml_bytes = (plan.ml_bytes + 15) / 16 * 16;
@@ -885,7 +899,8 @@ int launch_form(const AttentionParams& p, hipStream_t st) {
 
 template <typename T, int DP, bool FP8>
 int launch_scores(const AttentionParams& p, hipStream_t st) {
-  if (p.slopes != nullptr) return launch_form<T, DP, FP8, kSloped>(p, st);
+  // (a cap of at most 128 is off by 2^-15 in the shorter form, much less than a weight's own rounding)
+  if (p.slopes != nullptr || p.cap > 128.0f) return launch_form<T, DP, FP8, kSloped>(p, st);
   return p.cap > 0.0f ? launch_form<T, DP, FP8, kCapped>(p, st) : launch_form<T, DP, FP8, kPlain>(p, st);
 }
 
@@ -939,8 +954,8 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   SONAR_REQUIRE(page_size >= 1 && pages >= 0 && pages < (1LL << 31) && table_pages >= 0 && page_size < (1LL << 31) &&
                     table_pages < (1LL << 31) && table_pages * page_size < (1LL << 31) - 1024,
                 "pages = %ld of %ld slots, %ld a sequence", (long)pages, (long)page_size, (long)table_pages);
-  SONAR_REQUIRE(scale > 0.0 && scale <= 3e38, "scale = %g must be positive", scale);
-  SONAR_REQUIRE(cap >= 0.0 && cap <= 1e30, "cap = %g must be 0 (none) or positive", cap);
+  SONAR_REQUIRE(scale >= 1e-30 && scale <= 1e30, "scale = %g must be positive, from 1e-30 to 1e30", scale);
+  SONAR_REQUIRE(cap == 0.0 || (cap >= 1e-30 && cap <= 1e30), "cap = %g must be 0 (none) or positive, from 1e-30 to 1e30", cap);
   SONAR_REQUIRE(tree_mask == nullptr || (tree_words >= 1 && tree_words < (1 << 20)), "tree_words = %ld", (long)tree_words);
   SONAR_REQUIRE(tree_mask == nullptr || (window == 0 && slopes == nullptr), "a tree mask goes with neither a window nor slopes");
   SONAR_REQUIRE(window == 0 || causal, "a window goes with causal attention only");
@@ -965,7 +980,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, cache_dtype == SONAR_CACHE_FP8, max_seq_len, window);
   if (scratch_bytes < plan.ml_bytes + plan.o_bytes || scratch == nullptr) plan.splits = 1;
   SONAR_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
-  SONAR_REQUIRE(plan.blocks * kv_heads * plan.splits < (1LL << 24) && (plan.splits == 1 || tokens * heads < (1LL << 24)),
+  SONAR_REQUIRE(plan.blocks * kv_heads * plan.splits < (1LL << 24),
                 "%ld tokens of %ld sequences and %ld heads take too many workgroups", (long)tokens, (long)seqs, (long)heads);
   auto pages_of = [&](const sonar_kv_cache* c) {
     const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
@@ -985,7 +1000,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   p.page_shift = 31 + log, p.page_magic = (uint32_t)((1ULL << p.page_shift) / (uint64_t)page_size + 1);
   p.page_size = (int)page_size, p.pages = (int)pages, p.table_pages = (int)table_pages;
   p.tokens = (int)tokens, p.seqs = (int)seqs, p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads);
-  p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles;
+  p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles, p.longest = plan.longest, p.few_share = plan.few_share;
   p.by_dies = plan.rows == 16;
   const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
   hipStream_t st = (hipStream_t)stream;

@@ -12,6 +12,7 @@ typedef float floatx16_t __attribute__((ext_vector_type(16)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 
+constexpr int kTile = 64;   // keys
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kInfinity = __builtin_inff();
 
@@ -41,6 +42,8 @@ struct AttentionParams {
   int page_shift, page_size, pages, table_pages;
   int window, tree_words, tokens, seqs, heads, kv_heads, group, dim;
   int rows, blocks, splits, split_tiles;   // rows of a block, blocks of rows; at most `splits` parts of the keys, of `split_tiles` tiles at least
+  int longest;                             // keys of a sequence at most, as far as the host knows
+  float few_share;                         // not 0: parts of few_tiles() tiles at least
   bool causal, clear_rest, by_dies;
 };
 
@@ -51,6 +54,7 @@ struct RowBlock {
   int first;      // row of the block's first one in its sequence
   int rows;       // of the sequence
   int len, past;  // keys of the sequence; position of its first query
+  int longest;    // keys of the longest sequence, as far as they are known
 };
 
 // What workgroup `b` takes: a kv head and one of `items`.  Neighbouring workgroups run on different dies (8, in turn): each die gets
@@ -92,6 +96,8 @@ __device__ __forceinline__ RowBlock sequence_of(const AttentionParams& p, int b,
   r.rows = max(end - r.token, 0) * p.group;
   r.len = (int)min((long)max(of_lane(len, found), 0), (long)p.table_pages * p.page_size);
   r.past = r.len - (end - r.token);
+  r.longest = p.longest;
+  if (p.splits > 1 && p.seqs <= 62) r.longest = min(over_wave(len, 0, [](int a, int b) { return max(a, b); }), p.longest);   // (all lengths are here)
   return r;
 }
 
@@ -111,9 +117,24 @@ __device__ __forceinline__ void keys_seen(const AttentionParams& p, const RowBlo
   low = bounded && p.window > 0 ? max(r.past + t0 - p.window + 1, 0) : 0;
 }
 
-// The part of the tiles [first, last) of a block that split s takes; false where there is none.  Sets how many parts there are.
-__device__ __forceinline__ bool split_of(const AttentionParams& p, int s, int& first, int& last, int& parts) {
-  const int tiles = last - first, each = max(p.split_tiles, (tiles + p.splits - 1) / p.splits);
+// Tiles of a part at least, of `tiles` in all, in the form for few rows.  `share`: kv heads and their blocks of rows over 4096.  With t tiles
+// a workgroup takes some 0.6 t us, and joining the others 0.1 us a part, so that the square root of 0.15 times the tiles is about the
+// best for one sequence (8000 keys: 4 tiles 17.2 us, 2 19.1); with more of them about 4096 workgroups, which even out (64 sequences
+// of 800 to 4096 keys: 155 us with 8 tiles, 4 158, 16 164).
+__host__ __device__ __forceinline__ int few_tiles(int tiles, float share) {
+  const int least = (int)(share * (float)tiles), for_one = (int)__builtin_sqrtf(0.15f * (float)tiles + 0.25f);
+  const int most = least > for_one ? least : for_one;
+  return most < 2 ? 2 : most > 8 ? 8 : most;
+}
+
+// The part of the tiles [first, last) of a block that split s takes; false where there is none.  Sets how many parts there are.  Of how many
+// tiles a part is, the lengths say that there are, as the caller may not know them: 64 sequences of 800 to 4096 keys in 8-bit codes take
+// 91 us also where they might have had 131072, by parts chosen for those 344.
+__device__ __forceinline__ bool split_of(const AttentionParams& p, const RowBlock& r, int s, int& first, int& last, int& parts) {
+  const int tiles = last - first;
+  // few rows: parts of each sequence's own size; many: of one size for all, so that what is short is not cut for nothing
+  const int least = p.few_share > 0.0f ? few_tiles(tiles, p.few_share) : max(p.split_tiles, ((r.longest + kTile - 1) / kTile + p.splits - 1) / p.splits);
+  const int each = max(least, (tiles + p.splits - 1) / p.splits);
   parts = max((tiles + each - 1) / each, 1);
   first += s * each;
   last = min(last, first + each);

@@ -63,6 +63,13 @@ __device__ __forceinline__ float fp8_number(float y, float inverse) {
 }
 __device__ __forceinline__ float inverse_scale(const Pages& c, int head) { return 1.0f / c.scale[c.scale_heads ? head : 0]; }
 
+// (a launch has fewer than 2^32 threads a dimension)
+__device__ __forceinline__ long block_number() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 grid_of(long blocks) {
+  const long rows = (blocks + (1 << 23) - 1) >> 23;
+  return dim3((uint32_t)((blocks + rows - 1) / rows), (uint32_t)rows);
+}
+
 // Sum over `lanes` neighbouring lanes (a power of two, 4 at least), in every lane.
 __device__ __forceinline__ float sum_over(float v, int lanes) {
   auto moved_by = [](float x, auto ctrl) {
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(kThreads, VEC * sizeof(T) > 16 ? 3 : 4) void qk_nor
 #pragma clang fp contract(off)
   const int slot = threadIdx.x / p.lanes, j = threadIdx.x % p.lanes;
   const int tokens_here = kThreads / p.lanes / p.of_token;
-  const long token = (long)blockIdx.x * tokens_here + slot / p.of_token;
+  const long token = block_number() * tokens_here + slot / p.of_token;
   if (token >= p.tokens) return;
   const int turned = p.rotary / (2 * VEC);
   const bool turns = j < turned;
@@ -234,7 +241,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_any_kernel(const RopeParams p) {
 #pragma clang fp contract(off)
   const int lane = threadIdx.x & 63, all = p.heads + (p.cached ? 2 : 1) * p.kv_heads;
-  const long item = (long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
+  const long item = block_number() * (kThreads / 64) + threadIdx.x / 64;
   if (item >= p.tokens * all) return;
   const long token = item / all;
   const int h = item % all;
@@ -303,7 +310,7 @@ int launch_runs(RopeParams p, hipStream_t st) {
   // threads enough: 16384 tokens of 40 heads of 128 with norms 77 us, a head or two a thread 111; 4096 20.4 and 24.3.
   while (p.of_token > 1 && all / p.of_token < kAhead && p.tokens * (p.of_token / 2) * p.lanes >= 262144) p.of_token /= 2;
   const int tokens_here = slots / p.of_token;
-  qk_norm_rope_kernel<T, VEC><<<(uint32_t)((p.tokens + tokens_here - 1) / tokens_here), kThreads, 0, st>>>(p);
+  qk_norm_rope_kernel<T, VEC><<<grid_of((p.tokens + tokens_here - 1) / tokens_here), kThreads, 0, st>>>(p);
   return launch_status("qk_norm_rope_kernel");
 }
 
@@ -314,7 +321,7 @@ int launch(RopeParams p, hipStream_t st) {
   if (runs_fit(p, 4, sizeof(T)) && p.dim <= 512) return launch_runs<T, 4>(p, st);
   if (runs_fit(p, 2, sizeof(T)) && p.dim <= 256) return launch_runs<T, 2>(p, st);
   const long items = p.tokens * (p.heads + (p.cached ? 2 : 1) * p.kv_heads);
-  qk_norm_rope_any_kernel<T><<<(uint32_t)((items + kThreads / 64 - 1) / (kThreads / 64)), kThreads, 0, st>>>(p);
+  qk_norm_rope_any_kernel<T><<<grid_of((items + kThreads / 64 - 1) / (kThreads / 64)), kThreads, 0, st>>>(p);
   return launch_status("qk_norm_rope_any_kernel");
 }
 

@@ -357,9 +357,9 @@ def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
 
     key_cache, value_cache: (pages, page_size, kv_heads, head_dim) of any strides but the last (a layout with the heads before the
     slots is a transposed view), of query's type or float8_e4m3fn.  An 8-bit cache holds codes that stand for code * scale: the nearest
-    to y / scale, at most 448; k_scale and v_scale: float32, one number or one a kv head.  slot_mapping: (tokens,), int64 or int32:
+    to y / scale, at most 448; k_scale and v_scale: float32, one positive number or one a kv head.  slot_mapping: (tokens,), int64 or int32:
     token t goes to slot s % page_size of page s // page_size, s = slot_mapping[t]; nowhere where s is negative or past the last page.
-    Which of two tokens with the same slot stays is not defined.  Without a table and weights this is the plain append."""
+    Which of two tokens with the same slot stays is not defined, for each head anew.  Without a table and weights this is the plain append."""
     return _qk_norm_rope_append(query, key, value, key_cache, value_cache, slot_mapping, positions, cos_sin_cache, q_weight, k_weight,
                                 epsilon, is_neox, k_scale, v_scale)
 
@@ -387,8 +387,9 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     they are.  NaNs and infinities in what a query does not see do not reach it.  Pages that no query sees are not read; a
     page number outside the cache among the others makes the results NaN.
 
-    max_seq_len: the longest sequence, if the caller knows: how far the keys are split over workgroups is chosen for it, and for
-    all of the block table without it; results are right, if not the same bits, for any number.
+    max_seq_len: the longest sequence, if the caller knows: how far the keys may be split over workgroups is chosen for it, and for
+    all of the block table without it (a captured call whose lengths change does without); results are right, if not the same bits, for
+    any number.  scale, and softcap if not 0, from 1e-30 to 1e30; k_scale negative or NaN makes the results NaN.
     head_dim a multiple of 16, at most 256."""
     if scale is None:
         scale = query.shape[-1] ** -0.5

@@ -10,6 +10,7 @@ def rotary_rates(rotary_dim: int, base: float = 10000.0, scaling: dict | None = 
     """The angle of each pair per position, float64 (rotary_dim / 2,): base ** (-2 i / rotary_dim), and with `scaling`, as a model's
     configuration holds it ("rope_type" and its numbers):
 
+      default  as without
       linear   every rate divided by `factor`
       llama3   by wavelength: those longer than original_max_position_embeddings / low_freq_factor are divided by `factor`, those
                shorter than it / high_freq_factor stay, a straight line of the inverse wavelength between
@@ -20,7 +21,10 @@ def rotary_rates(rotary_dim: int, base: float = 10000.0, scaling: dict | None = 
     rates = float(base) ** -(torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
     if scaling is None:
         return rates
-    kind, factor = scaling["rope_type"], float(scaling["factor"])
+    kind = scaling["rope_type"]
+    if kind == "default":
+        return rates
+    factor = float(scaling["factor"])
     if kind == "linear":
         return rates / factor
     original = scaling["original_max_position_embeddings"]

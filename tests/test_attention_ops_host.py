@@ -244,3 +244,27 @@ def test_oracle_values():
     assert np.allclose(call(tree=np.array([[0], [1]])), [0, 4]) and np.allclose(call(tree=np.array([[2], [3]])), [8, 7])
     # a page that no query sees is not looked at
     assert np.allclose(ao.paged_attention(np.ones((1, 1, 1)), k, v, np.array([[99, 0]]), [2], [0, 1], 1.0, window=1)[0], 8)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(scale=1e-31), "scale"), (dict(scale=1e31), "scale"), (dict(cap=1e-50), "cap"), (dict(cap=1e-31), "cap"), (dict(cap=1e31), "cap")])
+def test_scales_that_float32_does_not_hold_are_refused(change, message):
+    _lib, lib = library()
+    assert attention_call(lib, _lib, **change) == _lib.E_INVALID and message in lib.sonar_attention_last_error().decode()
+
+
+@pytest.mark.parametrize("cache_dtype", [1, 3])
+@pytest.mark.parametrize("tokens,seqs,heads,kv_heads", [(1, 1, 32, 8), (64, 64, 32, 8), (256, 256, 32, 8), (4096, 4096, 32, 8), (192, 24, 32, 8),
+                                                       (1, 1, 128, 1), (8192, 1, 32, 8), (20000, 20000, 64, 8)])
+def test_scratch_for_long_tables_is_bounded(tokens, seqs, heads, kv_heads, cache_dtype):
+    """Sequences that might be very long do not take memory for it: at most 256 parts, and no call is
+    refused for the parts that it might have."""
+    _lib, lib = library()
+    for longest in (100, 5000, 131072, 2 ** 30):
+        size = lib.sonar_paged_attention_scratch_bytes(tokens, seqs, heads, kv_heads, 128, cache_dtype, longest, 0)
+        assert size <= 256 * tokens * heads * (128 * 4 + 8) + 16
+
+
+def test_default_rotary_scaling():
+    from sonar_amd import rotary
+    assert torch.equal(rotary.rotary_rates(64, 5e5, {"rope_type": "default"}), rotary.rotary_rates(64, 5e5))

@@ -170,3 +170,35 @@ def test_every_form(dtype, dim, fp8, extra):
     for lengths in (ONES, PIECES, [(3000, 1)], [(1500, 130)]):
         b = Batch(dim, lengths, kv_heads=1, dim=dim, dtype=dtype, fp8=fp8)
         b.check(b.call(**extra), **extra)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("lengths", [ONES, PIECES], ids=["few", "many"])
+@pytest.mark.parametrize("cap", [128.0, 129.0, 5e3, 1e7, 1e30])
+def test_large_caps(lengths, cap, fp8):
+    """A cap far above the scores hardly changes them, and is not off by a share of itself either: from 129 on a score below an eighth
+    of the cap is off by 2^-22 of itself (7 roundings of the series more), a larger one by 2^-22 of the cap, so by 2^-19 of itself."""
+    b = Batch(17, lengths, kv_heads=2, dim=64, fp8=fp8)
+    want, size, most = b.want(softcap=cap)
+    h, u = HALF_STEP["bf16"], 2.0 ** -24
+    e = (64 + 16) * u * most + 2.0 ** -22 + (cap * 2.0 ** -20 if cap <= 128 else most * 2.0 ** -19)
+    keys = max(n for n, _ in lengths)
+    limit = size * (h + 2 * e[:, :, None] + keys * u) + np.abs(want) * h + 2.0 ** -24
+    assert (np.abs(numbers(b.call(softcap=cap)) - want) <= limit).all()
+    if cap > 1e6:   # what is off by 2^-22 of the cap would not be near this
+        assert np.abs(want - b.want()[0]).max() < 1e-6
+
+
+@pytest.mark.parametrize("lengths", [ONES, PIECES], ids=["few", "many"])
+@pytest.mark.parametrize("softcap", [0.0, 1e-30, 30.0])
+def test_smallest_and_largest_scales(lengths, softcap):
+    """Scores next to nothing, whose weights are all one, and a scale of the codes that is 0: means of what is seen."""
+    b = Batch(18, lengths, kv_heads=2, dim=64, fp8=True)
+    b.check(b.call(scale=1e-30, softcap=softcap), scale=1e-30, softcap=softcap)
+    b.k_scale = torch.zeros(1)
+    b.check(b.call(scale=1e30), scale=1e30)
+    for bad in (-1.0, float("nan")):
+        b.k_scale = torch.tensor([bad])
+        got = b.call(softcap=softcap)
+        seen = torch.cat([torch.arange(n - q, n) >= 0 for n, q in lengths if q]).to(DEV)
+        assert got[seen].isnan().all()

@@ -336,3 +336,42 @@ def test_opcheck():
     torch.library.opcheck(s.qk_norm_rope, (q, kv, at, cos_sin, w, w, 1e-6, True), test_utils=utils)
     torch.library.opcheck(s.qk_norm_rope, (q, kv, None, None, None, None, 1e-6, True), test_utils=utils)
     torch.library.opcheck(s.qk_norm_rope_append, (q, kv, kv, k, v, at, at, cos_sin, w, None, 1e-6, False, None, None), test_utils=utils)
+
+
+def test_a_table_that_sequences_share():
+    """One row of pages for all sequences, as a view without a copy: drafts of one prompt."""
+    from sonar_amd import ops
+    b = Batch(19, [(300, 1)], heads=4, kv_heads=2, dim=64)
+    d = lambda t: t.to(DEV)  # noqa: E731
+    q = torch.cat([b.q] * 5)
+    lens, starts = torch.full((5,), 300, dtype=torch.int32), torch.arange(6, dtype=torch.int32)
+    got = ops.paged_attention(d(q), d(b.k), d(b.v), d(b.table).expand(5, -1), d(lens), d(starts))
+    assert torch.equal(got, ops.paged_attention(d(q), d(b.k), d(b.v), d(b.table.repeat(5, 1)), d(lens), d(starts)))
+    b.check(got[:1])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("seqs", [4, 70], ids=["few", "many"])
+def test_starts_that_do_not_rise(seqs, fp8):
+    """Not allowed, and then nothing is said of the results; but what lies around them is left alone, and the call ends."""
+    rng = np.random.default_rng(20)
+    for queries in (1, 30):
+        b = Batch(20, [(200, queries)] * seqs, heads=4, kv_heads=2, dim=64, fp8=fp8)
+        tokens = len(b.q)
+        for starts in (rng.permutation(seqs + 1) * queries, np.full(seqs + 1, tokens), np.arange(seqs, -1, -1) * queries,
+                       rng.integers(-1000, 1000, seqs + 1), rng.integers(-2 ** 31, 2 ** 31, seqs + 1)):
+            b.starts = torch.from_numpy(starts.astype(np.int32))
+            around = torch.full((tokens + 200, 4, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+            b.call(out=around[100:100 + tokens])
+            assert (around[:100] == 7.0).all() and (around[100 + tokens:] == 7.0).all()
+
+
+def test_lengths_known_only_on_the_device():
+    """A table wide enough for any sequence, and lengths far below it, of one sequence and of more than a wavefront looks at."""
+    for lengths in ([(700, 1)], [(3000, 1), (40, 1)], [(1200, 20), (900, 33)], [(40 + 13 * i, 1 + i % 3) for i in range(80)]):
+        for fp8 in (False, True):
+            b = Batch(21, lengths, heads=4, kv_heads=1, dim=128, fp8=fp8)
+            b.check(b.call())
+            b.table = torch.nn.functional.pad(b.table, (0, 8192 - b.table.shape[1]), value=-1)
+            b.check(b.call())
+            b.check(b.call(100))

@@ -235,3 +235,19 @@ def test_a_cache_past_32_bits():
     assert torch.equal(got[slots].view(FP8).float(), want.float()) and int((got != 0).sum()) <= 3 * 64
     del keys, values, got
     torch.cuda.empty_cache()
+
+
+def test_more_heads_than_a_launch_has_threads_for():
+    """Every head a wavefront, in more wavefronts than 2^32 threads have: odd heads, number by number."""
+    from sonar_amd import ops
+    tokens, gen = 36_000_000, torch.Generator(device=DEV).manual_seed(3)
+    q, k = (torch.randn((tokens, 1, 3), device=DEV, generator=gen, dtype=torch.float16) for _ in range(2))
+    got_q, got_k = ops.qk_norm_rope(q, k)
+    assert torch.equal(got_q, q) and torch.equal(got_k, k)
+
+
+def test_one_cache_for_keys_and_values_is_refused():
+    from sonar_amd import ops
+    x, cache = torch.zeros((2, 2, 64), device=DEV), torch.zeros((4, 16, 2, 64), device=DEV)
+    with pytest.raises(RuntimeError, match="(?i)overlap|memory"):
+        ops.qk_norm_rope_append(x, x, x, cache, cache, torch.zeros(2, dtype=torch.int64, device=DEV))
