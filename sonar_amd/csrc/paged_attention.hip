@@ -85,7 +85,7 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
                             p.tree == nullptr ? nullptr : p.tree + token * p.tree_words, p.tree_words, p.causal};
           if (!(sight.of(key) & 1)) continue;
           if (parts > 1) {
-            p.part_o[(((long)split * p.tokens + token) * p.heads + head) * p.dim + d] += v;
+            p.part_o[part_at(p, r, split, kv_head, row) * p.dim + d] += v;
           } else {
             T* to = (T*)p.out + token * p.out_token + head * p.out_head + d;
             *to = (T)((float)*to + v);
@@ -136,11 +136,20 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   int* const flags = (int*)lds;   // behind the last tile
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int item, kv_head;
-  item_of(p, p.blocks * p.splits, blockIdx.x, item, kv_head);
-  const int split = item / p.blocks;
-  // the blocks of the last tokens, which see the most keys, first
-  const RowBlock r = row_block<kRows>(p, p.blocks - 1 - item % p.blocks);
+  int kv_head, split;
+  RowBlock r;
+  const int others = (int)blockIdx.x - p.blocks * p.splits * p.kv_heads;
+  if (others < 0) {
+    int item;
+    item_of(p, p.blocks * p.splits, blockIdx.x, item, kv_head);
+    split = item / p.blocks;
+    // the blocks of the last tokens, which see the most keys, first
+    r = row_block<kRows>(p, p.blocks - 1 - item % p.blocks);
+  } else {   // the parts but the first of a sequence's last rows
+    kv_head = others % p.kv_heads, split = 1 + others / p.kv_heads / p.seqs;
+    r = last_rows(p, others / p.kv_heads % p.seqs);
+    if (!is_tail(r)) return;
+  }
   if (r.first < 0 || r.first >= r.rows || (r.seq == p.seqs && !p.clear_rest)) return;   // (negative where starts do not rise)
 
   const int row = r.first + wave * 32 + (lane & 31), half = lane >> 5;
@@ -432,7 +441,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   if (found & 1) sum = __builtin_nanf("");
   if (parts > 1) {
     if (row < r.rows) {
-      const long at = ((long)split * p.tokens + token) * p.heads + head;
+      const long at = part_at(p, r, split, kv_head, row);
       if (half == 0) p.part_ml[at] = make_float2(most, sum);
       float* to = p.part_o + at * p.dim + 4 * half;
 #pragma unroll
@@ -714,7 +723,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_
   __shared__ float4 numbers[WAVES][LANES];
   __shared__ float2 sums[WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = lane % LANES * 4;
-  const long row = WAVES == 1 ? (long)blockIdx.x * 4 + wave : (long)blockIdx.x, step = (long)p.tokens * p.heads;
+  const long row = WAVES == 1 ? (long)blockIdx.x * 4 + wave : (long)blockIdx.x;
+  const long step = p.tails > 0 ? (long)p.seqs * p.kv_heads * kTail : (long)p.tokens * p.heads;
   if (row >= step) return;
   float2 ml[kBatch];
   floatx4_t o[kBatch];
@@ -727,16 +737,26 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_
     }
   };
   int s = (WAVES == 1 ? 0 : wave * kAtOnce) + lane / LANES;
-  load(s, p.splits);
-  const int token = row / p.heads, head = row % p.heads, kv_head = head / p.group;
-  RowBlock r = sequence_of(p, token, [](int, int start) { return start; });
-  if (r.seq == p.seqs || token < r.token) return;
-  r.first = ((token - r.token) * p.group + head % p.group) / p.rows * p.rows;
+  int token, head, kv_head;
+  RowBlock r;
+  if (p.tails > 0) {   // (most rows have no parts)
+    kv_head = row / kTail % p.kv_heads, r = last_rows(p, row / kTail / p.kv_heads);
+    const int in = r.first + row % kTail;
+    if (!is_tail(r) || in >= r.rows) return;
+    token = r.token + in / p.group, head = kv_head * p.group + in % p.group;
+  } else {
+    load(s, p.splits);
+    token = row / p.heads, head = row % p.heads, kv_head = head / p.group;
+    r = sequence_of(p, token, [](int, int start) { return start; });
+    if (r.seq == p.seqs || token < r.token) return;
+    r.first = ((token - r.token) * p.group + head % p.group) / p.rows * p.rows;
+  }
   int low, high;
   keys_seen(p, r, r.first / p.group, min(r.first + p.rows - 1, r.rows - 1) / p.group, low, high);
   int first = low / kTile, last = high > low ? (high + kTile - 1) / kTile : low / kTile, parts;
   split_of(p, r, 0, first, last, parts);
   if (parts <= 1) return;
+  if (p.tails > 0) load(s, parts);
   float most = -kInfinity, sum = 0.0f;
   floatx4_t out{};
   // (to the powers of two of another maximum; both -infinity where there is nothing yet)
@@ -812,7 +832,7 @@ constexpr bool eight_waves(int dp) { return dp == 128; }
 
 struct Plan {
   int rows;   // of a block: 16 in the form for few rows, 128 and 256 in that for many
-  long blocks, splits, split_tiles;
+  long blocks, splits, split_tiles, tails;
   int longest;
   float few_share;
   size_t ml_bytes, o_bytes;
@@ -862,18 +882,25 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     plan.splits = parts, plan.split_tiles = std::min<int64_t>((longest + parts - 1) / parts, 4);
   }
   if (tokens * heads >= 1LL << 24 || plan.blocks * kv_heads * plan.splits >= 1LL << 24) plan.splits = 1;   // (2^32 threads are a launch's most)
-  if (plan.splits > 1) {
-    plan.ml_bytes = (size_t)(plan.splits * tokens * heads) * sizeof(float2);
+  // Many rows, but not of each sequence: single tokens beside prompts.  Their keys are split, though the rest has workgroups enough, as
+  // a workgroup for all of them would end long after the others (one token with 100000 keys beside 16 prompts of 1000: 1816 us, so
+  // 392; parts of 4 tiles at least: 9 sequences with a window of 1024 92 us, 2 tiles 95, 8 101, unsplit 108).
+  if (!few && plan.splits == 1 && seqs > 1 && queries * group > kTail && 2 * queries < max_seq_len && seqs * kv_heads <= 8192)
+    plan.tails = std::min<int64_t>(std::max<int64_t>(2048 / (seqs * kv_heads), 4), (longest + 3) / 4);
+  if (plan.tails < 2) plan.tails = 0;
+  if (plan.splits > 1 || plan.tails > 0) {
+    const int64_t rows = plan.tails > 0 ? plan.tails * seqs * kv_heads * kTail : plan.splits * tokens * heads;
+    plan.ml_bytes = (size_t)rows * sizeof(float2);
     plan.ml_bytes = (plan.ml_bytes + 15) / 16 * 16;
-    plan.o_bytes = (size_t)(plan.splits * tokens * heads * head_dim) * sizeof(float);
+    plan.o_bytes = (size_t)(rows * head_dim) * sizeof(float);
   }
   return plan;
 }
 
 template <typename T, int DP>
 int launch_join(const AttentionParams& p, hipStream_t st) {
-  if (p.splits == 1) return SONAR_OK;
-  const long rows = (long)p.tokens * p.heads;
+  if (p.splits == 1 && p.tails == 0) return SONAR_OK;
+  const long rows = p.tails > 0 ? (long)p.seqs * p.kv_heads * kTail : (long)p.tokens * p.heads;
   // (a workgroup a row where parts are many and rows few: one sequence of 8000 keys 18 us, a wavefront a row 24)
   if (p.splits > 8 && rows <= 256) attention_join_kernel<T, DP / 4, 8><<<(uint32_t)rows, 512, 0, st>>>(p);
   else attention_join_kernel<T, DP / 4, 1><<<(uint32_t)((rows + 3) / 4), 256, 0, st>>>(p);
@@ -883,7 +910,7 @@ int launch_join(const AttentionParams& p, hipStream_t st) {
 template <typename K>
 int launch_one(K kernel, const AttentionParams& p, int waves, int lds, const char* name, hipStream_t st) {
   if (lds > 65536) SONAR_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  kernel<<<(uint32_t)(p.blocks * p.kv_heads * p.splits), waves * 64, lds, st>>>(p);
+  kernel<<<(uint32_t)(p.blocks * p.kv_heads * p.splits + std::max(p.tails - 1, 0) * p.seqs * p.kv_heads), waves * 64, lds, st>>>(p);
   return launch_status(name);
 }
 
@@ -978,7 +1005,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   SONAR_REQUIRE(seq_lens && (table_pages == 0 || (block_table && table_stride >= table_pages && pages >= 1 && key_cache->data && value_cache->data)),
                 "seq_lens, a block_table of %ld pages a row and caches with pages are needed", (long)table_pages);
   Plan plan = plan_of(tokens, seqs, heads, kv_heads, head_dim, cache_dtype == SONAR_CACHE_FP8, max_seq_len, window);
-  if (scratch_bytes < plan.ml_bytes + plan.o_bytes || scratch == nullptr) plan.splits = 1;
+  if (scratch_bytes < plan.ml_bytes + plan.o_bytes || scratch == nullptr) plan.splits = 1, plan.tails = 0;
   SONAR_REQUIRE((uintptr_t)scratch % 16 == 0, "scratch must be 16-byte aligned");
   SONAR_REQUIRE(plan.blocks * kv_heads * plan.splits < (1LL << 24),
                 "%ld tokens of %ld sequences and %ld heads take too many workgroups", (long)tokens, (long)seqs, (long)heads);
@@ -1000,7 +1027,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   p.page_shift = 31 + log, p.page_magic = (uint32_t)((1ULL << p.page_shift) / (uint64_t)page_size + 1);
   p.page_size = (int)page_size, p.pages = (int)pages, p.table_pages = (int)table_pages;
   p.tokens = (int)tokens, p.seqs = (int)seqs, p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads);
-  p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles, p.longest = plan.longest, p.few_share = plan.few_share;
+  p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles, p.tails = (int)plan.tails, p.longest = plan.longest, p.few_share = plan.few_share;
   p.by_dies = plan.rows == 16;
   const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
   hipStream_t st = (hipStream_t)stream;

@@ -13,6 +13,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kTile = 64;   // keys
+constexpr int kTail = 32;   // rows
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kInfinity = __builtin_inff();
 
@@ -35,13 +36,14 @@ struct AttentionParams {
   long out_token, out_head;
   const float* slopes;
   const uint64_t* tree;
-  float* part_o;    // [split][token][head][dim], not yet divided by the sum
-  float2* part_ml;  // [split][token][head]: running maximum (of scores times log2 e) and sum
+  float* part_o;    // [split][token][head][dim], not yet divided by the sum; with tails [split][seq][kv head][row of kTail][dim]
+  float2* part_ml;  // the same without dim: running maximum (of scores times log2 e) and sum
   float scale, cap;
   uint32_t page_magic;   // key / page_size = key * page_magic >> page_shift for keys below 2^31
   int page_shift, page_size, pages, table_pages;
   int window, tree_words, tokens, seqs, heads, kv_heads, group, dim;
   int rows, blocks, splits, split_tiles;   // rows of a block, blocks of rows; at most `splits` parts of the keys, of `split_tiles` tiles at least
+  int tails;                               // not 0: at most so many parts of the sequences' last rows, where those are no more than kTail
   int longest;                             // keys of a sequence at most, as far as the host knows
   float few_share;                         // not 0: parts of few_tiles() tiles at least
   bool causal, clear_rest, by_dies;
@@ -110,6 +112,17 @@ __device__ __forceinline__ RowBlock row_block(const AttentionParams& p, int b) {
   return r;
 }
 
+// The last rows of sequence `i`, in blocks of p.rows.
+__device__ __forceinline__ RowBlock last_rows(const AttentionParams& p, int i) {
+  RowBlock r;
+  r.seq = i, r.token = start_of(p, i), r.longest = p.longest;
+  const int queries = max(start_of(p, i + 1) - r.token, 0);
+  r.rows = queries * p.group, r.first = max(r.rows - 1, 0) / p.rows * p.rows;
+  r.len = (int)min((long)max(p.lens[i], 0), (long)p.table_pages * p.page_size), r.past = r.len - queries;
+  return r;
+}
+__device__ __forceinline__ bool is_tail(const RowBlock& r) { return r.rows - r.first <= kTail; }
+
 // Keys [low, high) that a query of tokens [t0, t1] of the sequence may see, t counted from its first query.
 __device__ __forceinline__ void keys_seen(const AttentionParams& p, const RowBlock& r, int t0, int t1, int& low, int& high) {
   const bool bounded = p.causal && p.tree == nullptr;
@@ -133,12 +146,18 @@ __host__ __device__ __forceinline__ int few_tiles(int tiles, float share) {
 __device__ __forceinline__ bool split_of(const AttentionParams& p, const RowBlock& r, int s, int& first, int& last, int& parts) {
   const int tiles = last - first;
   // few rows: parts of each sequence's own size; many: of one size for all, so that what is short is not cut for nothing
-  const int least = p.few_share > 0.0f ? few_tiles(tiles, p.few_share) : max(p.split_tiles, ((r.longest + kTile - 1) / kTile + p.splits - 1) / p.splits);
-  const int each = max(least, (tiles + p.splits - 1) / p.splits);
+  const int least = p.tails > 0 ? (is_tail(r) ? 4 : max(tiles, 1)) : p.few_share > 0.0f ? few_tiles(tiles, p.few_share) : max(p.split_tiles, ((r.longest + kTile - 1) / kTile + p.splits - 1) / p.splits);
+  const int most = p.tails > 0 ? p.tails : p.splits, each = max(least, (tiles + most - 1) / most);
   parts = max((tiles + each - 1) / each, 1);
   first += s * each;
   last = min(last, first + each);
   return s < parts;
+}
+
+// Where part `split` of a row lies.
+__device__ __forceinline__ long part_at(const AttentionParams& p, const RowBlock& r, int split, int kv_head, int row) {
+  if (p.tails > 0) return (((long)split * p.seqs + r.seq) * p.kv_heads + kv_head) * kTail + row - r.first;
+  return ((long)split * p.tokens + r.token + row / p.group) * p.heads + kv_head * p.group + row % p.group;
 }
 
 // Which of the 64 keys from `base` on a query sees, a bit each.

@@ -202,3 +202,57 @@ def test_smallest_and_largest_scales(lengths, softcap):
         got = b.call(softcap=softcap)
         seen = torch.cat([torch.arange(n - q, n) >= 0 for n, q in lengths if q]).to(DEV)
         assert got[seen].isnan().all()
+
+
+# prompts, pieces of them and single tokens: many rows in all, few of some sequences
+MIXED = [(150, 150), (700, 1), (300, 130), (9, 1), (260, 33), (520, 8), (129, 129), (64, 1), (200, 140), (33, 32), (0, 0), (321, 1)]
+
+
+def parts_of_tails(b, kv_heads):
+    """How many parts the last rows of a sequence get, from the scratch memory that is asked for (csrc/paged_attention.hip: 32 rows a
+    sequence, kv head and part); 0 where none."""
+    from sonar_amd import _lib
+    lib = _lib.load_attention()
+    size = lib.sonar_paged_attention_scratch_bytes(len(b.q), len(b.lengths), b.q.shape[1], kv_heads, b.dim, _lib.CACHE_FP8 if b.k_scale is not None else 1,
+                                                   b.table.shape[1] * b.k.shape[1], 0)
+    return size / (len(b.lengths) * kv_heads * 32 * (4 * b.dim + 8))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dim", [64, 112, 128, 256])
+@pytest.mark.parametrize("extra", [{}, dict(softcap=20.0), dict(window=300), dict(causal=False), dict(alibi_slopes=torch.rand(64, generator=torch.Generator().manual_seed(1)))],
+                         ids=["plain", "capped", "window", "all", "sloped"])
+def test_few_rows_beside_many(dim, fp8, extra):
+    """Workgroups enough without a split: only the last rows of each sequence, where they are few, are split over the keys."""
+    b = Batch(22, MIXED, heads=64, kv_heads=64, dim=dim, fp8=fp8, behind=3)
+    assert parts_of_tails(b, 64) in (2, 3, 4)
+    got = b.call(**extra)
+    b.check(got, **extra)
+    assert torch.equal(got, b.call(**extra)) and (got[-3:] == 0).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_few_rows_beside_many_trees(fp8):
+    b = Batch(23, MIXED, heads=64, kv_heads=32, dim=128, fp8=fp8, tree_words=2)
+    assert parts_of_tails(b, 32) in (2, 3, 4)
+    b.check(b.call())
+
+
+def test_few_rows_beside_many_specials():
+    """An infinity and a NaN in the values of a sequence's last key, which the last query alone sees, and in a part of its own; a bad page."""
+    b = Batch(24, MIXED, heads=64, kv_heads=64, dim=128)
+    assert parts_of_tails(b, 64) >= 2
+    clean = numbers(b.call())
+    want, limit = b.limits()
+    at = 519   # of the sixth sequence: 520 keys, 8 queries
+    page = int(b.table[5, at // 16])
+    b.v[page, at % 16, :, 3], b.v[page, at % 16, :, 5] = float("inf"), float("nan")
+    got = numbers(b.call())
+    last = int(b.starts[6]) - 1
+    assert np.isposinf(got[last, :, 3]).all() and np.isnan(got[last, :, 5]).all()
+    others = np.ones(got.shape, dtype=bool)
+    others[last, :, 3], others[last, :, 5] = False, False
+    assert (np.abs(got - want)[others] <= limit[others]).all()
+    b.table[1, 20] = 10 ** 6   # a page of the second sequence
+    got = numbers(b.call())
+    assert np.isnan(got[150]).all() and not np.isnan(got[:150]).any() and np.isfinite(clean).all()

@@ -375,3 +375,22 @@ def test_lengths_known_only_on_the_device():
             b.table = torch.nn.functional.pad(b.table, (0, 8192 - b.table.shape[1]), value=-1)
             b.check(b.call())
             b.check(b.call(100))
+
+
+def test_one_long_sequence_beside_prompts():
+    """A single token with 40000 keys beside prompts that fill the card: its keys are split, and the last part is there."""
+    from sonar_amd import ops
+    lengths = [(400, 400)] * 12 + [(40000, 1)]
+    b = Batch(25, lengths, heads=32, kv_heads=8, dim=128)
+    got = b.call()
+    alone = Batch(25, lengths, heads=32, kv_heads=8, dim=128)
+    d = lambda t: t.to(DEV)  # noqa: E731
+    one = ops.paged_attention(d(alone.q[-1:]), d(alone.k), d(alone.v), d(alone.table[-1:]), d(alone.lens[-1:]), d(torch.tensor([0, 1], dtype=torch.int32)))
+    k = alone.k[alone.table[-1].long()].reshape(-1, 8, 128)[:40000].double().repeat_interleave(4, 1)
+    v = alone.v[alone.table[-1].long()].reshape(-1, 8, 128)[:40000].double().repeat_interleave(4, 1)
+    weights = (torch.einsum("hd,khd->hk", alone.q[-1].double(), k) * 128 ** -0.5).softmax(1)
+    want, size = torch.einsum("hk,khd->hd", weights, v), torch.einsum("hk,khd->hd", weights, v.abs())
+    h = HALF_STEP["bf16"]   # (the fp32 sums' share, 40000 keys of 2^-24, is 2^-8.7 of the mean of |v| in the worst order)
+    limit = size * (h + 2.0 ** -8.7 + 2.0 ** -12) + want.abs() * h
+    for x in (got[-1], one[0]):
+        assert ((x.double().cpu() - want).abs() <= limit).all()
