@@ -6,10 +6,6 @@
  * stream), all work enqueued on that stream, no synchronisation with the host, 0 or a negative SONAR_E_* code, nothing
  * launched when a call fails.  sonar_attention_last_error() returns the calling thread's message.  The element types are
  * SONAR_DTYPE_F16 / _BF16 / _F32.  Strides count elements.  Nothing is kept from one call to the next.
- *
- * Counterparts in the reference, which reaches them as ops of its own extensions:
- *   sonar_qk_norm_rope     -> _C::rotary_embedding, _C::fused_qk_norm_rope, _C_cache_ops::reshape_and_cache_flash
- *   sonar_paged_attention  -> the attention of a ragged batch over a paged cache
  */
 #ifndef SONAR_ATTENTION_H_
 #define SONAR_ATTENTION_H_

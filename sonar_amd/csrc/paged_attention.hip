@@ -98,10 +98,12 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
 // ---------------------------------------------------------------- many rows
 // A workgroup takes 32 rows of a kv head for each of its WAVES wavefronts, and walks the keys in tiles of 64 that they share through
 // LDS, two tiles there: while one is worked on, the next one is on its way.  Bound by the matrix pipes and the vector units together:
-// 8192 tokens of 32 heads of 128 (8 kv heads) in bf16 take 567 us, 970 TFLOP/s, with 43 % of the pipes' cycles; the same without its
-// copies to LDS 489, without its reads of LDS too 442.  Each step of the way there, at that size: copies through registers and
-// products, weights, products one after the other 769; addresses found once a key 656; scores a half tile ahead 612; instructions
-// in turn 586 (heads of 256: 466 to 365 for 4096 tokens); copies straight into LDS 574.
+// 8192 tokens of 32 heads of 128 (8 kv heads) in bf16 take 550 us, 1000 TFLOP/s, with 43 % of the pipes' cycles.  Each step of the way
+// there, at that size: copies through registers and products, weights, products one after the other 769; addresses found once a key
+// 656; scores a half tile ahead 612; instructions in turn 586 (heads of 256: 466 to 365 for 4096 tokens); copies straight into
+// LDS 574 (without them 489, without the reads of LDS too 442); wavefronts without rows copy only 567; first copies all at once and
+// results through LDS 550.  Other orders of the instructions and the heads of an item on one die gave nothing.  Where a sequence
+// has few rows (64 sequences of 800 to 4096 keys, 4 rows each) it is memory: 142 us, 4.6 TB/s, what a large copy reaches less 4 %.
 
 // A row of a tile in LDS has no gap, as the copies straight into LDS leave none: its pieces of 16 bytes are swapped instead, by
 // the row's number, so that the lanes which read at once find different banks: 16 lanes a piece of a row each of the keys, 32 lanes
@@ -483,7 +485,10 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
 // ---------------------------------------------------------------- few rows
 // A workgroup takes 16 rows of a kv head, and its wavefronts take 32 keys in turn, each with a maximum, a sum and an output
 // of its own, which are joined at the end.  Keys go from memory straight into the registers of the product, values through a piece
-// of LDS that is the wavefront's own, to be turned there: no wavefront waits for another until the end.
+// of LDS that is the wavefront's own, to be turned there: no wavefront waits for another until the end.  Bound by memory where there is
+// much to read (64 sequences of 800 to 4096 keys of 8-bit codes: 90 us, 3.7 TB/s; what widens them takes the rest), else by the trips to
+// memory one after the other: lengths, page numbers, keys (one sequence of 700 keys: 6 us of the 9.7, the join the rest).  Two units'
+// loads on their way at once, which cost a wavefront a SIMD, gave nothing (8000 keys 18.4 us for 17.2, heads of 64 55 for 53), nor did 8 wavefronts.
 constexpr int kFew = 4;      // wavefronts of a workgroup
 constexpr int kUnit = 32;    // keys that a wavefront takes at once
 
@@ -716,7 +721,8 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
 // ---------------------------------------------------------------- the parts of a split joined
 // out = sum over the parts of 2^(m_i - m) o_i, divided by that of their sums, with a running maximum m for each group of lanes.  WAVES
 // wavefronts a row (1: four rows a workgroup); LANES lanes hold a row's numbers, four each, so that a wavefront reads 64 / LANES
-// parts at once.  The first parts are read before it is known how many there are: one trip to memory less.
+// parts at once.  The first parts are read before it is known how many there are: one trip to memory less.  Bound by those trips where
+// rows are few (32 rows of 6 parts: 3 us), else by memory (24 sequences of up to 60 drafts, 32 heads in 2 parts: 48 MB, 15 us).
 template <typename T, int LANES, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_kernel(const AttentionParams p) {
   constexpr int kAtOnce = 64 / LANES, kStep = WAVES * kAtOnce, kBatch = 4;
@@ -737,15 +743,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_
     }
   };
   int s = (WAVES == 1 ? 0 : wave * kAtOnce) + lane / LANES;
+  load(s, p.splits);
   int token, head, kv_head;
   RowBlock r;
-  if (p.tails > 0) {   // (most rows have no parts)
+  if (p.tails > 0) {   // (most rows have no parts; the first one's place was read)
     kv_head = row / kTail % p.kv_heads, r = last_rows(p, row / kTail / p.kv_heads);
     const int in = r.first + row % kTail;
     if (!is_tail(r) || in >= r.rows) return;
     token = r.token + in / p.group, head = kv_head * p.group + in % p.group;
   } else {
-    load(s, p.splits);
     token = row / p.heads, head = row % p.heads, kv_head = head / p.group;
     r = sequence_of(p, token, [](int, int start) { return start; });
     if (r.seq == p.seqs || token < r.token) return;

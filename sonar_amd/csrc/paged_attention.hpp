@@ -99,7 +99,7 @@ __device__ __forceinline__ RowBlock sequence_of(const AttentionParams& p, int b,
   r.len = (int)min((long)max(of_lane(len, found), 0), (long)p.table_pages * p.page_size);
   r.past = r.len - (end - r.token);
   r.longest = p.longest;
-  if (p.splits > 1 && p.seqs <= 62) r.longest = min(over_wave(len, 0, [](int a, int b) { return max(a, b); }), p.longest);   // (all lengths are here)
+  if (p.splits > 1 && p.few_share == 0.0f && p.seqs <= 62) r.longest = min(over_wave(len, 0, [](int a, int b) { return max(a, b); }), p.longest);   // (all lengths are here)
   return r;
 }
 
@@ -135,9 +135,9 @@ __device__ __forceinline__ void keys_seen(const AttentionParams& p, const RowBlo
 // best for one sequence (8000 keys: 4 tiles 17.2 us, 2 19.1); with more of them about 4096 workgroups, which even out (64 sequences
 // of 800 to 4096 keys: 155 us with 8 tiles, 4 158, 16 164).
 __host__ __device__ __forceinline__ int few_tiles(int tiles, float share) {
-  const int least = (int)(share * (float)tiles), for_one = (int)__builtin_sqrtf(0.15f * (float)tiles + 0.25f);
-  const int most = least > for_one ? least : for_one;
-  return most < 2 ? 2 : most > 8 ? 8 : most;
+  const int for_many = (int)(share * (float)tiles);
+  const int for_one = 2 + (tiles >= 59) + (tiles >= 105) + (tiles >= 165) + (tiles >= 239) + (tiles >= 325) + (tiles >= 425);   // 3 to 8 squared
+  return for_many < for_one ? for_one : for_many > 8 ? 8 : for_many;
 }
 
 // The part of the tiles [first, last) of a block that split s takes; false where there is none.  Sets how many parts there are.  Of how many

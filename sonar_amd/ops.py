@@ -334,8 +334,8 @@ def topk_routing(gating_output: torch.Tensor, topk: int, scoring_func: str = "so
 def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor | None = None,
                  cos_sin_cache: torch.Tensor | None = None, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                  epsilon: float = 1e-6, is_neox: bool = True):
-    """Norm of each query and key head and rotation by the token's position, in one launch (the reference's rotary_embedding and
-    fused_qk_norm_rope): (query, key), new tensors of the inputs' shapes.
+    """Norm of each query and key head and rotation by the token's position, in one launch: (query, key), new tensors of the inputs'
+    shapes.
 
       y = x / sqrt(mean(x^2) + epsilon) * weight over head_dim, where a weight is given;
       the first rotary_dim numbers in pairs (a, b) -> (a cos - b sin, b cos + a sin), where a table is given
@@ -352,8 +352,7 @@ def qk_norm_rope_append(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
                         slot_mapping: torch.Tensor, positions: torch.Tensor | None = None, cos_sin_cache: torch.Tensor | None = None,
                         q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, epsilon: float = 1e-6,
                         is_neox: bool = True, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
-    """`qk_norm_rope` whose keys go, with the values, to the pages of a cache (the reference's reshape_and_cache_flash on the way):
-    returns the queries.
+    """`qk_norm_rope` whose keys go, with the values, to the pages of a cache: returns the queries.
 
     key_cache, value_cache: (pages, page_size, kv_heads, head_dim) of any strides but the last (a layout with the heads before the
     slots is a transposed view), of query's type or float8_e4m3fn.  An 8-bit cache holds codes that stand for code * scale: the nearest
