@@ -98,7 +98,7 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
 // ---------------------------------------------------------------- many rows
 // A workgroup takes 32 rows of a kv head for each of its WAVES wavefronts, and walks the keys in tiles of 64 that they share through
 // LDS, two tiles there: while one is worked on, the next one is on its way.  Bound by the matrix pipes and the vector units together:
-// 8192 tokens of 32 heads of 128 (8 kv heads) in bf16 take 550 us, 1000 TFLOP/s, with 43 % of the pipes' cycles.  Each step of the way
+// 8192 tokens of 32 heads of 128 (8 kv heads) in bf16 take 550 us, 1000 TFLOP/s, with 48 % of the pipes' cycles.  Each step of the way
 // there, at that size: copies through registers and products, weights, products one after the other 769; addresses found once a key
 // 656; scores a half tile ahead 612; instructions in turn 586 (heads of 256: 466 to 365 for 4096 tokens); copies straight into
 // LDS 574 (without them 489, without the reads of LDS too 442); wavefronts without rows copy only 567; first copies all at once and
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
 // of its own, which are joined at the end.  Keys go from memory straight into the registers of the product, values through a piece
 // of LDS that is the wavefront's own, to be turned there: no wavefront waits for another until the end.  Bound by memory where there is
 // much to read (64 sequences of 800 to 4096 keys of 8-bit codes: 90 us, 3.7 TB/s; what widens them takes the rest), else by the trips to
-// memory one after the other: lengths, page numbers, keys (one sequence of 700 keys: 6 us of the 9.7, the join the rest).  Two units'
+// memory one after the other: lengths, page numbers, keys (one sequence of 700 keys: 7 us, and 4 the join; 9.7 both).  Two units'
 // loads on their way at once, which cost a wavefront a SIMD, gave nothing (8000 keys 18.4 us for 17.2, heads of 64 55 for 53), nor did 8 wavefronts.
 constexpr int kFew = 4;      // wavefronts of a workgroup
 constexpr int kUnit = 32;    // keys that a wavefront takes at once

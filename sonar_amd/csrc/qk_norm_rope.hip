@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kThreads, VEC * sizeof(T) > 16 ? 3 : 4) void qk_nor
 }
 
 // Any head_dim, rotary_dim, stride and alignment: a wavefront a head, number by number, the head read again after its norm.  Bound by
-// the instructions a number, not by memory; no layout that a model here has comes to it.
+// the instructions a number and half-empty lines, not by memory: 16384 tokens of 40 heads of 127 360 us, of 128 in the form above 71.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_any_kernel(const RopeParams p) {
 #pragma clang fp contract(off)
