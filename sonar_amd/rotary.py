@@ -42,12 +42,25 @@ def rotary_rates(rotary_dim: int, base: float = 10000.0, scaling: dict | None = 
     return rates * stay + rates / factor * (1 - stay)
 
 
+def _yarn_size(scaling: dict) -> float:
+    """What yarn multiplies cosines and sines by."""
+    factor = scaling["factor"]
+    if scaling.get("attention_factor"):
+        return scaling["attention_factor"]
+    size = lambda m: 0.1 * m * math.log(factor) + 1 if factor > 1 else 1.0  # noqa: E731
+    queries, keys = scaling.get("mscale"), scaling.get("mscale_all_dim")
+    if queries and keys:
+        return size(queries) / size(keys)
+    if keys or (queries or 1) != 1:   # (what one of them alone stands for is not agreed)
+        raise ValueError(f"mscale = {queries} and mscale_all_dim = {keys} go together")
+    return size(1.0)
+
+
 def rotary_cos_sin(rotary_dim: int, max_position: int, base: float = 10000.0, scaling: dict | None = None,
                    device: torch.device | str | None = None) -> torch.Tensor:
     """float32 (max_position, rotary_dim): a position's cosines, then its sines.  The angles are formed in 64 bits, as those of far
-    positions need; for yarn both are multiplied by `attention_factor`, 0.1 ln(factor) + 1 if the configuration does not say."""
+    positions need; for yarn both are multiplied by `attention_factor`, and if the configuration does not say that, by
+    (0.1 mscale ln(factor) + 1) / (0.1 mscale_all_dim ln(factor) + 1), or 0.1 ln(factor) + 1 without those."""
     angles = torch.arange(max_position, dtype=torch.float64)[:, None] * rotary_rates(rotary_dim, base, scaling)
-    size = 1.0
-    if scaling is not None and scaling["rope_type"] == "yarn":
-        size = scaling.get("attention_factor") or (0.1 * math.log(scaling["factor"]) + 1 if scaling["factor"] > 1 else 1.0)
+    size = _yarn_size(scaling) if scaling is not None and scaling["rope_type"] == "yarn" else 1.0
     return (torch.cat([angles.cos(), angles.sin()], dim=1) * size).float().to(device)
