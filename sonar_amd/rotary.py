@@ -15,7 +15,8 @@ def rotary_rates(rotary_dim: int, base: float = 10000.0, scaling: dict | None = 
       llama3   by wavelength: those longer than original_max_position_embeddings / low_freq_factor are divided by `factor`, those
                shorter than it / high_freq_factor stay, a straight line of the inverse wavelength between
       yarn     by turns within original_max_position_embeddings: pairs of `beta_fast` (32) turns or more stay, of `beta_slow` (1) or
-               fewer are divided by `factor`, a straight line of the pair's number between"""
+               fewer are divided by `factor`, a straight line of the pair's number between, whose ends are whole pairs unless
+               `truncate` is false"""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim = {rotary_dim} must be even and positive")
     rates = float(base) ** -(torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
@@ -34,8 +35,10 @@ def rotary_rates(rotary_dim: int, base: float = 10000.0, scaling: dict | None = 
     elif kind == "yarn":
         # the pair that turns n times within the original context
         pair = lambda n: rotary_dim * math.log(original / (2 * math.pi * n)) / (2 * math.log(base))  # noqa: E731
-        first = max(math.floor(pair(scaling.get("beta_fast", 32))), 0)
-        last = min(math.ceil(pair(scaling.get("beta_slow", 1))), rotary_dim - 1)
+        first, last = pair(scaling.get("beta_fast", 32)), pair(scaling.get("beta_slow", 1))
+        if scaling.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rotary_dim - 1)
         stay = 1 - ((torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0, 1)
     else:
         raise ValueError(f"rope_type = {kind!r} is not linear, llama3 or yarn")

@@ -28,3 +28,22 @@ def test_size_of_yarn_tables(more, want):
 def test_one_of_two_sizes_is_refused(more):
     with pytest.raises(ValueError, match="mscale"):
         size_of(**more)
+
+
+@pytest.mark.parametrize("truncate,rates", [
+    # pairs 8, 9 and 17, 18 lie beside the ends of the line, 8.09 and 17.40; whole ends are 8 and 18
+    (False, {0: 1.0, 7: 0.07374456524848938, 8: 0.05081327259540558, 9: 0.031705696135759354, 12: 0.006794959306716919,
+             16: 0.0004564839182421565, 17: 0.00012931869423482567, 18: 3.830881178146228e-05, 31: 3.023511396804679e-07}),
+    (True, {7: 150000.0 ** (-14 / 64), 8: 150000.0 ** (-16 / 64), 9: 150000.0 ** (-18 / 64) * (0.9 + 0.1 / 32),
+            17: 150000.0 ** (-34 / 64) * (0.1 + 0.9 / 32), 18: 150000.0 ** (-36 / 64) / 32})])
+def test_ends_of_the_yarn_line(truncate, rates):
+    """The numbers for ends that are not rounded are another implementation's, in float32 (each off by a few steps of 2^-23)."""
+    got = rotary_rates(64, 150000.0, {"rope_type": "yarn", "factor": 32.0, "original_max_position_embeddings": 4096, "truncate": truncate})
+    for pair, want in rates.items():
+        assert abs(got[pair] - want) <= 4 * 2.0 ** -23 * want, pair
+    ends = [64 * math.log(4096 / (2 * math.pi * turns)) / (2 * math.log(150000.0)) for turns in (32, 1)]
+    if not truncate:   # and by the definition
+        stay = [1 - min(max((i - ends[0]) / (ends[1] - ends[0]), 0), 1) for i in range(32)]
+        want = [150000.0 ** (-2 * i / 64) * (s + (1 - s) / 32) for i, s in enumerate(stay)]
+        assert torch.allclose(got, torch.tensor(want, dtype=torch.float64), rtol=1e-13)
+    assert 8 < ends[0] < 9 and 17 < ends[1] < 18
