@@ -47,3 +47,29 @@ def test_ends_of_the_yarn_line(truncate, rates):
         want = [150000.0 ** (-2 * i / 64) * (s + (1 - s) / 32) for i, s in enumerate(stay)]
         assert torch.allclose(got, torch.tensor(want, dtype=torch.float64), rtol=1e-13)
     assert 8 < ends[0] < 9 and 17 < ends[1] < 18
+
+
+LINEAR = {"rope_type": "linear", "factor": 4.0}
+
+
+@pytest.mark.parametrize("scaling,message", [
+    ({**YARN, "beta": 3}, "beta"), ({**LINEAR, "truncate": False}, "truncate"), ({"rope_type": "default", "mrope_section": [8, 12, 12]}, "mrope_section"),
+    ({"rope_type": "linear"}, "factor"), ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0}, "original_max"),
+    ({"rope_type": "longrope", "short_factor": [1.0]}, "longrope"), ({"factor": 4.0}, "rope_type"), ({**LINEAR, "type": "yarn"}, "type"),
+    ({**LINEAR, "rope_theta": 5e5}, "rope_theta"), ({**LINEAR, "factor": 0.0}, "factor")])
+def test_what_is_not_known_is_refused(scaling, message):
+    for table in (lambda: rotary_rates(64, scaling=scaling), lambda: rotary_cos_sin(64, 3, scaling=scaling)):
+        with pytest.raises(ValueError, match=message):
+            table()
+
+
+@pytest.mark.parametrize("scaling", [
+    {**LINEAR, "type": "linear"}, {"type": "linear", "factor": 4.0}, {**LINEAR, "rope_theta": 10000.0}, {**LINEAR, "partial_rotary_factor": 0.5},
+    {**LINEAR, "original_max_position_embeddings": 4096}, {**LINEAR, "truncate": None}])
+def test_what_changes_no_table(scaling):
+    assert torch.equal(rotary_cos_sin(64, 9, scaling=scaling), rotary_cos_sin(64, 9, scaling=LINEAR))
+
+
+def test_numbers_that_are_none_are_absent():
+    none = dict.fromkeys(("beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"))
+    assert torch.equal(rotary_cos_sin(64, 9, scaling={**YARN, **none}), rotary_cos_sin(64, 9, scaling=YARN))
