@@ -60,7 +60,8 @@ int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  * starts[i + 1] - 1, are its last ones: query j has the position seq_lens[i] - (starts[i + 1] - starts[i]) + j.  Query head h
  * reads kv head h / (heads / kv_heads).
  *   s = scale * (q . k);  cap > 0: s = cap * tanh(s / cap);  slopes: s -= slopes[h] * |query position - key position|
- *   out = sum over the keys that the query sees of softmax(s) * v, rounded once; a query that sees none gives zeros
+ *   out = sum over the keys that the query sees of softmax(s) * v, rounded once; a query that sees none gives zeros, one all of
+ *   whose scores are -infinity, or one of them NaN or +infinity, NaN
  * A query at position t sees key p < seq_lens[i] where
  *   causal: p <= t, and with window > 0 also p > t - window (the last `window` keys, its own among them);
  *   tree_mask: p lies before the sequence's queries, or is its query c (p = seq_lens[i] - queries + c) and bit c % 64 of

@@ -46,10 +46,6 @@ __device__ __forceinline__ Score score_of(const AttentionParams& p, int kv_head,
   return s;
 }
 
-__device__ __forceinline__ float value_scale(const AttentionParams& p, int kv_head) {
-  return p.v.scale == nullptr ? 1.0f : p.v.scale[p.v.scale_heads ? kv_head : 0];
-}
-
 template <typename T>
 using Four = T __attribute__((ext_vector_type(4)));
 template <typename T>
@@ -458,7 +454,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     __syncthreads();
     char* const mine = lds + wave * 32 * kPitch;
     constexpr int kPieces = kPitch / 16, kSwap = kPieces < 16 ? kPieces - 1 : 15;
-    const float by = sum == 0.0f ? 0.0f : value_scale(p, kv_head) / sum;
+    const float by = row_scale(p, r, t, kv_head, sum);
 #pragma unroll
     for (int c = 0; c < kColumns; ++c)
 #pragma unroll
@@ -697,7 +693,7 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
     if (flags[0] & 1) total = __builtin_nanf("");
     const long at = ((long)split * p.tokens + token) * p.heads + head;
     if (parts > 1 && threadIdx.x % 16 == 0) p.part_ml[at] = make_float2(all, total);
-    const float scale = total == 0.0f ? 0.0f : value_scale(p, kv_head) / total;
+    const float scale = row_scale(p, r, row / p.group, kv_head, total);
 #pragma unroll
     for (int j = 0; j < DP / 64; ++j) {
       const int d = 64 * j + 4 * (threadIdx.x % 16);
@@ -826,7 +822,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_
     }
   }
   if (lane >= LANES || d >= p.dim) return;
-  const float scale = sum == 0.0f ? 0.0f : value_scale(p, kv_head) / sum;
+  const float scale = row_scale(p, r, token - r.token, kv_head, sum);
   *reinterpret_cast<Four<T>*>((T*)p.out + token * p.out_token + head * p.out_head + d) =
       four<T>(out[0] * scale, out[1] * scale, out[2] * scale, out[3] * scale);
 }

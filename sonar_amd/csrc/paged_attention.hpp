@@ -178,6 +178,27 @@ struct Sight {
   }
 };
 
+// Whether query `t` of the sequence sees any key.
+__device__ __forceinline__ bool sees_any(const AttentionParams& p, const RowBlock& r, int t) {
+  if (p.tree == nullptr) {
+    int low, high;
+    keys_seen(p, r, t, t, low, high);
+    return high > low;
+  }
+  uint64_t seen = r.past > 0 && r.len > 0;
+  const uint64_t* words = p.tree + (long)(r.token + t) * p.tree_words;   // (of queries whose keys are 0 to len - 1)
+  for (int w = 0; w < p.tree_words && 64 * w < r.len - r.past; ++w)
+    seen |= words[w] & Sight::below(r.len - r.past - 64 * w) & ~Sight::below(-r.past - 64 * w);
+  return seen != 0;
+}
+
+// What a row's sums are multiplied by.  A sum of 0 is that of a query without keys, whose result is 0, or of one all of whose scores
+// are -infinity, whose result is NaN: the largest of finite scores has a weight of 1 at least.
+__device__ __forceinline__ float row_scale(const AttentionParams& p, const RowBlock& r, int t, int kv_head, float sum) {
+  if (sum == 0.0f) return sees_any(p, r, t) ? __builtin_nanf("") : 0.0f;
+  return (p.v.scale == nullptr ? 1.0f : p.v.scale[p.v.scale_heads ? kv_head : 0]) / sum;
+}
+
 // A score where bit `i` of `seen` is set, else -infinity.
 __device__ __forceinline__ float shown(float score, uint32_t seen, int i) {
   const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)seen, i, 1);
