@@ -67,8 +67,8 @@ int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  *   tree_mask: p lies before the sequence's queries, or is its query c (p = seq_lens[i] - queries + c) and bit c % 64 of
  *   tree_mask[token][c / 64] is set, c < 64 * tree_words.  Neither slopes nor a window go with a tree mask, nor a window with causal = 0.
  * What lies in masked places, NaN included, does not reach the result.  Pages that no query sees are not read, and their
- * numbers not looked at; a number outside [0, pages) among the others makes the results that read it NaN.  seq_lens are taken as at most
- * table_pages * page_size.  Tokens from starts[seqs] on get zeros where clear_rest, else are left as they are.
+ * numbers not looked at; a number outside [0, pages) among the others makes the results of the queries that see a key of that page NaN,
+ * and no others.  seq_lens are taken as at most table_pages * page_size.  Tokens from starts[seqs] on get zeros where clear_rest, else are left as they are.
  *   q, out      dtype (SONAR_DTYPE_F16 / _BF16) (token, head, d) with strides; q 16-byte aligned, its strides multiples of 8; out 8-byte
  *               aligned, its strides multiples of 4; out does not overlap the inputs
  *   caches      of dtype or SONAR_CACHE_FP8; 16-byte aligned, strides multiples of 16 bytes; page_size slots a page; 64 GiB at most

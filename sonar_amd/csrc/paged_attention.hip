@@ -91,6 +91,38 @@ __device__ __forceinline__ void add_specials(const AttentionParams& p, const Row
     }
 }
 
+// NaN for the rows of the block that see a key whose page is none: `bad` pages were taken for the first one so far.  A thread a row; the
+// keys are those of tiles [first, last), whose results this workgroup has written.
+template <typename T>
+__device__ __forceinline__ void spoil_rows(const AttentionParams& p, const RowBlock& r, int kv_head, int split, int parts, int first, int last,
+                                           int rows_end) {
+  __threadfence();
+  __syncthreads();
+  const bool bounded = p.causal && p.tree == nullptr;
+  const int row = r.first + (int)threadIdx.x;
+  if (row >= rows_end) return;
+  const int t = row / p.group, end = min(last * kTile, r.len);
+  const Sight sight{r.past + t, r.len, r.past, bounded && p.window > 0 ? r.past + t - p.window + 1 : 0,
+                    p.tree == nullptr ? nullptr : p.tree + (long)(r.token + t) * p.tree_words, p.tree_words, p.causal};
+  bool spoiled = false;
+  for (int tile = first; tile < last && !spoiled; ++tile) {
+    const uint64_t seen = sight.of(tile * kTile);
+    for (int key = tile * kTile; key < min(tile * kTile + kTile, end) && seen != 0;) {
+      const int at = page_of(p, key), next = (int)min((long)(at + 1) * p.page_size, (long)(tile * kTile + kTile));
+      const bool known = (uint32_t)p.table[(long)r.seq * p.table_stride + at] < (uint32_t)p.pages;
+      spoiled |= !known && (seen & Sight::below(next - tile * kTile) & ~Sight::below(key - tile * kTile)) != 0;
+      key = next;
+    }
+  }
+  if (!spoiled) return;
+  if (parts > 1) {
+    p.part_ml[part_at(p, r, split, kv_head, row)].y = __builtin_nanf("");
+  } else {
+    T* to = (T*)p.out + (long)(r.token + t) * p.out_token + (kv_head * p.group + row % p.group) * p.out_head;
+    for (int d = 0; d < p.dim; ++d) to[d] = (T)__builtin_nanf("");
+  }
+}
+
 // ---------------------------------------------------------------- many rows
 // A workgroup takes 32 rows of a kv head for each of its WAVES wavefronts, and walks the keys in tiles of 64 that they share through
 // LDS, two tiles there: while one is worked on, the next one is on its way.  Bound by the matrix pipes and the vector units together:
@@ -436,7 +468,6 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   __syncthreads();
   const int found = flags[0];
   sum = joined<true>(sum, [](float a, float b) { return a + b; });
-  if (found & 1) sum = __builtin_nanf("");
   if (parts > 1) {
     if (row < r.rows) {
       const long at = part_at(p, r, split, kv_head, row);
@@ -476,6 +507,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
   }
   if (found & 2)
     add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last, min(r.rows, r.first + kRows), block_full_low, block_full_high);
+  if (found & 1) spoil_rows<T>(p, r, kv_head, split, parts, first_tile, last, min(r.rows, r.first + kRows));
 }
 
 // ---------------------------------------------------------------- few rows
@@ -690,7 +722,6 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
       by[w] = __builtin_amdgcn_exp2f(sums[w * 16 + in_tile].x - less);
       total = __builtin_fmaf(by[w], sums[w * 16 + in_tile].y, total);
     }
-    if (flags[0] & 1) total = __builtin_nanf("");
     const long at = ((long)split * p.tokens + token) * p.heads + head;
     if (parts > 1 && threadIdx.x % 16 == 0) p.part_ml[at] = make_float2(all, total);
     const float scale = row_scale(p, r, row / p.group, kv_head, total);
@@ -712,6 +743,7 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
   }
   if (flags[0] & 2)
     add_specials<T, FP8>(p, r, kv_head, split, parts, first_tile, last_tile, min(r.rows, r.first + 16), full_low, full_high);
+  if (flags[0] & 1) spoil_rows<T>(p, r, kv_head, split, parts, first_tile, last_tile, min(r.rows, r.first + 16));
 }
 
 // ---------------------------------------------------------------- the parts of a split joined

@@ -384,7 +384,7 @@ def paged_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: t
     bit c % 64 of word c // 64 is query c of the sequence (a draft's own bit among them); it takes the place of `causal` and goes with
     neither window nor slopes.  A query that sees no key gives zeros, as do tokens behind the last sequence; with `out`, those are left as
     they are.  One that sees a score of +infinity or NaN, or none but -infinity, gives NaN.  NaNs and infinities in what a query does not see do not reach it.  Pages that no query sees are not read; a
-    page number outside the cache among the others makes the results NaN.
+    page number outside the cache among the others makes the results of the queries that see a key of it NaN.
 
     max_seq_len: the longest sequence, if the caller knows: how far the keys may be split over workgroups is chosen for it, and for
     all of the block table without it (a captured call whose lengths change does without); results are right, if not the same bits, for
