@@ -3,7 +3,9 @@
 // One pass over the keys with a running maximum m and sum l: a tile's scores s give p = 2^(s log2 e - m), out = out + p v,
 // l = l + sum p, and where a score is above m by more than 8 (in powers of two) m rises to it, out and l shrinking with it.
 // (Rising only then leaves p up to 2^8, which p's type and the sums hold as precisely.)  Products on the matrix
-// instructions, sums in fp32; p is rounded to the type of v for its product, by at most half a step of each.
+// instructions, sums in fp32; p is rounded to 16 bits for its product, by at most half a step of each.  For fp16 p is formed 2^7 times
+// larger, the sums too: only what is below 2^-21 of the largest is then subnormal, and off by up to 2^-32 of it, so that 2^20 such
+// keys together are off by less than half a step of the largest |v|.
 //
 // Both products are formed turned, k q^T and v^T p^T: a lane then holds scores of one query only, so that m, l and what
 // out shrinks by are a lane's own numbers, and the scores lie where the second product takes them as its operand.  The keys of
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
       weights[h][e / 8][e % 8] = both[0], weights[h][e / 8][e % 8 + 1] = both[1];
       sum = E::add(both, sum);
     };
-    const float less = most == -kInfinity ? 0.0f : most;
+    const float less = most == -kInfinity ? 0.0f : most - E::kRaise;
     float last_weight = 0.0f;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(WAVES * 64, DP == 64 && !FP8 ? 3 : DP <= 128 ? 2 : 
     if (SCORES == kPlain) top *= score.by;
     if (__any(top > most + 8.0f)) {
       const float now = fmaxf(most, joined<true>(top, [](float a, float b) { return fmaxf(a, b); }));
-      const float less = now == -kInfinity ? 0.0f : now, by = __builtin_amdgcn_exp2f(most - less);
+      const float less = now == -kInfinity ? 0.0f : now - E::kRaise, by = now == -kInfinity ? 1.0f : __builtin_amdgcn_exp2f(most - now);
       most = now, sum = before * by;
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) out[c] *= by;
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(kFew * 64, few_waves(DP, FP8)) void attention_few_k
 #pragma unroll
       for (int c = 0; c < kColumns; ++c) out[c] *= by;
     }
-    const float less = most == -kInfinity ? 0.0f : most;
+    const float less = most == -kInfinity ? 0.0f : most - E::kRaise;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = s[i / 4][i % 4];

@@ -193,7 +193,7 @@ __device__ __forceinline__ bool sees_any(const AttentionParams& p, const RowBloc
 }
 
 // What a row's sums are multiplied by.  A sum of 0 is that of a query without keys, whose result is 0, or of one all of whose scores
-// are -infinity, whose result is NaN: the largest of finite scores has a weight of 1 at least.
+// are -infinity, whose result is NaN: the largest of finite scores has a weight of 1 or more.
 __device__ __forceinline__ float row_scale(const AttentionParams& p, const RowBlock& r, int t, int kv_head, float sum) {
   if (sum == 0.0f) return sees_any(p, r, t) ? __builtin_nanf("") : 0.0f;
   return (p.v.scale == nullptr ? 1.0f : p.v.scale[p.v.scale_heads ? kv_head : 0]) / sum;
@@ -223,6 +223,7 @@ template <>
 struct Element<__bf16> {
   typedef bf16x8_t eight;
   static constexpr uint16_t kExponent = 0x7f80;
+  static constexpr float kRaise = 0.0f;   // weights are formed larger by 2 to this
   __device__ __forceinline__ static floatx16_t mfma32(eight a, eight b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -244,6 +245,7 @@ template <>
 struct Element<_Float16> {
   typedef half8_t eight;
   static constexpr uint16_t kExponent = 0x7c00;
+  static constexpr float kRaise = 7.0f;   // so that they use the whole range, up to 2^15
   __device__ __forceinline__ static floatx16_t mfma32(eight a, eight b, floatx16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
