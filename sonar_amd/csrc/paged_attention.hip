@@ -866,6 +866,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void attention_join_
 // (8192 tokens of 32 heads of 64: 353 us, with 128 rows 344; of 128: 574 and 590).
 constexpr bool eight_waves(int dp) { return dp == 128; }
 
+// Bytes of scratch memory at most: a call must not fail for parts that it can do without, and a captured one holds them.  What more
+// parts would be chosen for gains little by them: 64 sequences of 33 tokens with 131072 keys 10.0 ms with 7 parts and with 16; 512 of up to
+// 17 tokens, one with 100000 keys, 2.11 ms with 3 and 2.03 with 4; 1024 of up to 17 in heads of 256 4.2 ms with none and 4.8 with 4.
+constexpr int64_t kMostScratch = 256 << 20;
+
 struct Plan {
   int rows;   // of a block: 16 in the form for few rows, 128 and 256 in that for many
   long blocks, splits, split_tiles, tails;
@@ -880,6 +885,8 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
   const int64_t keys = std::max<int64_t>(window > 0 ? std::min(max_seq_len, window + queries) : max_seq_len, 1), longest = (keys + kTile - 1) / kTile;
   const int dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
   plan.longest = (int)keys;
+  const int64_t row_bytes = head_dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2);
+  auto parts_of = [&](int64_t rows) { return std::max<int64_t>((kMostScratch - 16) / (rows * row_bytes), 1); };   // at most
   auto groups_of = [&](int rows) {
     return std::max<int64_t>((tokens * group + rows - 1) / rows, std::min(seqs, tokens)) * kv_heads;
   };
@@ -899,6 +906,7 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     plan.split_tiles = 2;
     plan.splits = std::min<int64_t>(std::max<int64_t>(4096 / groups, 4), 256);
     plan.splits = std::min<int64_t>(plan.splits, (longest + few_tiles((int)longest, plan.few_share) - 1) / few_tiles((int)longest, plan.few_share));
+    plan.splits = std::min(plan.splits, parts_of(tokens * heads));
   } else {
     // Parts, by what a compute unit's workgroups take for a tile (us, measured: alone, and as many as it holds together) and what
     // writing and reading the parts takes.
@@ -910,7 +918,7 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     };
     double best = 0.0;
     int64_t parts = 1;
-    for (int64_t n = 1; n <= 64 && n <= tiles; ++n) {
+    for (int64_t n = 1, most = std::min<int64_t>(parts_of(tokens * heads), 64); n <= most && n <= tiles; ++n) {
       const double bytes = 8.0 * (double)(n * tokens * heads * head_dim);
       const double time = (double)((tiles + n - 1) / n) * of_tile((groups * n + 255) / 256) + (n > 1 ? 5.0 + 0.3 * (double)n + bytes / 4e6 : 0.0);
       if (n == 1 || time < 0.97 * best) best = time, parts = n;
@@ -922,7 +930,7 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
   // a workgroup for all of them would end long after the others (one token with 100000 keys beside 16 prompts of 1000: 1816 us, so
   // 392; parts of 4 tiles at least: 9 sequences with a window of 1024 92 us, 2 tiles 95, 8 101, unsplit 108).
   if (!few && plan.splits == 1 && seqs > 1 && queries * group > kTail && 2 * queries < max_seq_len && seqs * kv_heads <= 8192)
-    plan.tails = std::min<int64_t>(std::max<int64_t>(2048 / (seqs * kv_heads), 4), (longest + 3) / 4);
+    plan.tails = std::min({std::max<int64_t>(2048 / (seqs * kv_heads), 4), (longest + 3) / 4, parts_of(seqs * kv_heads * kTail)});
   if (plan.tails < 2) plan.tails = 0;
   if (plan.splits > 1 || plan.tails > 0) {
     const int64_t rows = plan.tails > 0 ? plan.tails * seqs * kv_heads * kTail : plan.splits * tokens * heads;
