@@ -74,7 +74,8 @@ int sonar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  *   caches      of dtype or SONAR_CACHE_FP8; 16-byte aligned, strides multiples of 16 bytes; page_size slots a page; 64 GiB at most
  *   block_table int32[seqs][table_stride], table_pages of a row in use;  seq_lens int32[seqs];  starts int32[seqs + 1], rising, from 0
  *   slopes      float[heads] or NULL;  tree_mask int64[tokens][tree_words] or NULL
- *   max_seq_len what the split of the keys is chosen for; longer sequences are right too, and much shorter ones about as fast
+ *   max_seq_len what the split of the keys is chosen for; longer sequences are right too, and much shorter ones, of up to 1024
+ *               sequences, nearly as fast
  *   scratch     device memory, 16-byte aligned, of sonar_paged_attention_scratch_bytes(...) bytes (0 to 256 MiB); calls that overlap in
  *               time need scratches of their own
  * head_dim a multiple of 16, at most 256; scale, and cap if not 0, from 1e-30 to 1e30; tokens * heads below 2^31, table_pages * page_size below 2^31 - 1024. */

@@ -874,8 +874,9 @@ constexpr int64_t kMostScratch = 256 << 20;
 struct Plan {
   int rows;   // of a block: 16 in the form for few rows, 128 and 256 in that for many
   long blocks, splits, split_tiles, tails;
-  int longest;
+  int longest, queries;
   float few_share;
+  PartsCost cost;
   size_t ml_bytes, o_bytes;
 };
 
@@ -908,22 +909,19 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
     plan.splits = std::min<int64_t>(plan.splits, (longest + few_tiles((int)longest, plan.few_share) - 1) / few_tiles((int)longest, plan.few_share));
     plan.splits = std::min(plan.splits, parts_of(tokens * heads));
   } else {
-    // Parts, by what a compute unit's workgroups take for a tile (us, measured: alone, and as many as it holds together) and what
-    // writing and reading the parts takes.
-    const int64_t tiles = (keys - std::min(queries, keys) / 2 + kTile - 1) / kTile;
-    auto of_tile = [&](int64_t workgroups) {   // of one compute unit
-      if (dp == 256 || plan.rows == 256) return (double)workgroups * (dp == 256 ? 2.6 : 2.2);
-      if (dp == 64) return (double)(workgroups / 3) * 1.3 + (workgroups % 3 == 0 ? 0.0 : workgroups % 3 == 1 ? 0.9 : 1.1);
-      return (double)(workgroups / 2) * 2.1 + (workgroups % 2 == 0 ? 0.0 : queries * group > 64 ? 1.9 : 1.35);
-    };
-    double best = 0.0;
-    int64_t parts = 1;
-    for (int64_t n = 1, most = std::min<int64_t>(parts_of(tokens * heads), 64); n <= most && n <= tiles; ++n) {
-      const double bytes = 8.0 * (double)(n * tokens * heads * head_dim);
-      const double time = (double)((tiles + n - 1) / n) * of_tile((groups * n + 255) / 256) + (n > 1 ? 5.0 + 0.3 * (double)n + bytes / 4e6 : 0.0);
-      if (n == 1 || time < 0.97 * best) best = time, parts = n;
-    }
-    plan.splits = parts, plan.split_tiles = std::min<int64_t>((longest + parts - 1) / parts, 4);
+    // (for a tile: alone, and as many workgroups as a compute unit holds together)
+    plan.cost = dp == 256 || plan.rows == 256 ? PartsCost{0, 1, dp == 256 ? 2.6f : 2.2f, 0.0f, 0.0f, 0.0f}
+                : dp == 64                    ? PartsCost{0, 3, 1.3f, 0.9f, 1.1f, 0.0f}
+                                              : PartsCost{0, 2, 2.1f, queries * group > 64 ? 1.9f : 1.35f, 0.0f, 0.0f};
+    plan.cost.groups = (int)std::min<int64_t>(groups, 1 << 24);
+    plan.cost.part = 0.3f + (float)(8.0 * (double)(tokens * heads * head_dim) / 4e6);
+    plan.queries = (int)queries;
+    const int tiles = mean_tiles((int)keys, plan.queries), most = (int)std::min<int64_t>({parts_of(tokens * heads), 64, tiles});
+    float best = plan.cost.of(tiles, 1);
+    plan.splits = 1;
+    for (int n = 2; n <= most; ++n)
+      if (plan.cost.of(tiles, n) < kWorth * best) best = plan.cost.of(tiles, n), plan.splits = n;
+    plan.split_tiles = std::min<int64_t>((longest + plan.splits - 1) / plan.splits, 4);
   }
   if (tokens * heads >= 1LL << 24 || plan.blocks * kv_heads * plan.splits >= 1LL << 24) plan.splits = 1;   // (2^32 threads are a launch's most)
   // Many rows, but not of each sequence: single tokens beside prompts.  Their keys are split, though the rest has workgroups enough, as
@@ -1072,6 +1070,7 @@ extern "C" int sonar_paged_attention(const void* q, int64_t q_token_stride, int6
   p.page_size = (int)page_size, p.pages = (int)pages, p.table_pages = (int)table_pages;
   p.tokens = (int)tokens, p.seqs = (int)seqs, p.heads = (int)heads, p.kv_heads = (int)kv_heads, p.group = (int)(heads / kv_heads);
   p.dim = (int)head_dim, p.rows = plan.rows, p.blocks = (int)plan.blocks, p.splits = (int)plan.splits, p.split_tiles = (int)plan.split_tiles, p.tails = (int)plan.tails, p.longest = plan.longest, p.few_share = plan.few_share;
+  p.queries = plan.queries, p.cost = plan.cost;
   p.by_dies = plan.rows == 16;
   const bool fp8 = cache_dtype == SONAR_CACHE_FP8;
   hipStream_t st = (hipStream_t)stream;

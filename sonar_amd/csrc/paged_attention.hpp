@@ -25,6 +25,25 @@ struct CachePages {
   int scale_heads;         // scale holds a number for each kv head
 };
 
+// What parts of the keys cost in the form for many rows (us, measured): what a compute unit's workgroups take for a tile, `period` of
+// them together `whole`, one or two beside those `one` and `two`; and each part, to be written, read and joined.
+struct PartsCost {
+  int groups, period;   // workgroups without parts
+  float whole, one, two, part;
+  __host__ __device__ __forceinline__ float of(int tiles, int n) const {
+#pragma clang fp contract(off)
+    const int workgroups = (groups * n + 255) / 256, rest = workgroups % period;   // of one compute unit
+    const float tile = (float)(workgroups / period) * whole + (rest == 0 ? 0.0f : rest == 1 ? one : two);
+    return (float)((tiles + n - 1) / n) * tile + (n > 1 ? 5.0f + part * (float)n : 0.0f);
+  }
+};
+// Tiles of a sequence of `keys` keys, the last `queries` of which see them: on average.
+__host__ __device__ __forceinline__ int mean_tiles(int keys, int queries) {
+  return (int)(((uint32_t)keys - (uint32_t)(queries < keys ? queries : keys) / 2 + kTile - 1) / kTile);
+}
+// More parts are taken where they are cheaper by 3 %.
+constexpr float kWorth = 0.97f;
+
 struct AttentionParams {
   const char* q;
   long q_token, q_head;   // strides in elements
@@ -45,6 +64,8 @@ struct AttentionParams {
   int rows, blocks, splits, split_tiles;   // rows of a block, blocks of rows; at most `splits` parts of the keys, of `split_tiles` tiles at least
   int tails;                               // not 0: at most so many parts of the sequences' last rows, where those are no more than kTail
   int longest;                             // keys of a sequence at most, as far as the host knows
+  int queries;                             // of a sequence, on average
+  PartsCost cost;
   float few_share;                         // not 0: parts of few_tiles() tiles at least
   bool causal, clear_rest, by_dies;
 };
@@ -76,10 +97,18 @@ __device__ __forceinline__ int start_of(const AttentionParams& p, int i) { retur
 
 // The last sequence i of [0, seqs] with number(i, its start) <= b, for numbers that rise from 0, and its sizes; its first row is left
 // to the caller.  A wavefront looks at 64 places at a time; in the last round the lanes have the sizes too, so that a batch of up
-// to 62 sequences takes one trip to memory.
+// to 62 sequences takes one trip to memory.  Where parts are chosen by the longest length, those of up to 1024 sequences are read on the
+// way (from 1025 on there are workgroups enough whatever the parts are).
 template <typename F>
 __device__ __forceinline__ RowBlock sequence_of(const AttentionParams& p, int b, F number) {
   const int lane = threadIdx.x & 63;
+  const bool by_longest = p.splits > 1 && p.few_share == 0.0f && p.seqs <= 1024;
+  int lens[4] = {};   // this lane's (some twice), the last one the largest of those from there on
+  if (by_longest && p.seqs > 62) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lens[j] = p.lens[min(lane + 64 * j, p.seqs - 1)];
+    for (int i = lane + 256; i < p.seqs; i += 64) lens[3] = max(lens[3], p.lens[i]);
+  }
   int low = 0, count = p.seqs + 1;
   while (count > 63) {
     const int step = (count + 63) / 64, i = low + min(lane * step, count - 1);
@@ -99,7 +128,10 @@ __device__ __forceinline__ RowBlock sequence_of(const AttentionParams& p, int b,
   r.len = (int)min((long)max(of_lane(len, found), 0), (long)p.table_pages * p.page_size);
   r.past = r.len - (end - r.token);
   r.longest = p.longest;
-  if (p.splits > 1 && p.few_share == 0.0f && p.seqs <= 62) r.longest = min(over_wave(len, 0, [](int a, int b) { return max(a, b); }), p.longest);   // (all lengths are here)
+  if (by_longest) {
+    auto larger = [](int a, int b) { return max(a, b); };
+    r.longest = min(over_wave(p.seqs <= 62 ? len : max(max(lens[0], lens[1]), max(lens[2], lens[3])), 0, larger), p.longest);
+  }
   return r;
 }
 
@@ -140,13 +172,34 @@ __host__ __device__ __forceinline__ int few_tiles(int tiles, float share) {
   return for_many < for_one ? for_one : for_many > 8 ? 8 : for_many;
 }
 
+// Tiles of a part at least in the form for many rows.  Where the longest sequence is shorter than the host knew, the host's choice of
+// parts is made anew: each lane prices a number of parts, of which there are no more than the host's.  (64 sequences of 800 to 4096 keys of
+// one kv head that might have had 131072 take 28 us, with parts chosen for those 82; 32 of 33 tokens with 4096 keys 214 and 287.)
+__device__ __forceinline__ int many_tiles(const AttentionParams& p, const RowBlock& r) {
+  const int longest = (r.longest + kTile - 1) / kTile;
+  int parts = p.splits;
+  if (parts > 1 && longest < (p.longest + kTile - 1) / kTile) {
+    const int tiles = max(mean_tiles(r.longest, p.queries), 1), lane = threadIdx.x & 63;
+    const float time = p.cost.of(tiles, lane + 1);
+    const int most = min(p.splits, tiles);
+    float best = of_lane(time, 0);
+    parts = 1;
+    for (;;) {
+      const uint64_t better = __ballot(lane >= parts && lane < most && time < kWorth * best);
+      if (better == 0) break;
+      parts = __builtin_ctzll(better) + 1;
+      best = of_lane(time, parts - 1);
+    }
+  }
+  return max(p.split_tiles, (longest + parts - 1) / parts);
+}
+
 // The part of the tiles [first, last) of a block that split s takes; false where there is none.  Sets how many parts there are.  Of how many
-// tiles a part is, the lengths say that there are, as the caller may not know them: 64 sequences of 800 to 4096 keys in 8-bit codes take
-// 91 us also where they might have had 131072, by parts chosen for those 344.
+// tiles a part is, the lengths say that there are.
 __device__ __forceinline__ bool split_of(const AttentionParams& p, const RowBlock& r, int s, int& first, int& last, int& parts) {
   const int tiles = last - first;
   // few rows: parts of each sequence's own size; many: of one size for all, so that what is short is not cut for nothing
-  const int least = p.tails > 0 ? (is_tail(r) ? 4 : max(tiles, 1)) : p.few_share > 0.0f ? few_tiles(tiles, p.few_share) : max(p.split_tiles, ((r.longest + kTile - 1) / kTile + p.splits - 1) / p.splits);
+  const int least = p.tails > 0 ? (is_tail(r) ? 4 : max(tiles, 1)) : p.few_share > 0.0f ? few_tiles(tiles, p.few_share) : many_tiles(p, r);
   const int most = p.tails > 0 ? p.tails : p.splits, each = max(least, (tiles + most - 1) / most);
   parts = max((tiles + each - 1) / each, 1);
   first += s * each;
