@@ -927,6 +927,8 @@ Plan plan_of(int64_t tokens, int64_t seqs, int64_t heads, int64_t kv_heads, int6
   // Many rows, but not of each sequence: single tokens beside prompts.  Their keys are split, though the rest has workgroups enough, as
   // a workgroup for all of them would end long after the others (one token with 100000 keys beside 16 prompts of 1000: 1816 us, so
   // 392; parts of 4 tiles at least: 9 sequences with a window of 1024 92 us, 2 tiles 95, 8 101, unsplit 108).
+  // Not in batches of single tokens alone: 63 sequences of up to 4096 keys and one of 100000 take 1904 us so, 668 with such parts, but 64 of up
+  // to 1000 that might have had 131072 34 and 55.
   if (!few && plan.splits == 1 && seqs > 1 && queries * group > kTail && 2 * queries < max_seq_len && seqs * kv_heads <= 8192)
     plan.tails = std::min({std::max<int64_t>(2048 / (seqs * kv_heads), 4), (longest + 3) / 4, parts_of(seqs * kv_heads * kTail)});
   if (plan.tails < 2) plan.tails = 0;
